@@ -19,13 +19,15 @@ int launch_failed(cudaError_t e) {
   return TT_ATTN_ERR_LAUNCH;
 }
 
-// Equivalent of the reference's CudaDeviceGuard (src/Utils/CUDAUtils.h:100-113).
+// Equivalent of the reference's CudaDeviceGuard (src/Utils/CUDAUtils.h:100-113).  The device is set even where it is the
+// current one: in a thread that has made no CUDA call yet (one of an autograd engine's, say) that makes the context current, without
+// which the driver encodes no tensor maps.
 struct DeviceGuard {
   int prev = -1;
   bool ok = false;
   explicit DeviceGuard(int device) {
     if (cudaGetDevice(&prev) != cudaSuccess) return;
-    ok = (prev == device) || cudaSetDevice(device) == cudaSuccess;
+    ok = cudaSetDevice(device) == cudaSuccess;
     if (prev == device) prev = -1;
   }
   ~DeviceGuard() {
