@@ -931,8 +931,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int cc = 0; cc < D / 32; ++cc) ptx::tmem_ld32p(tO + cc * 32, s + cc * 32);
       ptx::tmem_wait_ld();
-      const float l = l2.x + l2.y;
+      // (a row without a key: D = 64's exponentials on the FMA pipe have left denormals in its sum and in O)
+      const float l = GEN && m_ref == -INFINITY ? 0.f : l2.x + l2.y;
       const float inv = l > 0.f ? 1.f / l : 0.f;
+      if (GEN && !(l > 0.f)) {
+#pragma unroll
+        for (int e = 0; e < D; ++e) s[e] = 0;
+      }
       // O leaves through shared memory and TMA stores (coalesced; rows beyond Lq
       // are clipped by the tensor map): one 64-column block at a time, written in
       // the 128-byte-swizzled layout the map expects.
