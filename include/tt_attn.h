@@ -245,6 +245,73 @@ typedef struct tt_attn_decode_append_params {
   int32_t* status;
 } tt_attn_decode_append_params;
 
+/* Attention over sequences packed behind one another, without padding: q [total_q, Hq, D], k and v
+ * [total_k, Hkv, D]; sequence n is the rows [cu_q[n], cu_q[n + 1]) of q and [cu_k[n], cu_k[n + 1]) of k and v
+ * (device int32 [n_seqs + 1]; cu_k NULL: the same as cu_q, and total_k = total_q).  No counterpart in the
+ * reference, which has padded batches only.  Float16 / BFloat16.
+ *  - Every sequence is what tt_attn_fwd / tt_attn_bwd would make of it as a batch of one; is_causal as
+ *    there, by the lengths of the sequence.  Rows of one sequence never touch another's, infinities included.
+ *  - Sequences may be empty.  Queries of a sequence without keys give O = 0, LSE = -inf.
+ *  - Rows in front of the first sequence and behind the last are read by nobody and come out as O = 0,
+ *    LSE = -inf and zero gradients.
+ *  - Offsets that fall, are negative or lie beyond the rows set bit 16 of *status, and all results are
+ *    those of rows without a sequence.
+ *  - Strides: s per row, h per head; b is not looked at.  All zeros mean dense [total, H, D].
+ *  - lse is [Hq, total_q].
+ *  - Scratch: tt_attn_packed_workspace_bytes. */
+typedef struct tt_attn_packed_fwd_params {
+  uint32_t struct_size;
+  int32_t dtype;
+  int32_t n_seqs, Hq, Hkv, total_q, total_k, D;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  float* lse; /* may be NULL */
+  tt_attn_strides q_strides, k_strides, v_strides, o_strides;
+  const int32_t* cu_q;
+  const int32_t* cu_k; /* or NULL */
+  int32_t is_causal;
+  float scale;
+  int32_t device;
+  void* stream;
+  void* workspace;
+  size_t workspace_bytes;
+  const tt_attn_alloc_hook* alloc;
+  int32_t* status;
+} tt_attn_packed_fwd_params;
+
+typedef struct tt_attn_packed_bwd_params {
+  uint32_t struct_size;
+  int32_t dtype;
+  int32_t n_seqs, Hq, Hkv, total_q, total_k, D;
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* o;
+  const void* d_o;
+  const float* lse;
+  void* dq; /* any of the three may be NULL */
+  void* dk;
+  void* dv;
+  tt_attn_strides q_strides, k_strides, v_strides, o_strides, do_strides, dq_strides, dk_strides, dv_strides;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int32_t is_causal;
+  float scale;
+  int32_t device;
+  void* stream;
+  void* workspace;
+  size_t workspace_bytes;
+  const tt_attn_alloc_hook* alloc;
+  int32_t* status;
+} tt_attn_packed_bwd_params;
+
+TT_ATTN_API int tt_attn_packed_fwd(const tt_attn_packed_fwd_params* p);
+TT_ATTN_API int tt_attn_packed_bwd(const tt_attn_packed_bwd_params* p);
+/* kind: TT_ATTN_KIND_FWD or TT_ATTN_KIND_BWD; 0 for any other. */
+TT_ATTN_API size_t tt_attn_packed_workspace_bytes(int kind, int n_seqs, int Hq, int Hkv, int total_q, int total_k, int D);
+
 enum tt_attn_kind {
   TT_ATTN_KIND_FWD = 0,
   TT_ATTN_KIND_BWD = 1,

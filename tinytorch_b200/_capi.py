@@ -123,11 +123,68 @@ class LinearParams(C.Structure):
     ]
 
 
-FUSED_EXPORTS = ("tt_fused_add_rms_norm", "tt_silu_mul", "tt_linear", "tt_linear_selftest")  # include/tt_fused.h
+class PackedFwdParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32),
+        ("n_seqs", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("total_q", C.c_int32), ("total_k", C.c_int32),
+        ("D", C.c_int32),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p),
+        ("q_strides", Strides), ("k_strides", Strides), ("v_strides", Strides), ("o_strides", Strides),
+        ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("is_causal", C.c_int32), ("scale", C.c_float),
+        ("device", C.c_int32), ("stream", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("alloc", C.POINTER(AllocHook)), ("status", C.c_void_p),
+    ]
+
+
+class PackedBwdParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32),
+        ("n_seqs", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("total_q", C.c_int32), ("total_k", C.c_int32),
+        ("D", C.c_int32),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("d_o", C.c_void_p),
+        ("lse", C.c_void_p), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+        ("q_strides", Strides), ("k_strides", Strides), ("v_strides", Strides), ("o_strides", Strides),
+        ("do_strides", Strides), ("dq_strides", Strides), ("dk_strides", Strides), ("dv_strides", Strides),
+        ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("is_causal", C.c_int32), ("scale", C.c_float),
+        ("device", C.c_int32), ("stream", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("alloc", C.POINTER(AllocHook)), ("status", C.c_void_p),
+    ]
+
+
+MAX_ROPE_AXES = 4  # TT_ATTN_MAX_ROPE_AXES
+
+
+class QkNormRopeParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32),
+        ("B", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("S", C.c_int32), ("D", C.c_int32),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p),
+        ("q_strides", Strides), ("k_strides", Strides), ("q_out_strides", Strides), ("k_out_strides", Strides),
+        ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("eps", C.c_float), ("rope_positions", C.c_int32),
+        ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p), ("rope_interleaved", C.c_int32), ("n_axes", C.c_int32),
+        ("positions", C.c_void_p), ("position_axis_stride", C.c_int64), ("position_batch_stride", C.c_int64),
+        ("sections", C.c_int32 * MAX_ROPE_AXES), ("device", C.c_int32), ("stream", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
+class QkNormRopeBwdParams(C.Structure):
+    _fields_ = [
+        ("fwd", QkNormRopeParams), ("struct_size", C.c_uint32), ("reserved0", C.c_int32),
+        ("dq_out", C.c_void_p), ("dk_out", C.c_void_p), ("dq_out_strides", Strides), ("dk_out_strides", Strides),
+        ("dq_weight", C.c_void_p), ("dk_weight", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("alloc", C.POINTER(AllocHook)),
+    ]
+
+
+FUSED_EXPORTS = ("tt_fused_add_rms_norm", "tt_silu_mul", "tt_linear", "tt_linear_selftest", "tt_qk_norm_rope", "tt_qk_norm_rope_bwd",
+                 "tt_qk_norm_rope_workspace_bytes")  # include/tt_fused.h
 
 EXPORTS = ("tt_attn_fwd", "tt_attn_bwd", "tt_attn_decode", "tt_attn_decode_append", "tt_attn_decode_static",
            "tt_attn_selftest_wait_expiry", "tt_attn_bwd_selftest", "tt_attn_workspace_bytes", "tt_attn_strerror",
-           "tt_attn_last_cuda_error", "tt_attn_version")
+           "tt_attn_last_cuda_error", "tt_attn_version", "tt_attn_packed_fwd", "tt_attn_packed_bwd",
+           "tt_attn_packed_workspace_bytes")
 
 _lib = None
 _native = None
@@ -165,6 +222,13 @@ def lib():
         L.tt_attn_selftest_wait_expiry.restype = C.c_int
         L.tt_attn_bwd_selftest.argtypes = [C.POINTER(BwdParams), C.c_int32, C.POINTER(C.c_int32)]
         L.tt_attn_bwd_selftest.restype = C.c_int
+        for n, params in (("tt_attn_packed_fwd", PackedFwdParams), ("tt_attn_packed_bwd", PackedBwdParams),
+                          ("tt_qk_norm_rope", QkNormRopeParams), ("tt_qk_norm_rope_bwd", QkNormRopeBwdParams)):
+            getattr(L, n).argtypes, getattr(L, n).restype = [C.POINTER(params)], C.c_int
+        L.tt_attn_packed_workspace_bytes.argtypes = [C.c_int] * 7
+        L.tt_attn_packed_workspace_bytes.restype = C.c_size_t
+        L.tt_qk_norm_rope_workspace_bytes.argtypes = [C.c_int] * 5
+        L.tt_qk_norm_rope_workspace_bytes.restype = C.c_size_t
         for n in ("tt_attn_fwd", "tt_attn_bwd", "tt_attn_decode", "tt_attn_version"):
             getattr(L, n).restype = C.c_int
         L.tt_attn_workspace_bytes.argtypes = [C.c_int] * 8

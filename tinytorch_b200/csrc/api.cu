@@ -7,6 +7,8 @@
 
 #include "../../include/tt_fused.h"
 #include "common.cuh"
+#include "norm_rope.cuh"
+#include "packed.cuh"
 #include "tma_host.cuh"
 
 namespace ttattn {
@@ -157,6 +159,60 @@ size_t append_bytes(int dtype, int B, int Hq, int Hkv, int D) {
   probe.Hq = Hq, probe.Hkv = Hkv;
   if (!decode_tc_applies(dtype, D, probe)) return 0;
   return round256(static_cast<size_t>(B) * Hq * D * elem_size(dtype)) + round256(static_cast<size_t>(B) * 4);
+}
+
+int check_packed(int dtype, int n, int Hq, int Hkv, int total_q, int total_k, int D, const int32_t* cu_q, const int32_t* cu_k, int causal) {
+  if (dtype != TT_ATTN_F16 && dtype != TT_ATTN_BF16) return TT_ATTN_ERR_DTYPE;
+  if (n <= 0 || Hq <= 0 || Hkv <= 0 || total_q < 0 || total_k < 0 || Hq % Hkv != 0) return TT_ATTN_ERR_SHAPE;
+  if (D != 64 && D != 128) return TT_ATTN_ERR_HEAD_DIM;
+  if (Hq > 65535) return TT_ATTN_ERR_TOO_LARGE;
+  // work items are counted in 32 bits
+  if (packed_items(n, total_q, Hq, 1) > 0x7fffffff || packed_items(n, total_k, Hkv, 1) > 0x7fffffff) return TT_ATTN_ERR_TOO_LARGE;
+  if (!cu_q) return TT_ATTN_ERR_NULL;
+  if (!cu_k && total_q != total_k) return TT_ATTN_ERR_SHAPE;
+  if (reinterpret_cast<uintptr_t>(cu_q) % 4 || reinterpret_cast<uintptr_t>(cu_k) % 4) return TT_ATTN_ERR_ALIGN;
+  if (causal < 0 || causal > TT_ATTN_CAUSAL_BOTTOM_RIGHT) return TT_ATTN_ERR_SHAPE;
+  return TT_ATTN_OK;
+}
+Str3 packed_strides(const tt_attn_strides& st, int64_t H, int64_t total, int64_t D) {
+  if (st.h == 0 && st.s == 0) return Str3{total * H * D, D, H * D};
+  // (a batch of one: its stride is not used, but a tensor map wants one that is no smaller than the others)
+  return Str3{st.s * total > st.h * H ? st.s * total : st.h * H, st.h, st.s};
+}
+
+// Checks what the forward and the backward of tt_qk_norm_rope share and fills in the arguments.
+int norm_rope_args(const tt_qk_norm_rope_params& p, bool bwd, NormRopeArgs* a) {
+  if (p.struct_size != sizeof(tt_qk_norm_rope_params)) return TT_ATTN_ERR_STRUCT;
+  if (p.dtype < TT_ATTN_F32 || p.dtype > TT_ATTN_BF16) return TT_ATTN_ERR_DTYPE;
+  if (p.B < 0 || p.S < 0 || p.Hq <= 0 || p.Hkv <= 0) return TT_ATTN_ERR_SHAPE;
+  if (p.D != 64 && p.D != 128) return TT_ATTN_ERR_HEAD_DIM;
+  if (static_cast<int64_t>(p.B) * p.S > 0x7fffffff || p.Hq > 65535 || p.Hkv > 65535) return TT_ATTN_ERR_TOO_LARGE;
+  const bool rows = p.B > 0 && p.S > 0;
+  if (rows && (!p.q || !p.k || (!bwd && (!p.q_out || !p.k_out)))) return TT_ATTN_ERR_NULL;
+  if ((p.rope_cos == nullptr) != (p.rope_sin == nullptr)) return TT_ATTN_ERR_NULL;
+  const size_t es = elem_size(p.dtype);
+  a->x[0] = p.q, a->x[1] = p.k, a->y[0] = p.q_out, a->y[1] = p.k_out, a->w[0] = p.q_weight, a->w[1] = p.k_weight;
+  a->xs[0] = dense_or(p.q_strides, p.Hq, p.S, p.D), a->xs[1] = dense_or(p.k_strides, p.Hkv, p.S, p.D);
+  a->ys[0] = dense_or(p.q_out_strides, p.Hq, p.S, p.D), a->ys[1] = dense_or(p.k_out_strides, p.Hkv, p.S, p.D);
+  for (int t = 0; t < 2; ++t)
+    if (!aligned16(a->x[t]) || !aligned16(a->y[t]) || !aligned16(a->w[t]) || (rows && (!strides_ok(a->xs[t], es) || !strides_ok(a->ys[t], es))))
+      return TT_ATTN_ERR_ALIGN;
+  a->heads[0] = p.Hq, a->heads[1] = p.Hkv, a->B = p.B, a->S = p.S, a->eps = p.eps, a->status = p.status;
+  if (!p.rope_cos) return TT_ATTN_OK;
+  if (p.rope_positions <= 0 || p.n_axes < 1 || p.n_axes > TT_ATTN_MAX_ROPE_AXES || p.position_axis_stride < 0 || p.position_batch_stride < 0)
+    return TT_ATTN_ERR_SHAPE;
+  if (rows && !p.positions) return TT_ATTN_ERR_NULL;
+  if (!aligned16(p.rope_cos) || !aligned16(p.rope_sin) || reinterpret_cast<uintptr_t>(p.positions) % 4) return TT_ATTN_ERR_ALIGN;
+  int end = 0;
+  for (int x = 0; x < TT_ATTN_MAX_ROPE_AXES; ++x) {
+    const int n = p.n_axes == 1 ? (x == 0 ? p.D / 2 : 0) : (x < p.n_axes ? p.sections[x] : 0);
+    if (n < 0 || n > p.D / 2) return TT_ATTN_ERR_SHAPE;
+    a->axis_end[x] = end += n;
+  }
+  if (end != p.D / 2) return TT_ATTN_ERR_SHAPE;
+  a->cos = p.rope_cos, a->sin = p.rope_sin, a->rope_positions = p.rope_positions, a->interleaved = p.rope_interleaved != 0;
+  a->positions = p.positions, a->pos_axis = p.position_axis_stride, a->pos_b = p.position_batch_stride, a->axes = p.n_axes;
+  return TT_ATTN_OK;
 }
 }  // namespace
 
@@ -479,6 +535,134 @@ int tt_silu_mul(const tt_silu_mul_params* p) {
   DeviceGuard guard(p->device);
   if (!guard.ok) return TT_ATTN_ERR_NO_DEVICE;
   cudaError_t e = launch_silu_mul(p->dtype, p->out, p->x, p->rows, p->d, static_cast<cudaStream_t>(p->stream));
+  return e == cudaSuccess ? TT_ATTN_OK : launch_failed(e);
+}
+
+size_t tt_attn_packed_workspace_bytes(int kind, int n, int Hq, int Hkv, int total_q, int total_k, int D) {
+  if (n <= 0 || Hq <= 0 || Hkv <= 0 || total_q < 0 || total_k < 0 || D <= 0) return 0;
+  if (kind == TT_ATTN_KIND_FWD) return 256 + packed_plan_bytes(n, total_q, total_k, Hq / Hkv, false);
+  if (kind != TT_ATTN_KIND_BWD) return 0;
+  const size_t rows = static_cast<size_t>(Hq) * total_q;
+  return 256 + packed_plan_bytes(n, total_q, total_k, Hq / Hkv, true) + round256(rows * sizeof(float)) + round256(rows * D * sizeof(float));
+}
+
+int tt_attn_packed_fwd(const tt_attn_packed_fwd_params* p) {
+  if (!p) return TT_ATTN_ERR_NULL;
+  if (p->struct_size != sizeof(tt_attn_packed_fwd_params)) return TT_ATTN_ERR_STRUCT;
+  if (int rc = check_packed(p->dtype, p->n_seqs, p->Hq, p->Hkv, p->total_q, p->total_k, p->D, p->cu_q, p->cu_k, p->is_causal)) return rc;
+  if (p->total_q == 0) return TT_ATTN_OK;
+  if (!p->q || !p->o || (p->total_k > 0 && (!p->k || !p->v))) return TT_ATTN_ERR_NULL;
+  const size_t es = elem_size(p->dtype);
+  FwdArgs a{};
+  a.q = p->q, a.k = p->k, a.v = p->v, a.o = p->o, a.lse = p->lse;
+  a.qs = packed_strides(p->q_strides, p->Hq, p->total_q, p->D);
+  a.ks = packed_strides(p->k_strides, p->Hkv, p->total_k, p->D);
+  a.vs = packed_strides(p->v_strides, p->Hkv, p->total_k, p->D);
+  a.os = packed_strides(p->o_strides, p->Hq, p->total_q, p->D);
+  a.Skv = p->total_k;
+  if (p->total_k == 0) a.k = a.v = p->q, a.ks = a.vs = a.qs, a.Skv = 1;  // (for tensor maps that nothing is loaded through)
+  if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.o) || !strides_ok(a.qs, es) || !strides_ok(a.ks, es) ||
+      !strides_ok(a.vs, es) || !strides_ok(a.os, es))
+    return TT_ATTN_ERR_ALIGN;
+  a.B = 1, a.Hq = p->Hq, a.Hkv = p->Hkv, a.Lq = p->total_q;
+  a.causal = p->is_causal, a.scale = p->scale, a.status = p->status;
+  DeviceGuard guard(p->device);
+  if (!guard.ok) return TT_ATTN_ERR_NO_DEVICE;
+  Workspace ws;
+  const size_t need = 256 + packed_plan_bytes(p->n_seqs, p->total_q, p->total_k, p->Hq / p->Hkv, false);
+  if (int rc = ws.acquire(need, p->workspace, p->workspace_bytes, p->alloc, p->device)) return rc;
+  a.sched = static_cast<int*>(ws.ptr);
+  const PackedCall c{p->cu_q, p->cu_k ? p->cu_k : p->cu_q, p->n_seqs, p->total_k, static_cast<char*>(ws.ptr) + 256};
+  cudaError_t e = launch_fwd_packed(p->dtype, p->D, a, c, p->device, static_cast<cudaStream_t>(p->stream));
+  return e == cudaSuccess ? TT_ATTN_OK : launch_failed(e);
+}
+
+int tt_attn_packed_bwd(const tt_attn_packed_bwd_params* p) {
+  if (!p) return TT_ATTN_ERR_NULL;
+  if (p->struct_size != sizeof(tt_attn_packed_bwd_params)) return TT_ATTN_ERR_STRUCT;
+  if (int rc = check_packed(p->dtype, p->n_seqs, p->Hq, p->Hkv, p->total_q, p->total_k, p->D, p->cu_q, p->cu_k, p->is_causal)) return rc;
+  if (!p->dq && !p->dk && !p->dv) return TT_ATTN_OK;
+  if (p->total_q == 0 && p->total_k == 0) return TT_ATTN_OK;
+  if (p->total_q == 0 || p->total_k == 0) return TT_ATTN_ERR_SHAPE;  // (zeros, which the caller can write)
+  if (!p->q || !p->k || !p->v || !p->o || !p->d_o || !p->lse) return TT_ATTN_ERR_NULL;
+  const size_t es = elem_size(p->dtype);
+  BwdArgs a{};
+  a.q = p->q, a.k = p->k, a.v = p->v, a.o = p->o, a.d_o = p->d_o, a.lse = p->lse;
+  a.dq = p->dq, a.dk = p->dk, a.dv = p->dv;
+  a.qs = packed_strides(p->q_strides, p->Hq, p->total_q, p->D);
+  a.ks = packed_strides(p->k_strides, p->Hkv, p->total_k, p->D);
+  a.vs = packed_strides(p->v_strides, p->Hkv, p->total_k, p->D);
+  a.os = packed_strides(p->o_strides, p->Hq, p->total_q, p->D);
+  a.dos = packed_strides(p->do_strides, p->Hq, p->total_q, p->D);
+  a.dqs = packed_strides(p->dq_strides, p->Hq, p->total_q, p->D);
+  a.dks = packed_strides(p->dk_strides, p->Hkv, p->total_k, p->D);
+  a.dvs = packed_strides(p->dv_strides, p->Hkv, p->total_k, p->D);
+  const void* ptrs[] = {p->q, p->k, p->v, p->o, p->d_o, p->dq, p->dk, p->dv, p->lse};
+  for (const void* q : ptrs)
+    if (!aligned16(q)) return TT_ATTN_ERR_ALIGN;
+  const Str3* sts[] = {&a.qs, &a.ks, &a.vs, &a.os, &a.dos, &a.dqs, &a.dks, &a.dvs};
+  for (const Str3* s : sts)
+    if (!strides_ok(*s, es)) return TT_ATTN_ERR_ALIGN;
+  a.B = 1, a.Hq = p->Hq, a.Hkv = p->Hkv, a.Lq = p->total_q, a.Skv = p->total_k;
+  a.causal = p->is_causal, a.scale = p->scale, a.status = p->status;
+  const size_t rows = static_cast<size_t>(p->Hq) * p->total_q;
+  if (rows > 0x7fffffff) return TT_ATTN_ERR_TOO_LARGE;
+  DeviceGuard guard(p->device);
+  if (!guard.ok) return TT_ATTN_ERR_NO_DEVICE;
+  Workspace ws;  // work counter | plan | delta | dQ accumulator
+  const size_t plan = packed_plan_bytes(p->n_seqs, p->total_q, p->total_k, p->Hq / p->Hkv, true), delta = round256(rows * sizeof(float));
+  if (int rc = ws.acquire(256 + plan + delta + round256(rows * p->D * sizeof(float)), p->workspace, p->workspace_bytes, p->alloc, p->device)) return rc;
+  char* at = static_cast<char*>(ws.ptr);
+  a.sched = reinterpret_cast<int*>(at);
+  a.delta = reinterpret_cast<float*>(at + 256 + plan);
+  a.dq_accum = reinterpret_cast<float*>(at + 256 + plan + delta);
+  const PackedCall c{p->cu_q, p->cu_k ? p->cu_k : p->cu_q, p->n_seqs, p->total_k, at + 256};
+  cudaError_t e = launch_bwd_packed(p->dtype, p->D, a, c, p->device, static_cast<cudaStream_t>(p->stream));
+  return e == cudaSuccess ? TT_ATTN_OK : launch_failed(e);
+}
+
+size_t tt_qk_norm_rope_workspace_bytes(int B, int Hq, int Hkv, int S, int D) {
+  if (B < 0 || S < 0 || Hq <= 0 || Hkv <= 0 || D <= 0) return 0;
+  const int heads[2] = {Hq, Hkv};
+  int ctas[2];
+  norm_rope_bwd_ctas(B, S, heads, ctas);
+  return round256(static_cast<size_t>(ctas[0] + ctas[1]) * D * sizeof(float));
+}
+
+int tt_qk_norm_rope(const tt_qk_norm_rope_params* p) {
+  if (!p) return TT_ATTN_ERR_NULL;
+  NormRopeArgs a{};
+  if (int rc = norm_rope_args(*p, false, &a)) return rc;
+  if (p->B == 0 || p->S == 0) return TT_ATTN_OK;
+  DeviceGuard guard(p->device);
+  if (!guard.ok) return TT_ATTN_ERR_NO_DEVICE;
+  cudaError_t e = launch_norm_rope(p->dtype, p->D, a, p->device, static_cast<cudaStream_t>(p->stream));
+  return e == cudaSuccess ? TT_ATTN_OK : launch_failed(e);
+}
+
+int tt_qk_norm_rope_bwd(const tt_qk_norm_rope_bwd_params* p) {
+  if (!p) return TT_ATTN_ERR_NULL;
+  if (p->struct_size != sizeof(tt_qk_norm_rope_bwd_params)) return TT_ATTN_ERR_STRUCT;
+  NormRopeArgs a{};
+  if (int rc = norm_rope_args(p->fwd, true, &a)) return rc;
+  const bool rows = p->fwd.B > 0 && p->fwd.S > 0, sums = p->dq_weight || p->dk_weight;
+  if ((p->dq_weight && !p->fwd.q_weight) || (p->dk_weight && !p->fwd.k_weight)) return TT_ATTN_ERR_NULL;
+  if (!sums && (!rows || (!a.y[0] && !a.y[1]))) return TT_ATTN_OK;
+  if (rows && (!p->dq_out || !p->dk_out)) return TT_ATTN_ERR_NULL;
+  const size_t es = elem_size(p->fwd.dtype);
+  a.dy[0] = p->dq_out, a.dy[1] = p->dk_out, a.dw[0] = p->dq_weight, a.dw[1] = p->dk_weight;
+  a.dys[0] = dense_or(p->dq_out_strides, p->fwd.Hq, p->fwd.S, p->fwd.D), a.dys[1] = dense_or(p->dk_out_strides, p->fwd.Hkv, p->fwd.S, p->fwd.D);
+  for (int t = 0; t < 2; ++t)
+    if (!aligned16(a.dy[t]) || (rows && !strides_ok(a.dys[t], es)) || reinterpret_cast<uintptr_t>(a.dw[t]) % es) return TT_ATTN_ERR_ALIGN;
+  DeviceGuard guard(p->fwd.device);
+  if (!guard.ok) return TT_ATTN_ERR_NO_DEVICE;
+  Workspace ws;
+  if (sums)
+    if (int rc = ws.acquire(tt_qk_norm_rope_workspace_bytes(p->fwd.B, p->fwd.Hq, p->fwd.Hkv, p->fwd.S, p->fwd.D), p->workspace, p->workspace_bytes,
+                            p->alloc, p->fwd.device))
+      return rc;
+  a.part = static_cast<float*>(ws.ptr);
+  cudaError_t e = launch_norm_rope_bwd(p->fwd.dtype, p->fwd.D, a, p->fwd.device, static_cast<cudaStream_t>(p->fwd.stream));
   return e == cudaSuccess ? TT_ATTN_OK : launch_failed(e);
 }
 

@@ -24,6 +24,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
+#include <torch/csrc/utils/object_ptr.h>
 
 #include <cmath>
 #include <cstdarg>
@@ -47,6 +48,10 @@ struct Api {
   int (*add_rms_norm)(const tt_fused_add_rms_norm_params*);
   int (*silu_mul)(const tt_silu_mul_params*);
   int (*linear)(const tt_linear_params*);
+  int (*packed_fwd)(const tt_attn_packed_fwd_params*);
+  int (*packed_bwd)(const tt_attn_packed_bwd_params*);
+  int (*qk_norm_rope)(const tt_qk_norm_rope_params*);
+  int (*qk_norm_rope_bwd)(const tt_qk_norm_rope_bwd_params*);
   const char* (*strerror)(int);
   const char* (*last_cuda_error)();
 } api;
@@ -462,6 +467,294 @@ Tensor linear_autograd(const Tensor& x, const Tensor& w, const Tensor& bias) {
   return y;
 }
 
+// ------------------------------------------------------------------------------------------- packed sequences --
+// Strides of an operand of three or four dimensions for a kernel that reads 16 bytes at a time: those of the rows and heads, of a
+// dimension of one element any (torch leaves anything there).
+int64_t stride_or(const Tensor& t, int64_t dim, int64_t any) { return t.size(dim) > 1 ? t.stride(dim) : any; }
+tt_attn_strides packed_strides_of(const Tensor& t) {  // [rows, heads, D]
+  const int64_t D = t.size(2);
+  return {0, stride_or(t, 1, D), stride_or(t, 0, t.size(1) * D)};
+}
+bool vector_aligned(const Tensor& t) {
+  const int64_t es = t.element_size();
+  if (t.stride(-1) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d)
+    if (t.size(d) > 1 && (t.stride(d) <= 0 || t.stride(d) * es % 16)) return false;
+  return true;
+}
+// A gradient may be a part of a larger one, or one value expanded: any strides and offset.  It is copied where a kernel cannot read it.
+Tensor readable(const Tensor& t) { return t.numel() == 0 || vector_aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+
+void check_packed_tensor(const Tensor& t, const char* name, const Tensor& q) {
+  if (!t.is_cuda()) raise(PyExc_ValueError, "%s must be a CUDA tensor (this op has no CPU path)", name);
+  if (t.dim() != 3) raise(PyExc_ValueError, "%s must be [rows, H, D]", name);
+  if (t.scalar_type() != at::kHalf && t.scalar_type() != at::kBFloat16)
+    raise(PyExc_ValueError, "%s: packed sequences are float16 or bfloat16 (float32 goes through sdpAttention, a sequence at a time)", name);
+  if (t.scalar_type() != q.scalar_type() || t.device() != q.device()) raise(PyExc_ValueError, "%s must have the dtype and device of q", name);
+  if (t.size(2) != q.size(2)) raise(PyExc_ValueError, "%s must have the head dimension of q", name);
+  if (t.numel() > 0 && t.stride(2) != 1) raise(PyExc_ValueError, "%s: innermost dimension must be contiguous", name);
+}
+void check_offsets(const Tensor& cu, const char* name, const Tensor& q) {
+  if (cu.dim() != 1 || cu.size(0) < 2) raise(PyExc_ValueError, "%s must be [sequences + 1], with one sequence or more", name);
+  check_ints(cu, name, 2, q);
+}
+struct Packed {
+  Tensor cu_q, cu_k;  // cu_k undefined: the same as cu_q
+  int mode;
+  float scale;
+};
+void check_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Packed& s) {
+  check_packed_tensor(q, "q", q);
+  check_packed_tensor(k, "k", q);
+  check_packed_tensor(v, "v", q);
+  if (v.sizes() != k.sizes()) raise(PyExc_ValueError, "v must have the shape of k");
+  check_offsets(s.cu_q, "cuSeqlens", q);
+  if (s.cu_k.defined()) {
+    check_offsets(s.cu_k, "cuSeqlensK", q);
+    if (s.cu_k.size(0) != s.cu_q.size(0)) raise(PyExc_ValueError, "cuSeqlensK must have as many elements as cuSeqlens");
+  } else if (k.size(0) != q.size(0)) {
+    raise(PyExc_ValueError, "k must have the rows of q, unless cuSeqlensK says which are whose");
+  }
+}
+
+template <typename P>
+void set_packed(P* p, const Tensor& q, const Tensor& k, const Tensor& v, const Packed& s, const Tensor& status) {
+  set_common(p, q);
+  p->dtype = dtype_of(q.scalar_type());
+  p->n_seqs = static_cast<int32_t>(s.cu_q.size(0) - 1), p->Hq = q.size(1), p->Hkv = k.size(1);
+  p->total_q = q.size(0), p->total_k = k.size(0), p->D = q.size(2);
+  p->q = q.data_ptr(), p->k = k.data_ptr(), p->v = v.data_ptr();
+  p->q_strides = packed_strides_of(q), p->k_strides = packed_strides_of(k), p->v_strides = packed_strides_of(v);
+  p->cu_q = ints_ptr(s.cu_q), p->cu_k = ints_ptr(s.cu_k), p->is_causal = s.mode, p->scale = s.scale;
+  p->alloc = &hook, p->status = ints_ptr(status);
+}
+
+FwdResult packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Packed& s, bool need_lse, const Tensor& status) {
+  FwdResult r;
+  r.o = empty(q.sizes(), q.scalar_type(), q.device());
+  if (need_lse) r.lse = empty({q.size(1), q.size(0)}, at::kFloat, q.device());
+  tt_attn_packed_fwd_params p{};
+  set_packed(&p, q, k, v, s, status);
+  p.o = r.o.data_ptr(), p.o_strides = packed_strides_of(r.o);
+  p.lse = need_lse ? static_cast<float*>(r.lse.data_ptr()) : nullptr;
+  check(api.packed_fwd(&p));
+  return r;
+}
+
+void check_packed_bwd(const Tensor& dO, const Tensor& q, const Tensor& o, const Tensor& lse) {
+  check_packed_tensor(dO, "dO", q);
+  check_packed_tensor(o, "o", q);
+  if (dO.sizes() != q.sizes() || o.sizes() != q.sizes()) raise(PyExc_ValueError, "dO and o must have the shape of q");
+  if (lse.scalar_type() != at::kFloat || lse.device() != q.device() || !lse.is_contiguous() || lse.numel() != q.size(0) * q.size(1))
+    raise(PyExc_ValueError, "lse must be a contiguous float32 tensor [Hq, rows] on the device of q");
+}
+BwdResult packed_bwd(const Tensor& dO, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse, const Packed& s,
+                     const bool (&needs)[3]) {
+  BwdResult r;
+  const Tensor* like[3] = {&q, &k, &v};
+  const bool nothing = q.numel() == 0 || k.numel() == 0;
+  for (int i = 0; i < 3; ++i) {
+    if (!needs[i]) continue;
+    r.g[i] = empty(like[i]->sizes(), q.scalar_type(), q.device());
+    if (nothing) r.g[i].zero_();
+  }
+  if (nothing) return r;
+  tt_attn_packed_bwd_params p{};
+  set_packed(&p, q, k, v, s, Tensor());
+  p.o = o.data_ptr(), p.d_o = dO.data_ptr(), p.lse = static_cast<const float*>(lse.data_ptr());
+  p.o_strides = packed_strides_of(o), p.do_strides = packed_strides_of(dO);
+  void** out[3] = {&p.dq, &p.dk, &p.dv};
+  tt_attn_strides* st[3] = {&p.dq_strides, &p.dk_strides, &p.dv_strides};
+  for (int i = 0; i < 3; ++i)
+    if (needs[i]) *out[i] = r.g[i].data_ptr(), *st[i] = packed_strides_of(r.g[i]);
+  check(api.packed_bwd(&p));
+  return r;
+}
+
+// As AttentionBackward.  The offsets are saved like the operands: changing them in place between the two passes is an error.
+struct PackedBackward : public torch::autograd::Node {
+  SavedVariable q, k, v, o, lse, cu_q, cu_k;
+  int mode;
+  float scale;
+  std::string name() const override { return "FuncSDPAttentionPackedBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    q.reset_data(), k.reset_data(), v.reset_data(), o.reset_data(), lse.reset_data(), cu_q.reset_data(), cu_k.reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(3);
+    Tensor dO = gradient_of(*this, grads);
+    std::lock_guard<std::mutex> lock(mutex_);
+    at::NoGradGuard no_grad;
+    const Tensor qt = q.unpack(), kt = k.unpack(), vt = v.unpack(), ot = o.unpack(shared_from_this()), lt = lse.unpack();
+    const Packed s{cu_q.unpack(), cu_k.unpack(), mode, scale};
+    dO = readable(dO);
+    check_packed(qt, kt, vt, s);
+    check_packed_bwd(dO, qt, ot, lt);
+    const bool needs[3] = {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2)};
+    BwdResult r = packed_bwd(dO, qt, kt, vt, ot, lt, s, needs);
+    for (int i = 0; i < 3; ++i) out[i] = std::move(r.g[i]);
+    return out;
+  }
+};
+
+// --------------------------------------------------------------------------- norm and rotation of queries and keys --
+struct Rope {
+  Tensor cos, sin, pos;
+  int axes = 1;
+  int sections[TT_ATTN_MAX_ROPE_AXES] = {};
+  float eps;
+  bool interleaved;
+};
+// [B, H, S, D], or packed rows [T, H, D] as a batch of one
+struct Dims {
+  int64_t B, H, S, D;
+};
+Dims dims_of(const Tensor& t) {
+  return t.dim() == 4 ? Dims{t.size(0), t.size(1), t.size(2), t.size(3)} : Dims{1, t.size(1), t.size(0), t.size(2)};
+}
+tt_attn_strides head_strides_of(const Tensor& t) {
+  if (t.dim() == 3) return {t.size(0) * t.size(1) * t.size(2), stride_or(t, 1, t.size(2)), stride_or(t, 0, t.size(1) * t.size(2))};
+  const int64_t D = t.size(3);
+  return {stride_or(t, 0, D), stride_or(t, 1, D), stride_or(t, 2, D)};
+}
+// Dense, heads inside rows or rows inside heads as in `t`: attention and the next projection read it as they would have read `t`.
+Tensor empty_ordered(const Tensor& t) {
+  if (t.dim() == 3 || t.stride(1) >= t.stride(2)) return empty(t.sizes(), t.scalar_type(), t.device());
+  const int64_t H = t.size(1), S = t.size(2), D = t.size(3);
+  return Tensor(at::detail::empty_strided_cuda(t.sizes(), {S * H * D, D, H * D, 1}, t.scalar_type(), t.device()));
+}
+
+void check_head_tensor(const Tensor& t, const char* name, const Tensor& q) {
+  if (!t.is_cuda()) raise(PyExc_ValueError, "%s must be a CUDA tensor (this op has no CPU path)", name);
+  if (t.dim() != 3 && t.dim() != 4) raise(PyExc_ValueError, "%s must be [B, H, S, D] or packed [rows, H, D]", name);
+  if (dtype_of(t.scalar_type()) < 0) raise(PyExc_ValueError, "%s: dtype %s not supported", name, c10::toString(t.scalar_type()));
+  if (t.scalar_type() != q.scalar_type() || t.device() != q.device()) raise(PyExc_ValueError, "%s must have the dtype and device of q", name);
+  if (t.numel() > 0 && t.stride(-1) != 1) raise(PyExc_ValueError, "%s: innermost dimension must be contiguous", name);
+}
+void check_norm_rope(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, Rope* r) {
+  check_head_tensor(q, "q", q);
+  check_head_tensor(k, "k", q);
+  const Dims d = dims_of(q), e = dims_of(k);
+  if (k.dim() != q.dim() || e.B != d.B || e.S != d.S || e.D != d.D)
+    raise(PyExc_ValueError, "k must have the layout, batch, rows and head dimension of q");
+  for (const Tensor* w : {&qw, &kw})
+    if (w->defined() && (w->dim() != 1 || w->size(0) != d.D || w->scalar_type() != q.scalar_type() || w->device() != q.device() || !w->is_contiguous()))
+      raise(PyExc_ValueError, "norm weights must be contiguous [D] with the dtype and device of q");
+  if (r->cos.defined() != r->sin.defined()) raise(PyExc_ValueError, "rope tables come as cos and sin");
+  if (!r->cos.defined()) {
+    if (r->pos.defined()) raise(PyExc_ValueError, "positions need rope tables");
+    return;
+  }
+  if (r->cos.scalar_type() != at::kFloat || r->cos.sizes() != r->sin.sizes() || r->cos.dim() != 2 || r->cos.size(1) != d.D / 2 || r->cos.size(0) < 1 ||
+      !r->cos.is_contiguous() || !r->sin.is_contiguous() || r->sin.scalar_type() != at::kFloat || r->cos.device() != q.device() ||
+      r->sin.device() != q.device())
+    raise(PyExc_ValueError, "rope tables must be contiguous fp32 [positions, D/2] on the device of q");
+  if (!r->pos.defined()) raise(PyExc_ValueError, "positions are required with rope tables");
+  const bool many = r->axes > 0;  // sections were given
+  const int64_t lead = many ? 1 : 0, n = r->pos.dim() - lead;
+  const bool shape = (n == 1 || (n == 2 && q.dim() == 4)) && r->pos.size(-1) == d.S && (n == 1 || r->pos.size(-2) == d.B) && (!many || r->pos.size(0) == r->axes);
+  if (r->pos.scalar_type() != at::kInt || r->pos.device() != q.device() || !shape)
+    raise(PyExc_ValueError, "positions must be int32 [rows]%s on the device of q, with sections [axes, ..]", q.dim() == 4 ? " or [B, rows]" : "");
+  if (many) {
+    int64_t sum = 0;
+    for (int x = 0; x < r->axes; ++x) sum += r->sections[x];
+    if (sum != d.D / 2) raise(PyExc_ValueError, "sections must add up to D/2");
+  }
+  if (r->pos.size(-1) > 1 && r->pos.stride(-1) != 1) r->pos = r->pos.contiguous();
+}
+
+void set_norm_rope(tt_qk_norm_rope_params* p, const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Rope& r) {
+  set_common(p, q);
+  const Dims d = dims_of(q);
+  p->dtype = dtype_of(q.scalar_type());
+  p->B = d.B, p->Hq = d.H, p->Hkv = dims_of(k).H, p->S = d.S, p->D = d.D;
+  p->q = q.data_ptr(), p->k = k.data_ptr();
+  p->q_strides = head_strides_of(q), p->k_strides = head_strides_of(k);
+  p->q_weight = qw.defined() ? qw.data_ptr() : nullptr, p->k_weight = kw.defined() ? kw.data_ptr() : nullptr;
+  p->eps = r.eps;
+  if (!r.cos.defined()) return;
+  p->rope_cos = static_cast<const float*>(r.cos.data_ptr()), p->rope_sin = static_cast<const float*>(r.sin.data_ptr());
+  p->rope_positions = r.cos.size(0), p->rope_interleaved = r.interleaved;
+  const bool many = r.axes > 0;
+  p->n_axes = many ? r.axes : 1;
+  for (int x = 0; x < TT_ATTN_MAX_ROPE_AXES; ++x) p->sections[x] = r.sections[x];
+  p->positions = ints_ptr(r.pos);
+  p->position_axis_stride = many ? r.pos.stride(0) : 0;
+  p->position_batch_stride = r.pos.dim() - (many ? 1 : 0) == 2 && d.B > 1 ? r.pos.stride(-2) : 0;
+}
+
+struct Pair {
+  Tensor q, k;
+};
+Pair norm_rope_fwd(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Rope& r, const Tensor& status) {
+  Pair out{empty_ordered(q), empty_ordered(k)};
+  tt_qk_norm_rope_params p{};
+  set_norm_rope(&p, q, k, qw, kw, r);
+  p.q_out = out.q.data_ptr(), p.k_out = out.k.data_ptr();
+  p.q_out_strides = head_strides_of(out.q), p.k_out_strides = head_strides_of(out.k);
+  p.status = ints_ptr(status);
+  if (q.numel() > 0) check(api.qk_norm_rope(&p));
+  return out;
+}
+
+struct NormRopeGrads {
+  Tensor g[4];  // of q, k and their weights
+};
+NormRopeGrads norm_rope_bwd(const Tensor& gq, const Tensor& gk, const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Rope& r,
+                            const bool (&needs)[4]) {
+  NormRopeGrads out;
+  if (needs[0]) out.g[0] = empty_ordered(q);
+  if (needs[1]) out.g[1] = empty_ordered(k);
+  for (int i = 2; i < 4; ++i)
+    if (needs[i]) out.g[i] = empty({q.size(-1)}, q.scalar_type(), q.device());
+  const Tensor a = readable(gq), b = readable(gk);
+  tt_qk_norm_rope_bwd_params p{};
+  p.struct_size = sizeof(p);
+  set_norm_rope(&p.fwd, q, k, qw, kw, r);
+  if (needs[0]) p.fwd.q_out = out.g[0].data_ptr(), p.fwd.q_out_strides = head_strides_of(out.g[0]);
+  if (needs[1]) p.fwd.k_out = out.g[1].data_ptr(), p.fwd.k_out_strides = head_strides_of(out.g[1]);
+  p.dq_out = a.data_ptr(), p.dk_out = b.data_ptr();
+  p.dq_out_strides = head_strides_of(a), p.dk_out_strides = head_strides_of(b);
+  if (needs[2]) p.dq_weight = out.g[2].data_ptr();
+  if (needs[3]) p.dk_weight = out.g[3].data_ptr();
+  p.alloc = &hook;
+  check(api.qk_norm_rope_bwd(&p));
+  return out;
+}
+void check_norm_rope_bwd(const Tensor& gq, const Tensor& gk, const Tensor& q, const Tensor& k) {
+  if (gq.sizes() != q.sizes() || gk.sizes() != k.sizes() || gq.scalar_type() != q.scalar_type() || gk.scalar_type() != q.scalar_type() ||
+      gq.device() != q.device() || gk.device() != q.device())
+    raise(PyExc_ValueError, "gradients must have the shapes, dtype and device of q and k");
+}
+
+struct NormRopeBackward : public torch::autograd::Node {
+  SavedVariable q, k, qw, kw, cos, sin, pos;
+  Rope rope;  // (without its tensors)
+  std::string name() const override { return "FuncQkNormRopeBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    q.reset_data(), k.reset_data(), qw.reset_data(), kw.reset_data(), cos.reset_data(), sin.reset_data(), pos.reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(4);
+    const Tensor gq = grads[0].defined() ? grads[0] : input_metadata(0).zeros_like();
+    const Tensor gk = grads[1].defined() ? grads[1] : input_metadata(1).zeros_like();
+    std::lock_guard<std::mutex> lock(mutex_);
+    at::NoGradGuard no_grad;
+    const Tensor qt = q.unpack(), kt = k.unpack(), qwt = qw.unpack(), kwt = kw.unpack();
+    Rope r = rope;
+    r.cos = cos.unpack(), r.sin = sin.unpack(), r.pos = pos.unpack();
+    check_norm_rope(qt, kt, qwt, kwt, &r);  // (a hook may have brought back something else)
+    check_norm_rope_bwd(gq, gk, qt, kt);
+    bool needs[4];
+    for (int i = 0; i < 4; ++i) needs[i] = task_should_compute_output(i) && (i < 2 || (i == 2 ? qwt : kwt).defined());
+    NormRopeGrads g = norm_rope_bwd(gq, gk, qt, kt, qwt, kwt, r, needs);
+    for (int i = 0; i < 4; ++i) out[i] = std::move(g.g[i]);
+    return out;
+  }
+};
+
 // ------------------------------------------------------------------------------------------ python methods --
 // The nodes here know reverse mode only.  A trace has to record the operator, forward-mode derivatives and functorch's
 // transforms have to reach torch, which refuses them: the Python autograd functions (function.py, fused.py) see to that.
@@ -785,6 +1078,154 @@ PyObject* py_linear_raw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// sdp_attention_packed(q, k, v, cuSeqlens, cuSeqlensK, mode, scale) -> O; NotImplemented as sdp_attention
+PyObject* py_sdp_attention_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 7);
+  const Tensor &q = tensor_of(a[0], "q"), &k = tensor_of(a[1], "k"), &v = tensor_of(a[2], "v");
+  if (needs_python_function({&q, &k, &v})) Py_RETURN_NOTIMPLEMENTED;
+  const bool grad = wants_grad(q, k, v);
+  if (q.dim() != 3) raise(PyExc_ValueError, "q must be [rows, H, D]");
+  const Packed s{tensor_of(a[3], "cuSeqlens"), optional_of(a[4], "cuSeqlensK"), int_arg(a[5]), scale_or_default(scale_arg(a[6]), q.size(2))};
+  check_packed(q, k, v, s);
+  FwdResult r;
+  {
+    NoGil nogil;
+    r = packed_fwd(q, k, v, s, grad, Tensor());
+    if (grad) {
+      auto node = std::shared_ptr<PackedBackward>(new PackedBackward(), torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(q, k, v));
+      node->q = SavedVariable(q, false), node->k = SavedVariable(k, false), node->v = SavedVariable(v, false);
+      node->lse = SavedVariable(r.lse, false), node->cu_q = SavedVariable(s.cu_q, false), node->cu_k = SavedVariable(s.cu_k, false);
+      node->mode = s.mode, node->scale = s.scale;
+      torch::autograd::set_history(r.o, node);
+      node->o = SavedVariable(r.o, true);
+    }
+  }
+  return wrap(r.o);
+  END_HANDLE_TH_ERRORS
+}
+
+// packed_fwd(q, k, v, cuSeqlens, cuSeqlensK, mode, scale, needLse, status) -> (O, LSE or None)
+PyObject* py_packed_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 9);
+  const Tensor &q = tensor_of(a[0], "q"), &k = tensor_of(a[1], "k"), &v = tensor_of(a[2], "v");
+  if (q.dim() != 3) raise(PyExc_ValueError, "q must be [rows, H, D]");
+  const Packed s{tensor_of(a[3], "cuSeqlens"), optional_of(a[4], "cuSeqlensK"), int_arg(a[5]), scale_or_default(scale_arg(a[6]), q.size(2))};
+  const bool need_lse = bool_arg(a[7]);
+  const Tensor status = optional_of(a[8], "status");
+  check_packed(q, k, v, s);
+  check_ints(status, "status", 1, q);
+  FwdResult r;
+  {
+    NoGil nogil;
+    r = packed_fwd(q, k, v, s, need_lse, status);
+  }
+  return tuple_of({&r.o, &r.lse});
+  END_HANDLE_TH_ERRORS
+}
+
+// packed_bwd(dO, q, k, v, o, lse, cuSeqlens, cuSeqlensK, mode, scale, need_dq, need_dk, need_dv) -> (dQ, dK, dV), None where not needed
+PyObject* py_packed_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 13);
+  const Tensor &q = tensor_of(a[1], "q"), &k = tensor_of(a[2], "k"), &v = tensor_of(a[3], "v"), &o = tensor_of(a[4], "o"), &lse = tensor_of(a[5], "lse");
+  if (q.dim() != 3) raise(PyExc_ValueError, "q must be [rows, H, D]");
+  const Packed s{tensor_of(a[6], "cuSeqlens"), optional_of(a[7], "cuSeqlensK"), int_arg(a[8]), scale_or_default(scale_arg(a[9]), q.size(2))};
+  check_packed(q, k, v, s);
+  Tensor dO = tensor_of(a[0], "dO");
+  if (dO.dim() == 3 && dO.is_cuda()) dO = readable(dO);
+  check_packed_bwd(dO, q, o, lse);
+  const bool needs[3] = {bool_arg(a[10]), bool_arg(a[11]), bool_arg(a[12])};
+  BwdResult r;
+  {
+    NoGil nogil;
+    at::NoGradGuard no_grad;
+    r = packed_bwd(dO, q, k, v, o, lse, s, needs);
+  }
+  return tuple_of({&r.g[0], &r.g[1], &r.g[2]});
+  END_HANDLE_TH_ERRORS
+}
+
+// cos, sin, positions, eps, interleaved, sections (None or a sequence of integers)
+Rope rope_args(PyObject* const* a) {
+  Rope r;
+  r.cos = optional_of(a[0], "cos"), r.sin = optional_of(a[1], "sin"), r.pos = optional_of(a[2], "positions");
+  const double eps = PyFloat_AsDouble(a[3]);
+  if (eps == -1.0 && PyErr_Occurred()) throw python_error();
+  r.eps = static_cast<float>(eps);
+  r.interleaved = bool_arg(a[4]);
+  r.axes = 0;
+  if (a[5] != Py_None) {
+    THPObjectPtr seq(PySequence_Fast(a[5], "sections must be a sequence of integers"));
+    if (!seq) throw python_error();
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq.get());
+    if (n < 1 || n > TT_ATTN_MAX_ROPE_AXES) raise(PyExc_ValueError, "sections: one to %d axes", TT_ATTN_MAX_ROPE_AXES);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      r.sections[i] = int_arg(PySequence_Fast_GET_ITEM(seq.get(), i));
+      if (r.sections[i] < 0 || r.sections[i] > 1024) raise(PyExc_ValueError, "sections must add up to D/2");
+    }
+    r.axes = static_cast<int>(n);
+  }
+  return r;
+}
+
+// qk_norm_rope(q, k, qWeight, kWeight, cos, sin, positions, eps, interleaved, sections, status) -> (q', k'); NotImplemented as sdp_attention
+PyObject* qk_norm_rope(PyObject* const* a, Py_ssize_t n, bool differentiable) {
+  HANDLE_TH_ERRORS
+  expect(n, 11);
+  const Tensor &q = tensor_of(a[0], "q"), &k = tensor_of(a[1], "k");
+  const Tensor qw = optional_of(a[2], "qWeight"), kw = optional_of(a[3], "kWeight");
+  if (differentiable && needs_python_function({&q, &k, &qw, &kw})) Py_RETURN_NOTIMPLEMENTED;
+  Rope r = rope_args(a + 4);
+  const Tensor status = optional_of(a[10], "status");
+  check_norm_rope(q, k, qw, kw, &r);
+  check_ints(status, "status", 1, q);
+  const bool grad = differentiable && at::GradMode::is_enabled() &&
+                    (q.requires_grad() || k.requires_grad() || (qw.defined() && qw.requires_grad()) || (kw.defined() && kw.requires_grad()));
+  Pair out;
+  {
+    NoGil nogil;
+    out = norm_rope_fwd(q, k, qw, kw, r, status);
+    if (grad) {
+      auto node = std::shared_ptr<NormRopeBackward>(new NormRopeBackward(), torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(q, k, qw, kw));
+      node->q = SavedVariable(q, false), node->k = SavedVariable(k, false), node->qw = SavedVariable(qw, false), node->kw = SavedVariable(kw, false);
+      node->cos = SavedVariable(r.cos, false), node->sin = SavedVariable(r.sin, false), node->pos = SavedVariable(r.pos, false);
+      r.cos.reset(), r.sin.reset(), r.pos.reset();
+      node->rope = r;
+      torch::autograd::set_history(out.q, node);
+      torch::autograd::set_history(out.k, node);
+    }
+  }
+  return tuple_of({&out.q, &out.k});
+  END_HANDLE_TH_ERRORS
+}
+PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) { return qk_norm_rope(a, n, true); }
+// ... without autograd
+PyObject* py_qk_norm_rope_raw(PyObject*, PyObject* const* a, Py_ssize_t n) { return qk_norm_rope(a, n, false); }
+
+// qk_norm_rope_bwd(gq, gk, q, k, qWeight, kWeight, cos, sin, positions, eps, interleaved, sections, four needs) -> (dq, dk, dqWeight, dkWeight)
+PyObject* py_qk_norm_rope_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 16);
+  const Tensor &gq = tensor_of(a[0], "gq"), &gk = tensor_of(a[1], "gk"), &q = tensor_of(a[2], "q"), &k = tensor_of(a[3], "k");
+  const Tensor qw = optional_of(a[4], "qWeight"), kw = optional_of(a[5], "kWeight");
+  Rope r = rope_args(a + 6);
+  check_norm_rope(q, k, qw, kw, &r);
+  check_norm_rope_bwd(gq, gk, q, k);
+  const bool needs[4] = {bool_arg(a[12]), bool_arg(a[13]), bool_arg(a[14]) && qw.defined(), bool_arg(a[15]) && kw.defined()};
+  NormRopeGrads g;
+  {
+    NoGil nogil;
+    at::NoGradGuard no_grad;
+    g = norm_rope_bwd(gq, gk, q, k, qw, kw, r, needs);
+  }
+  return tuple_of({&g.g[0], &g.g[1], &g.g[2], &g.g[3]});
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(path of libtt_attn.so, exception class): the library the calls go to
 PyObject* py_bind(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
@@ -804,6 +1245,10 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   sym(api.add_rms_norm, "tt_fused_add_rms_norm");
   sym(api.silu_mul, "tt_silu_mul");
   sym(api.linear, "tt_linear");
+  sym(api.packed_fwd, "tt_attn_packed_fwd");
+  sym(api.packed_bwd, "tt_attn_packed_bwd");
+  sym(api.qk_norm_rope, "tt_qk_norm_rope");
+  sym(api.qk_norm_rope_bwd, "tt_qk_norm_rope_bwd");
   sym(api.strerror, "tt_attn_strerror");
   sym(api.last_cuda_error, "tt_attn_last_cuda_error");
   Py_INCREF(exc);
@@ -829,6 +1274,12 @@ PyMethodDef methods[] = {
     {"linear", fast(py_linear), METH_FASTCALL, nullptr},
     {"linear_bwd", fast(py_linear_bwd), METH_FASTCALL, nullptr},
     {"linear_raw", fast(py_linear_raw), METH_FASTCALL, nullptr},
+    {"sdp_attention_packed", fast(py_sdp_attention_packed), METH_FASTCALL, nullptr},
+    {"packed_fwd", fast(py_packed_fwd), METH_FASTCALL, nullptr},
+    {"packed_bwd", fast(py_packed_bwd), METH_FASTCALL, nullptr},
+    {"qk_norm_rope", fast(py_qk_norm_rope), METH_FASTCALL, nullptr},
+    {"qk_norm_rope_raw", fast(py_qk_norm_rope_raw), METH_FASTCALL, nullptr},
+    {"qk_norm_rope_bwd", fast(py_qk_norm_rope_bwd), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

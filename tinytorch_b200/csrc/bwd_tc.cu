@@ -39,6 +39,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "packed.cuh"
 #include "ptx.cuh"
 #include "tma_host.cuh"
 
@@ -57,6 +58,8 @@ struct Item {
   // the walk: n_steps query tiles from tile qt of query head h on; a head's tiles are [qt_begin, n_q_tiles)
   int qt_begin, n_steps, h, qt;  // n_steps < 0: no more items
   int mask;                      // whether the mask has to be looked at
+  int n_q;                       // packed: query tiles of the sequence,
+  int q0, lq, k0, lk, seq;       // its first rows of q and k, and how many
 };
 
 struct __align__(8) SmemCtl {
@@ -84,7 +87,8 @@ struct Cfg128 {
   static constexpr int kDsBytes = BM * BQ * 2;         // the dS^T tile
   static constexpr int kDqStage = (D / 32) * BQ * 128; // dQ staging: boxes of 128 rows x 32 floats, one per compute warpgroup
   static constexpr int kVecBytes = 2 * 2 * BQ * 4;     // lse / delta vectors, two buffers
-  static constexpr int kSmem = 2 * TB + 2 * TB + kDsBytes + kDqStage + kVecBytes + 256;
+  static constexpr int kSmem = 2 * TB + 2 * TB + kDsBytes + kDqStage + kVecBytes + 512;
+  static_assert(sizeof(SmemCtl) <= 512, "control block");
   static_assert(kSmem <= 232448, "exceeds the shared memory a CTA may request");
 };
 
@@ -212,8 +216,9 @@ __device__ __forceinline__ void ds_chunk(const uint32_t (&p)[16], const uint32_t
 
 // GEN: the general variant (a mask and / or a causal triangle that is not top-left
 // aligned); the fast variant compiles all of that out.  PARTS: a key tile's walk is
-// divided among a.parts work items (see bwd_parts).
-template <bool BF16, bool GEN, bool PARTS>
+// divided among a.parts work items (see bwd_parts).  PACKED: sequences packed behind one another, whose items and tensor
+// maps packed_plan.cu has made; without a mask, undivided.
+template <bool BF16, bool GEN, bool PARTS, bool PACKED>
 __global__ void __launch_bounds__(Cfg128::kThreads, 1)
     bwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
@@ -247,33 +252,48 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
   // last `tail_heads` heads are ordered differently, key tile by key tile ACROSS those heads, so that the items
   // drawn last are the short ones and the CTAs finish together.
   const int group = a.Hq / a.Hkv;
-  const int n_kt = (a.Skv + BM - 1) / BM, n_heads = a.Hkv * a.B;
-  const int n_items = n_kt * n_heads * (PARTS ? a.parts : 1);
-  const int n_q_tiles = (a.Lq + BQ - 1) / BQ;
+  constexpr bool MASK = GEN && !PACKED;
+  const int n_heads = a.Hkv * a.B;
+  int n_kt = (a.Skv + BM - 1) / BM, tail_heads = a.tail_heads;  // (packed: the producer asks the plan)
+  int n_items = n_kt * n_heads * (PARTS ? a.parts : 1);
+  const int n_q_all = (a.Lq + BQ - 1) / BQ;
+  auto read_plan = [&]() {
+    n_kt = *a.packed.n_items, n_items = n_kt * n_heads;
+    const int want = n_kt > 0 ? (2 * static_cast<int>(gridDim.x) + n_kt - 1) / n_kt : 0;
+    tail_heads = want < n_heads ? want : n_heads;
+  };
+  auto map_of = [&](int seq, int which) { return static_cast<const CUtensorMap*>(a.packed.maps) + seq * static_cast<int64_t>(kPackedBwdMaps) + which; };
   auto decode_item = [&](int w) {
     Item it;
     it.part = 0;
     if (PARTS) it.part = w % a.parts, w /= a.parts;
-    const int w0 = (n_heads - a.tail_heads) * n_kt;
+    const int w0 = (n_heads - tail_heads) * n_kt;
     int bh, nt;
     if (w < w0) {
       bh = w / n_kt;
       nt = w - bh * n_kt;
     } else {
       const int x = w - w0;
-      nt = x / a.tail_heads;
-      bh = n_heads - a.tail_heads + (x - nt * a.tail_heads);
+      nt = x / tail_heads;
+      bh = n_heads - tail_heads + (x - nt * tail_heads);
     }
     it.b = bh / a.Hkv, it.hk = bh - it.b * a.Hkv;
+    int kv_len = a.Skv, Lq = a.Lq, n_q_tiles = n_q_all;
+    if constexpr (PACKED) {
+      const int4* e = reinterpret_cast<const int4*>(a.packed.items + nt);
+      const int4 rows = __ldg(e), place = __ldg(e + 1);
+      it.q0 = rows.x, it.lq = Lq = rows.y, it.k0 = rows.z, it.lk = kv_len = rows.w;
+      nt = place.x, it.seq = place.y;
+      it.n_q = n_q_tiles = (Lq + BQ - 1) / BQ;
+    }
     it.kv0 = nt * BM;
-    int kv_len = a.Skv;
-    if (a.kv_lens) {
+    if (!PACKED && a.kv_lens) {
       int l = a.kv_lens[it.b];
       kv_len = l < 0 ? 0 : (l < a.Skv ? l : a.Skv);
     }
     it.kv_len = kv_len;
-    it.mask = GEN && a.mask.ptr && !(a.mask_pure && a.mask_pure[it.b]);
-    it.shift = GEN ? causal_shift(a.causal, kv_len, a.Lq) : 0;  // key j participates iff j <= i + shift
+    it.mask = MASK && a.mask.ptr && !(a.mask_pure && a.mask_pure[it.b]);
+    it.shift = GEN ? causal_shift(a.causal, kv_len, Lq) : 0;  // key j participates iff j <= i + shift
     // BM == BQ: query tiles before the key tile see none of it (general: first tile with a row i >= kv0 - shift)
     it.qt_begin = a.causal ? (GEN ? (it.kv0 - it.shift > 0 ? (it.kv0 - it.shift) / BQ : 0) : nt) : 0;
     const int per_head = (it.kv0 < kv_len && it.qt_begin < n_q_tiles) ? n_q_tiles - it.qt_begin : 0;
@@ -286,8 +306,8 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
     return it;
   };
   // the next query tile of the walk
-  auto advance = [&](int& h, int& qt, int qt_begin) {
-    if (++qt == n_q_tiles) qt = qt_begin, ++h;
+  auto advance = [&](int& h, int& qt, const Item& it) {
+    if (++qt == (PACKED ? it.n_q : n_q_all)) qt = it.qt_begin, ++h;
   };
 
   if (warp == C::kProdWarp && lane == 0) {
@@ -350,13 +370,13 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
       }
       const int q0 = it.qt * BQ;
       float lv[4], dl[4];
-      const int64_t base = (static_cast<int64_t>(it.b) * a.Hq + it.h) * a.Lq + q0;
+      const int64_t base = (static_cast<int64_t>(it.b) * a.Hq + it.h) * a.Lq + (PACKED ? it.q0 : 0) + q0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int row = j * 32 + lane;
         lv[j] = -INFINITY;  // rows beyond Lq behave like rows without any participating key: P = 0
         dl[j] = 0.f;
-        if (q0 + row < a.Lq) {
+        if (q0 + row < (PACKED ? it.lq : a.Lq)) {
           lv[j] = a.lse[base + row];
           dl[j] = a.delta[base + row];
         }
@@ -374,9 +394,10 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
     // latency of the atomic does not sit between two items.
     // The first item is the CTA's own number; the counter, which the delta pre-pass has zeroed, hands out the rest.
     int drawn = blockIdx.x;
-    if (GEN && a.mask_pure) {  // (the lengths come from the pre-pass)
+    if (PACKED || (MASK && a.mask_pure)) {  // (the items or the lengths come from a kernel before)
       ptx::grid_dep_wait();
       dep_waited = true;
+      if (PACKED) read_plan();
     }
     auto draw = [&]() {
       if (!dep_waited) ptx::grid_dep_wait();
@@ -398,10 +419,10 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
             void* base = t == 0 ? a.dv : a.dk;
             const Str3& st = t == 0 ? a.dvs : a.dks;
             if (!base || PARTS) continue;  // (of a divided key tile the last kernel knows which parts exist)
-            T* out = reinterpret_cast<T*>(base) + it.b * st.b + it.hk * st.h;
+            T* out = reinterpret_cast<T*>(base) + it.b * st.b + it.hk * st.h + (PACKED ? it.k0 * st.s : 0);
             for (int e = lane; e < BM * (D / 8); e += 32) {
               const int row = it.kv0 + e / (D / 8);
-              if (row < a.Skv)
+              if (row < (PACKED ? it.lk : a.Skv))
                 *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row) * st.s + (e % (D / 8)) * 8) =
                     make_uint4(0, 0, 0, 0);
             }
@@ -411,6 +432,11 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
         }
       }
       int ok = 1;
+      const CUtensorMap *mq = &tmQ, *mk = &tmK, *mv = &tmV, *mdo = &tmdO;
+      if (PACKED && w >= 0) {
+        mq = map_of(it.seq, kMapQ), mk = map_of(it.seq, kMapK), mv = map_of(it.seq, kMapV), mdo = map_of(it.seq, kMapdO);
+        if (lane == 0) ptx::tensormap_acquire(mq), ptx::tensormap_acquire(mk), ptx::tensormap_acquire(mv), ptx::tensormap_acquire(mdo);
+      }
       if (lane == 0) {
         const int slot = i & 1;
         ok = ptx::mbar_wait(&ctl->item_empty[slot], ((i >> 1) & 1) ^ 1, abort_flag);
@@ -424,16 +450,16 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
           ptx::mbar_arrive_expect_tx(&ctl->kv_full, 2 * TB);
 #pragma unroll
           for (int hf = 0; hf < HALVES; ++hf) {
-            ptx::tma_load_4d(sK + hf * kHalfBytes, &tmK, &ctl->kv_full, hf * 64, it.kv0, it.hk, it.b);
-            ptx::tma_load_4d(sV + hf * kHalfBytes, &tmV, &ctl->kv_full, hf * 64, it.kv0, it.hk, it.b);
+            ptx::tma_load_4d(sK + hf * kHalfBytes, mk, &ctl->kv_full, hf * 64, it.kv0, it.hk, it.b);
+            ptx::tma_load_4d(sV + hf * kHalfBytes, mv, &ctl->kv_full, hf * 64, it.kv0, it.hk, it.b);
           }
         }
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok || w < 0) break;
-      for (int n = 0; n < it.n_steps; ++n, advance(it.h, it.qt, it.qt_begin)) {
+      for (int n = 0; n < it.n_steps; ++n, advance(it.h, it.qt, it)) {
         if (redraw && n + 1 == it.n_steps) draw();
-        if (GEN && it.mask) prefetch_mask(a, it.b, it.h, it.qt * BQ, it.kv0, lane);
+        if (MASK && it.mask) prefetch_mask(a, it.b, it.h, it.qt * BQ, it.kv0, lane);
         const uint32_t g = gq + n;
         const int h = it.h, q0 = it.qt * BQ;
         // The vectors (two buffers) are fetched a step ahead of the tiles (one stage): the wait passed for the
@@ -447,8 +473,8 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
             ptx::mbar_arrive_expect_tx(&ctl->q_full, 2 * TB);
 #pragma unroll
             for (int hf = 0; hf < HALVES; ++hf) {
-              ptx::tma_load_4d(sQ + hf * kHalfBytes, &tmQ, &ctl->q_full, hf * 64, q0, h, it.b);
-              ptx::tma_load_4d(sdO + hf * kHalfBytes, &tmdO, &ctl->q_full, hf * 64, q0, h, it.b);
+              ptx::tma_load_4d(sQ + hf * kHalfBytes, mq, &ctl->q_full, hf * 64, q0, h, it.b);
+              ptx::tma_load_4d(sdO + hf * kHalfBytes, mdo, &ctl->q_full, hf * 64, q0, h, it.b);
             }
           }
         }
@@ -590,6 +616,9 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
       int h = it.h, qt = it.qt;  // query head and tile of the step
       const int kv_row = kv0 + r;
       const bool row_valid = kv_row < kv_len;
+      const CUtensorMap* mdq = PACKED ? map_of(it.seq, kMapdQ) : &tmdQ;
+      const CUtensorMap* mout = wg == 0 ? (PACKED ? map_of(it.seq, kMapdV) : &tmdV) : (PACKED ? map_of(it.seq, kMapdK) : &tmdK);
+      if (PACKED && r == 0) ptx::tensormap_acquire(mdq), ptx::tensormap_acquire(mout);
 
       // dQ of step n shares region A with S^T, so the four compute warpgroups move it out themselves before the
       // next step's S^T may be issued: thread r owns query row q0 + r, warpgroup w the columns [32w, 32w+32),
@@ -615,7 +644,7 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
         ptx::fence_proxy_async_smem();
         ptx::named_barrier(3 + wg, BM);
         if (r == 0 && ok) {
-          ptx::tma_reduce_add_4d(&tmdQ, stage, wg * 32, q0, h, b);
+          ptx::tma_reduce_add_4d(mdq, stage, wg * 32, q0, h, b);
           ptx::bulk_commit();
         }
       };
@@ -629,8 +658,8 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
           fetch_mask(a.mask, b * a.mask.sb + h * a.mask.sh + q * a.mask.sl + kv_row, kv_row < a.Skv ? a.Lq - q : 0, mw[sc]);
         }
       };
-      if (GEN && it.mask) fetch(h, qt);
-      for (int n = 0; n < n_steps; ++n, advance(h, qt, it.qt_begin)) {
+      if (MASK && it.mask) fetch(h, qt);
+      for (int n = 0; n < n_steps; ++n, advance(h, qt, it)) {
         const uint32_t g = g0 + n;
         const int q0 = qt * BQ;
         // per-query vectors of the step, written by the producer warp: [0,128) -lse * log2(e), [128,256) -delta * scale
@@ -652,7 +681,7 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
           uint32_t pk[8], dk[8];
           int n_hidden = 0;
           if (masked) n_hidden = !row_valid ? 16 : (diag ? kv_row - (q0 + col + shift) : 0);
-          p_chunk<BF16, GEN, T>(a, s, vec + col, c2v, n_hidden, GEN && it.mask, mw[sc], pk);
+          p_chunk<BF16, MASK, T>(a, s, vec + col, c2v, n_hidden, MASK && it.mask, mw[sc], pk);
           ds_chunk<BF16>(s, dp, vec + BQ + col, sc2, dk);
           // Warpgroup w keeps its 16-bit results in columns [32w, 32w+16) of the
           // region, i.e. over the first 16 columns it loaded itself, never over
@@ -678,9 +707,9 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before();
         ptx::mbar_arrive(&ctl->pds_full);
-        if (GEN && it.mask && n + 1 < n_steps) {
+        if (MASK && it.mask && n + 1 < n_steps) {
           int h1 = h, qt1 = qt;
-          advance(h1, qt1, it.qt_begin);
+          advance(h1, qt1, it);
           fetch(h1, qt1);
         }
         read_out_dq(n);
@@ -748,7 +777,7 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
             ptx::fence_proxy_async_smem();
             ptx::named_barrier(3 + wg, BM);
             if (r == 0 && ok && wanted) {
-              ptx::tma_store_4d(wg == 0 ? &tmdV : &tmdK, stage, hf * 64, kv0, hk, b);
+              ptx::tma_store_4d(mout, stage, hf * 64, kv0, hk, b);
               ptx::bulk_commit();
             }
           }
@@ -807,7 +836,7 @@ struct Cfg64 {
   static constexpr int kProdWarp = 20, kIssWarp = 21, kThreads = 768;
 };
 
-template <bool BF16, bool GEN, bool PARTS>
+template <bool BF16, bool GEN, bool PARTS, bool PACKED>
 __global__ void __launch_bounds__(Cfg64::kThreads, 1)
     bwd_tc64_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
@@ -836,33 +865,48 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
   // longest).  Only the last `tail_heads` heads are ordered key tile by key tile ACROSS those heads, so that the
   // items drawn last are the short ones and the CTAs finish together.
   const int group = a.Hq / a.Hkv;
-  const int n_kt = (a.Skv + BM - 1) / BM, n_heads = a.Hkv * a.B;
-  const int n_items = n_kt * n_heads * (PARTS ? a.parts : 1);
-  const int n_q_tiles = (a.Lq + BQ - 1) / BQ;
+  constexpr bool MASK = GEN && !PACKED;
+  const int n_heads = a.Hkv * a.B;
+  int n_kt = (a.Skv + BM - 1) / BM, tail_heads = a.tail_heads;  // (packed: the producer asks the plan)
+  int n_items = n_kt * n_heads * (PARTS ? a.parts : 1);
+  const int n_q_all = (a.Lq + BQ - 1) / BQ;
+  auto read_plan = [&]() {
+    n_kt = *a.packed.n_items, n_items = n_kt * n_heads;
+    const int want = n_kt > 0 ? (2 * static_cast<int>(gridDim.x) + n_kt - 1) / n_kt : 0;
+    tail_heads = want < n_heads ? want : n_heads;
+  };
+  auto map_of = [&](int seq, int which) { return static_cast<const CUtensorMap*>(a.packed.maps) + seq * static_cast<int64_t>(kPackedBwdMaps) + which; };
   auto decode_item = [&](int w) {
     Item it;
     it.part = 0;
     if (PARTS) it.part = w % a.parts, w /= a.parts;
-    const int w0 = (n_heads - a.tail_heads) * n_kt;
+    const int w0 = (n_heads - tail_heads) * n_kt;
     int bh, nt;
     if (w < w0) {
       bh = w / n_kt;
       nt = w - bh * n_kt;
     } else {
       const int x = w - w0;
-      nt = x / a.tail_heads;
-      bh = n_heads - a.tail_heads + (x - nt * a.tail_heads);
+      nt = x / tail_heads;
+      bh = n_heads - tail_heads + (x - nt * tail_heads);
     }
     it.b = bh / a.Hkv, it.hk = bh - it.b * a.Hkv;
+    int kv_len = a.Skv, Lq = a.Lq, n_q_tiles = n_q_all;
+    if constexpr (PACKED) {
+      const int4* e = reinterpret_cast<const int4*>(a.packed.items + nt);
+      const int4 rows = __ldg(e), place = __ldg(e + 1);
+      it.q0 = rows.x, it.lq = Lq = rows.y, it.k0 = rows.z, it.lk = kv_len = rows.w;
+      nt = place.x, it.seq = place.y;
+      it.n_q = n_q_tiles = (Lq + BQ - 1) / BQ;
+    }
     it.kv0 = nt * BM;
-    int kv_len = a.Skv;
-    if (a.kv_lens) {
+    if (!PACKED && a.kv_lens) {
       int l = a.kv_lens[it.b];
       kv_len = l < 0 ? 0 : (l < a.Skv ? l : a.Skv);
     }
     it.kv_len = kv_len;
-    it.mask = GEN && a.mask.ptr && !(a.mask_pure && a.mask_pure[it.b]);
-    it.shift = GEN ? causal_shift(a.causal, kv_len, a.Lq) : 0;  // key j participates iff j <= i + shift
+    it.mask = MASK && a.mask.ptr && !(a.mask_pure && a.mask_pure[it.b]);
+    it.shift = GEN ? causal_shift(a.causal, kv_len, Lq) : 0;  // key j participates iff j <= i + shift
     // BM == BQ: query tiles before the key tile see none of it (general: first tile with a row i >= kv0 - shift)
     it.qt_begin = a.causal ? (GEN ? (it.kv0 - it.shift > 0 ? (it.kv0 - it.shift) / BQ : 0) : nt) : 0;
     const int per_head = (it.kv0 < kv_len && it.qt_begin < n_q_tiles) ? n_q_tiles - it.qt_begin : 0;
@@ -875,8 +919,8 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
     return it;
   };
   // the next query tile of the walk
-  auto advance = [&](int& h, int& qt, int qt_begin) {
-    if (++qt == n_q_tiles) qt = qt_begin, ++h;
+  auto advance = [&](int& h, int& qt, const Item& it) {
+    if (++qt == (PACKED ? it.n_q : n_q_all)) qt = it.qt_begin, ++h;
   };
 
   if (warp == C::kProdWarp && lane == 0) {
@@ -946,9 +990,10 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
       // latency of the atomic does not sit between two items.
       // The first item is the CTA's own number; the counter, which the delta pre-pass has zeroed, hands out the rest.
       int drawn = blockIdx.x;
-      if (GEN && a.mask_pure) {  // (the lengths come from the pre-pass)
+      if (PACKED || (MASK && a.mask_pure)) {  // (the items or the lengths come from a kernel before)
         ptx::grid_dep_wait();
         dep_waited = true;
+        if (PACKED) read_plan();
       }
       auto draw = [&]() {
         if (!dep_waited) ptx::grid_dep_wait();
@@ -970,10 +1015,10 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
               void* base = t == 0 ? a.dv : a.dk;
               const Str3& st = t == 0 ? a.dvs : a.dks;
               if (!base || PARTS) continue;  // (of a divided key tile the last kernel knows which parts exist)
-              T* out = reinterpret_cast<T*>(base) + it.b * st.b + it.hk * st.h;
+              T* out = reinterpret_cast<T*>(base) + it.b * st.b + it.hk * st.h + (PACKED ? it.k0 * st.s : 0);
               for (int e = lane; e < BM * (D / 8); e += 32) {
                 const int row = it.kv0 + e / (D / 8);
-                if (row < a.Skv)
+                if (row < (PACKED ? it.lk : a.Skv))
                   *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row) * st.s + (e % (D / 8)) * 8) =
                       make_uint4(0, 0, 0, 0);
               }
@@ -983,6 +1028,11 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
           }
         }
         int ok = 1;
+        const CUtensorMap *mq = &tmQ, *mk = &tmK, *mv = &tmV, *mdo = &tmdO;
+        if (PACKED && w >= 0) {
+          mq = map_of(it.seq, kMapQ), mk = map_of(it.seq, kMapK), mv = map_of(it.seq, kMapV), mdo = map_of(it.seq, kMapdO);
+          if (lane == 0) ptx::tensormap_acquire(mq), ptx::tensormap_acquire(mk), ptx::tensormap_acquire(mv), ptx::tensormap_acquire(mdo);
+        }
         if (lane == 0) {
           const int slot = i & 1;
           ok = ptx::mbar_wait(&ctl->item_empty[slot], ((i >> 1) & 1) ^ 1, abort_flag);
@@ -994,15 +1044,15 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
           if (ok && w >= 0) ok = ptx::mbar_wait(&ctl->kv_empty[slot], ((i >> 1) & 1) ^ 1, abort_flag);
           if (ok && w >= 0) {
             ptx::mbar_arrive_expect_tx(&ctl->kv_full[slot], 2 * TB);
-            ptx::tma_load_4d(sKV + slot * 2 * TB, &tmK, &ctl->kv_full[slot], 0, it.kv0, it.hk, it.b);
-            ptx::tma_load_4d(sKV + slot * 2 * TB + TB, &tmV, &ctl->kv_full[slot], 0, it.kv0, it.hk, it.b);
+            ptx::tma_load_4d(sKV + slot * 2 * TB, mk, &ctl->kv_full[slot], 0, it.kv0, it.hk, it.b);
+            ptx::tma_load_4d(sKV + slot * 2 * TB + TB, mv, &ctl->kv_full[slot], 0, it.kv0, it.hk, it.b);
           }
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok || w < 0) break;
-        for (int n = 0; n < it.n_steps; ++n, advance(it.h, it.qt, it.qt_begin)) {
+        for (int n = 0; n < it.n_steps; ++n, advance(it.h, it.qt, it)) {
           if (redraw && n + 1 == it.n_steps) draw();
-          if (GEN && it.mask) prefetch_mask(a, it.b, it.h, it.qt * BQ, it.kv0, lane);
+          if (MASK && it.mask) prefetch_mask(a, it.b, it.h, it.qt * BQ, it.kv0, lane);
           const uint32_t g = gq + n;
           const int st = g % NQ;
           const int h = it.h, q0 = it.qt * BQ;
@@ -1010,12 +1060,12 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
             ok = ptx::mbar_wait(&ctl->q_empty[st], ((g / NQ) & 1) ^ 1, abort_flag);
             if (ok) {
               ptx::mbar_arrive_expect_tx(&ctl->q_full[st], TB);
-              ptx::tma_load_4d(sQ + st * TB, &tmQ, &ctl->q_full[st], 0, q0, h, it.b);
+              ptx::tma_load_4d(sQ + st * TB, mq, &ctl->q_full[st], 0, q0, h, it.b);
               ok = ptx::mbar_wait(&ctl->do_empty[g & 1], ((g >> 1) & 1) ^ 1, abort_flag);
             }
             if (ok) {
               ptx::mbar_arrive_expect_tx(&ctl->do_full[g & 1], TB);
-              ptx::tma_load_4d(sdO + (g & 1) * TB, &tmdO, &ctl->do_full[g & 1], 0, q0, h, it.b);
+              ptx::tma_load_4d(sdO + (g & 1) * TB, mdo, &ctl->do_full[g & 1], 0, q0, h, it.b);
             }
             // The vectors' buffer was last read in step g - 2.  (A barrier per buffer: it cannot complete its next
             // phase before this warp has written the buffer again, so the parity below is never ambiguous, as it
@@ -1031,13 +1081,13 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
             dep_waited = true;
           }
           float lv[4], dl[4];
-          const int64_t base = (static_cast<int64_t>(it.b) * a.Hq + h) * a.Lq + q0;
+          const int64_t base = (static_cast<int64_t>(it.b) * a.Hq + h) * a.Lq + (PACKED ? it.q0 : 0) + q0;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int row = j * 32 + lane;
             lv[j] = -INFINITY;  // rows beyond Lq behave like rows without any participating key: P = 0
             dl[j] = 0.f;
-            if (q0 + row < a.Lq) {
+            if (q0 + row < (PACKED ? it.lq : a.Lq)) {
               lv[j] = a.lse[base + row];
               dl[j] = a.delta[base + row];
             }
@@ -1180,7 +1230,12 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
       Item it = ctl->item[slot];
       ptx::mbar_arrive(&ctl->item_empty[slot]);
       if (!ok || it.n_steps < 0) break;
-      for (int n = 0; n < it.n_steps; ++n, ++g, advance(it.h, it.qt, it.qt_begin)) {
+      const CUtensorMap *mdq = &tmdQ, *mdk = &tmdK, *mdv = &tmdV;
+      if constexpr (PACKED) {
+        mdq = map_of(it.seq, kMapdQ), mdk = map_of(it.seq, kMapdK), mdv = map_of(it.seq, kMapdV);
+        if (lane == 0) ptx::tensormap_acquire(mdq), ptx::tensormap_acquire(mdk), ptx::tensormap_acquire(mdv);
+      }
+      for (int n = 0; n < it.n_steps; ++n, ++g, advance(it.h, it.qt, it)) {
         if (n + 1 == it.n_steps) {
           // dV, then dK: complete once the last step's products are (before its dQ); through the warp's staging
           // box (as [32 key rows][64 elements]) and a TMA store: coalesced, rows beyond Skv clipped
@@ -1219,11 +1274,11 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
             if (!PARTS && !half) continue;
             ptx::fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0 && ok && (is_v ? a.dv != nullptr : a.dk != nullptr) && it.kv0 + wj * 32 < a.Skv) {
+            if (lane == 0 && ok && (is_v ? a.dv != nullptr : a.dk != nullptr) && it.kv0 + wj * 32 < (PACKED ? it.lk : a.Skv)) {
               if (PARTS)
                 ptx::tma_store_4d(is_v ? &tmdV : &tmdK, box, (c & 1) * 32, it.kv0 + wj * 32, it.b * a.Hkv + it.hk, it.part);
               else
-                ptx::tma_store_4d(is_v ? &tmdV : &tmdK, box, 0, it.kv0 + wj * 32, it.hk, it.b);
+                ptx::tma_store_4d(is_v ? mdv : mdk, box, 0, it.kv0 + wj * 32, it.hk, it.b);
               ptx::bulk_commit();
             }
           }
@@ -1248,8 +1303,8 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
                 make_uint4(v[ch * 4 + 0], v[ch * 4 + 1], v[ch * 4 + 2], v[ch * 4 + 3]);
           ptx::fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0 && ok && q0 < a.Lq) {
-            ptx::tma_reduce_add_4d(&tmdQ, box, cc * 32, q0, h, it.b);
+          if (lane == 0 && ok && q0 < (PACKED ? it.lq : a.Lq)) {
+            ptx::tma_reduce_add_4d(mdq, box, cc * 32, q0, h, it.b);
             ptx::bulk_commit();
           }
         }
@@ -1279,13 +1334,13 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
         const int q = qt * BQ + wg * 32 + sc * 16;
         fetch_mask(a.mask, it.b * a.mask.sb + h * a.mask.sh + q * a.mask.sl + kv_row, kv_row < a.Skv ? a.Lq - q : 0, mw[sc]);
       };
-      for (int n = 0; n < it.n_steps; ++n, ++g, advance(it.h, it.qt, it.qt_begin)) {
+      for (int n = 0; n < it.n_steps; ++n, ++g, advance(it.h, it.qt, it)) {
         const int hq = it.h, q0 = it.qt * BQ;
         const float* vec = svec + (g & 1) * 2 * BQ;
         // some (query, key) pairs of this step are hidden: the diagonal step, a ragged last key tile
         const bool diag = a.causal && q0 + it.shift < it.kv0 + BM;
         const bool masked = diag || it.kv0 + BM > it.kv_len;
-        if (GEN && it.mask) fetch(0, hq, it.qt), fetch(1, hq, it.qt);
+        if (MASK && it.mask) fetch(0, hq, it.qt), fetch(1, hq, it.qt);
         if (ok) ok = ptx::mbar_wait(&ctl->vec_full[g & 1], (g >> 1) & 1, abort_flag);
         // phase 1: P^T from S^T; P stays in registers for phase 2
         if (ok) ok = ptx::mbar_wait(&ctl->s_full, g & 1, abort_flag);
@@ -1299,7 +1354,7 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
           uint32_t pk[8];
           int n_hidden = 0;
           if (masked) n_hidden = kv_row >= it.kv_len ? 16 : (diag ? kv_row - (q0 + col + it.shift) : 0);
-          p_chunk<BF16, GEN, T>(a, p[sc], vec + col, c2v, n_hidden, GEN && it.mask, mw[sc], pk);
+          p_chunk<BF16, MASK, T>(a, p[sc], vec + col, c2v, n_hidden, MASK && it.mask, mw[sc], pk);
           // Warpgroup w keeps its 16-bit results in columns [32w, 32w+16) of the region, i.e. over the first 16
           // columns it loaded itself, never over columns another warpgroup still has to read.
           ptx::tmem_st8(tA + lane_addr + wg * 32 + sc * 8, pk);
@@ -1439,8 +1494,8 @@ cudaError_t launch_t(const BwdArgs& a, int dtype, int device, cudaStream_t strea
     return cudaErrorInvalidValue;
   cudaError_t e;  // (dq_accum has been cleared by the delta pre-pass)
   void (*kern)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, BwdArgs);
-  if constexpr (D == 64) kern = a.parts > 1 ? bwd_tc64_kernel<BF16, GEN, true> : bwd_tc64_kernel<BF16, GEN, false>;
-  else kern = a.parts > 1 ? bwd_tc_kernel<BF16, GEN, true> : bwd_tc_kernel<BF16, GEN, false>;
+  if constexpr (D == 64) kern = a.parts > 1 ? bwd_tc64_kernel<BF16, GEN, true, false> : bwd_tc64_kernel<BF16, GEN, false, false>;
+  else kern = a.parts > 1 ? bwd_tc_kernel<BF16, GEN, true, false> : bwd_tc_kernel<BF16, GEN, false, false>;
   constexpr int kSmemBytes = D == 64 ? Cfg64::kSmem : Cfg128::kSmem;
   constexpr int kBlock = D == 64 ? Cfg64::kThreads : Cfg128::kThreads;
   e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
@@ -1468,7 +1523,64 @@ cudaError_t launch_t(const BwdArgs& a, int dtype, int device, cudaStream_t strea
   return launch_early(dq_convert_kernel<T, D>, dim3(blocks), dim3(256), 0, stream, 1, a);
 }
 
+// Packed sequences: the plan, the delta pre-pass over all rows as one sequence (it clears dQ's accumulator), the main kernel and
+// the conversion of dQ, again over all rows.
+template <int D, bool BF16, bool GEN>
+cudaError_t launch_packed(BwdArgs a, const PackedCall& c, int dtype, int device, cudaStream_t stream) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  constexpr int kOutRows = D == 64 ? 32 : 128;
+  const int sms = sm_count(device);
+  PackedPlan p{};
+  p.cu_q = c.cu_q, p.cu_k = c.cu_k, p.n = c.n, p.total_q = a.Lq, p.total_k = c.total_k;
+  p.group = a.Hq / a.Hkv, p.causal = a.causal, p.bwd = true, p.step = 1, p.status = a.status;
+  // (an absent output gets a map that is never used)
+  const Str3 accum{0, static_cast<int64_t>(a.Lq) * D, D};
+  const void* ptr[kPackedBwdMaps] = {a.q, a.k, a.v, a.d_o, a.dq_accum, a.dk ? a.dk : a.k, a.dv ? a.dv : a.v};
+  const Str3* st[kPackedBwdMaps] = {&a.qs, &a.ks, &a.vs, &a.dos, &accum, a.dk ? &a.dks : &a.ks, a.dv ? &a.dvs : &a.vs};
+  for (int m = 0; m < kPackedBwdMaps; ++m) {
+    const bool of_k = m == kMapK || m == kMapV || m == kMapdK || m == kMapdV;
+    const bool made = m == kMapdQ ? make_map_f32(&p.base[m], a.dq_accum, D, a.Lq, a.Hq, 1, D == 64 ? 32 : 128)
+                                  : make_map(&p.base[m], dtype, ptr[m], D, of_k ? a.Skv : a.Lq, of_k ? a.Hkv : a.Hq, 1, *st[m],
+                                             m == kMapdK || m == kMapdV ? kOutRows : 128);
+    if (!made) return cudaErrorInvalidValue;
+    p.of_k[m] = of_k, p.address[m] = static_cast<const char*>(ptr[m]), p.row_bytes[m] = st[m]->s * (m == kMapdQ ? 4 : 2);
+  }
+  p.n_maps = kPackedBwdMaps;
+  if (a.dk) p.zero[p.n_zero++] = PackedPlan::Rows{static_cast<char*>(a.dk), a.dks.s * 2, a.dks.h * 2, a.Hkv, D * 2, true};
+  if (a.dv) p.zero[p.n_zero++] = PackedPlan::Rows{static_cast<char*>(a.dv), a.dvs.s * 2, a.dvs.h * 2, a.Hkv, D * 2, true};
+  cudaError_t e = launch_packed_plan(p, c.scratch, &a.packed, stream);
+  if (e != cudaSuccess) return e;
+  a.parts = 1;
+  BwdArgs pre = a;
+  pre.zero_dq_accum = 1;
+  e = launch_bwd_delta(dtype, D, pre, stream);
+  if (e != cudaSuccess) return e;
+  void (*kern)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, BwdArgs);
+  if constexpr (D == 64) kern = bwd_tc64_kernel<BF16, GEN, false, true>;
+  else kern = bwd_tc_kernel<BF16, GEN, false, true>;
+  constexpr int kSmemBytes = D == 64 ? Cfg64::kSmem : Cfg128::kSmem;
+  constexpr int kBlock = D == 64 ? Cfg64::kThreads : Cfg128::kThreads;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  if (e != cudaSuccess) return e;
+  const size_t most = packed_items(c.n, a.Skv, 1, 1) * a.Hkv;
+  e = launch_early(kern, dim3(static_cast<unsigned>(most < static_cast<size_t>(sms) ? most : sms)), dim3(kBlock), kSmemBytes, stream, 1,
+                   p.base[kMapQ], p.base[kMapK], p.base[kMapV], p.base[kMapdO], p.base[kMapdQ], p.base[kMapdK], p.base[kMapdV], a);
+  if (e != cudaSuccess || !a.dq) return e;
+  const int64_t total = static_cast<int64_t>(a.Hq) * a.Lq * (D / 8), blocks = (total + 255) / 256;
+  return launch_early(dq_convert_kernel<T, D>, dim3(static_cast<unsigned>(blocks < 8 * sms ? blocks : 8 * sms)), dim3(256), 0, stream, 1, a);
+}
+
 }  // namespace
+
+cudaError_t launch_bwd_packed(int dtype, int D, const BwdArgs& a, const PackedCall& c, int device, cudaStream_t stream) {
+  const bool bf = dtype == TT_ATTN_BF16, general = a.causal == TT_ATTN_CAUSAL_BOTTOM_RIGHT;
+  if (D == 128) {
+    if (general) return bf ? launch_packed<128, true, true>(a, c, dtype, device, stream) : launch_packed<128, false, true>(a, c, dtype, device, stream);
+    return bf ? launch_packed<128, true, false>(a, c, dtype, device, stream) : launch_packed<128, false, false>(a, c, dtype, device, stream);
+  }
+  if (general) return bf ? launch_packed<64, true, true>(a, c, dtype, device, stream) : launch_packed<64, false, true>(a, c, dtype, device, stream);
+  return bf ? launch_packed<64, true, false>(a, c, dtype, device, stream) : launch_packed<64, false, false>(a, c, dtype, device, stream);
+}
 
 template <bool GEN>
 cudaError_t launch_g(int dtype, int D, const BwdArgs& a, int device, cudaStream_t stream) {

@@ -20,8 +20,9 @@ constexpr int kSms = 148;
 // Status bits a kernel may OR into the caller's status word.
 constexpr int kStatusWaitExpired = 1;
 constexpr int kStatusBadSmemAlign = 2;   // dynamic shared memory did not start on a 1024-byte boundary
-constexpr int kStatusCacheFull = 4;      // decode-append: no free row in the cache of some sequence
-constexpr int kStatusRopeRange = 8;      // decode-append: position beyond the rotary tables
+constexpr int kStatusCacheFull = 4;      // no free row in the cache of some sequence
+constexpr int kStatusRopeRange = 8;      // position beyond the rotary tables
+constexpr int kStatusBadOffsets = 16;    // packed sequences: offsets that fall or leave the rows; cacheAccept: a draft that does not exist
 
 // two values, rounded to the 16-bit type, in one register
 template <bool BF16>
@@ -52,6 +53,19 @@ struct MaskArgs {
   bool wide;        // every row starts on a 16-byte boundary
 };
 
+// Packed sequences (packed_plan.cu): work items, the longest walks first, and the tensor maps of every sequence.
+struct PackedEntry {
+  int q0, lq, k0, lk;  // the sequence's rows of q and of k
+  int x;               // forward: its first query block (query tile * group + head of the group); backward: its key tile
+  int seq, walk, reserved;
+};
+struct PackedArgs {
+  const PackedEntry* items;
+  const int* n_items;
+  const void* maps;  // CUtensorMap [sequence][kPackedFwdMaps or kPackedBwdMaps]
+};
+enum PackedMap { kMapQ, kMapK, kMapV, kMapO, kPackedFwdMaps, kMapdO = kMapO, kMapdQ, kMapdK, kMapdV, kPackedBwdMaps };
+
 // Arguments common to the prefill kernels.
 struct FwdArgs {
   const void* q;
@@ -69,6 +83,7 @@ struct FwdArgs {
   int* sched;  // tensor-core path: work counter in scratch memory
   int32_t* mask_lens;        // tensor-core path: scratch of 2 B integers for masked_lens, or null: a padding mask is read in full
   const int32_t* mask_pure;  // with masked_lens: whether the mask is all true up to the length
+  PackedArgs packed;         // packed sequences: B = 1, Lq and Skv are the rows of all of them
 };
 
 struct BwdArgs {
@@ -100,6 +115,7 @@ struct BwdArgs {
   MaskArgs mask;
   int32_t* mask_lens;        // as in FwdArgs
   const int32_t* mask_pure;  // as in FwdArgs
+  PackedArgs packed;         // as in FwdArgs
 };
 
 struct DecodeArgs {

@@ -46,6 +46,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "packed.cuh"
 #include "ptx.cuh"
 #include "tma_host.cuh"
 
@@ -71,6 +72,7 @@ struct Item {
   int j0, nt[QT];              // first key tile, and how many each half walks from there (KEYS: in turn)
   int n_max;                   // the longer walk; -1: no more items
   int mask;                    // whether the mask has to be looked at
+  int q0, lq, seq;             // packed: the sequence, its first row of q and how many
 };
 
 struct __align__(16) SmemCtl {
@@ -99,7 +101,8 @@ constexpr int smem_bytes() {
 // GEN: 1: the variant for a causal triangle that is not top-left aligned, 2: that and a mask; the fast variant (0) compiles
 // all of that out.
 // KEYS: `per_head` items (query blocks) per (batch, kv head), `rank` of `cluster` shares of the key tiles; else pairs.
-template <int GEN, bool KEYS>
+// PACKED: a head's items are those of all sequences, as the plan has sorted them.
+template <int GEN, bool KEYS, bool PACKED>
 __device__ __forceinline__ Item decode_item(const FwdArgs& a, int w, int per_head, int rank = 0, int cluster = 1) {
   Item it;
   // Heads in order, the longest (latest causal) pair of a head first: the CTAs running at any moment share few
@@ -122,15 +125,19 @@ __device__ __forceinline__ Item decode_item(const FwdArgs& a, int w, int per_hea
   }
   it.b = bh / a.Hkv;
   it.hk = bh - it.b * a.Hkv;
-  int kv_len = a.Skv;
-  if (a.kv_lens) {
+  int kv_len = a.Skv, Lq = a.Lq, first = KEYS ? mp : mp * QT;
+  if constexpr (PACKED) {
+    const int4* e = reinterpret_cast<const int4*>(a.packed.items + (per_head - 1 - mp));
+    const int4 rows = __ldg(e), place = __ldg(e + 1);
+    it.q0 = rows.x, it.lq = Lq = rows.y, kv_len = rows.w, first = place.x, it.seq = place.y;
+  } else if (a.kv_lens) {
     int l = a.kv_lens[it.b];
     kv_len = l < 0 ? 0 : (l < a.Skv ? l : a.Skv);
   }
   it.kv_len = kv_len;
   it.mask = GEN == 2 && !(a.mask_pure && a.mask_pure[it.b]);
-  it.shift = GEN ? causal_shift(a.causal, kv_len, a.Lq) : 0;  // key j participates iff j <= i + shift
-  const int x = KEYS ? mp : mp * QT, qt0 = x / group, qt1 = KEYS ? qt0 : (x + 1) / group;
+  it.shift = GEN ? causal_shift(a.causal, kv_len, Lq) : 0;  // key j participates iff j <= i + shift
+  const int x = first, qt0 = x / group, qt1 = KEYS ? qt0 : (x + 1) / group;
   it.h[0] = it.hk * group + x - qt0 * group, it.h[1] = KEYS ? it.h[0] : it.hk * group + x + 1 - qt1 * group;
   it.row0[0] = qt0 * BM, it.row0[1] = qt1 * BM;
   // key tiles that a block sees (0 for one wholly beyond Lq)
@@ -141,7 +148,7 @@ __device__ __forceinline__ Item decode_item(const FwdArgs& a, int w, int per_hea
       if (GEN) c = c > 0 ? c : 0;
       if (c < e) e = c;
     }
-    return row0 < a.Lq ? (e + BN - 1) / BN : 0;
+    return row0 < Lq ? (e + BN - 1) / BN : 0;
   };
   it.j0 = 0;
   if constexpr (KEYS) {
@@ -324,7 +331,7 @@ __device__ __forceinline__ void combine_rows(const FwdArgs& a, const Item& it, i
   }
 }
 
-template <int D, bool BF16, int GEN, bool KEYS>
+template <int D, bool BF16, int GEN, bool KEYS, bool PACKED>
 __global__ void __launch_bounds__(kThreads, 1)
     fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
@@ -343,10 +350,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
-  const int n_blocks = (a.Lq + BM - 1) / BM * (a.Hq / a.Hkv), per_head = KEYS ? n_blocks : (n_blocks + QT - 1) / QT;
-  const int n_items = per_head * a.Hkv * a.B;
-  const int rank = KEYS && cluster > 1 ? static_cast<int>(ptx::cluster_rank()) : 0;
-  auto item_of = [&](int w) { return KEYS ? decode_item<GEN, true>(a, w, per_head, rank, cluster) : decode_item<GEN, false>(a, w, per_head); };
+  const int n_blocks = (a.Lq + BM - 1) / BM * (a.Hq / a.Hkv);
+  int per_head = KEYS ? n_blocks : (n_blocks + QT - 1) / QT;  // (packed: the producer asks the plan)
+  const int rank = KEYS && !PACKED && cluster > 1 ? static_cast<int>(ptx::cluster_rank()) : 0;
+  auto item_of = [&](int w) {
+    return KEYS ? decode_item<GEN, true, PACKED>(a, w, per_head, rank, cluster) : decode_item<GEN, false, PACKED>(a, w, per_head);
+  };
+  // packed: the maps of an item's sequence, which the plan has made, instead of those of the whole tensors
+  auto map_of = [&](int seq, int which) { return static_cast<const CUtensorMap*>(a.packed.maps) + seq * static_cast<int64_t>(kPackedFwdMaps) + which; };
 
   constexpr int HALVES = D / 64;  // 64-element (128-byte) column blocks per row
   constexpr int HALF_BYTES = BM * 128;
@@ -405,6 +416,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         uint32_t g = 0;             // K/V tiles requested so far (ring position)
         uint32_t qc0 = 0, qc1 = 0;  // items whose Q tile 0 / 1 was requested so far
+        if (PACKED) per_head = *a.packed.n_items;
+        const int n_items = per_head * a.Hkv * a.B;
         for (uint32_t i = 0;; ++i) {
           // the first item is the CTA's own number; the counter, where one is needed, hands out the rest
           int w;
@@ -422,6 +435,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           ptx::mbar_arrive(&ctl->item_full[slot]);
           if (w < 0) break;
           if (it.n_max == 0) continue;
+          const CUtensorMap *mq = &tmQ, *mk = &tmK, *mv = &tmV;
+          if constexpr (PACKED) {
+            mq = map_of(it.seq, kMapQ), mk = map_of(it.seq, kMapK), mv = map_of(it.seq, kMapV);
+            ptx::tensormap_acquire(mq), ptx::tensormap_acquire(mk), ptx::tensormap_acquire(mv);
+          }
           bool ok = true;
           // a Q tile is loaded only if it has key tiles to walk; tile 0 goes first and, with the first K tile,
           // ahead of tile 1: the issuer starts tile 0 of this item while tile 1 of the previous one still works
@@ -431,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ptx::mbar_arrive_expect_tx(&ctl->q_full[t], TB);
 #pragma unroll
             for (int hf = 0; hf < HALVES; ++hf)
-              ptx::tma_load_4d(sQ + t * TB + hf * HALF_BYTES, &tmQ, &ctl->q_full[t], hf * 64,
+              ptx::tma_load_4d(sQ + t * TB + hf * HALF_BYTES, mq, &ctl->q_full[t], hf * 64,
                               t == 0 ? it.row0[0] : it.row0[1], t == 0 ? it.h[0] : it.h[1], it.b);
             ++qc;
             return true;
@@ -450,10 +468,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ptx::tma_load_4d(dst + st * TB + hf * HALF_BYTES, map, &full[st], hf * 64, (it.j0 + j) * BN, it.hk, it.b);
               return true;
             };
-            ok = load(sK, &tmK, ctl->k_full, ctl->k_empty, 0);
+            ok = load(sK, mk, ctl->k_full, ctl->k_empty, 0);
             for (int j = 0; j < n && ok; ++j) {
-              if (j + 1 < n) ok = load(sK, &tmK, ctl->k_full, ctl->k_empty, j + 1);
-              if (ok) ok = load(sV, &tmV, ctl->v_full, ctl->v_empty, j);
+              if (j + 1 < n) ok = load(sK, mk, ctl->k_full, ctl->k_empty, j + 1);
+              if (ok) ok = load(sV, mv, ctl->v_full, ctl->v_empty, j);
             }
             if (!ok) break;
             g += n;
@@ -465,13 +483,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               ptx::mbar_arrive_expect_tx(&ctl->k_full[st], TB);
 #pragma unroll
               for (int hf = 0; hf < HALVES; ++hf)
-                ptx::tma_load_4d(sK + st * TB + hf * HALF_BYTES, &tmK, &ctl->k_full[st], hf * 64, (it.j0 + j) * BN, it.hk, it.b);
+                ptx::tma_load_4d(sK + st * TB + hf * HALF_BYTES, mk, &ctl->k_full[st], hf * 64, (it.j0 + j) * BN, it.hk, it.b);
               if (j == 0 && !(ok = load_q(1, qc1))) break;
               if (!(ok = ptx::mbar_wait(&ctl->v_empty[st], ph ^ 1, abort_flag))) break;
               ptx::mbar_arrive_expect_tx(&ctl->v_full[st], TB);
 #pragma unroll
               for (int hf = 0; hf < HALVES; ++hf)
-                ptx::tma_load_4d(sV + st * TB + hf * HALF_BYTES, &tmV, &ctl->v_full[st], hf * 64, (it.j0 + j) * BN, it.hk, it.b);
+                ptx::tma_load_4d(sV + st * TB + hf * HALF_BYTES, mv, &ctl->v_full[st], hf * 64, (it.j0 + j) * BN, it.hk, it.b);
             }
           }
           if (!ok) break;
@@ -680,17 +698,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       const volatile Item* pub = &ctl->item[slot];
       const int b = pub->b, kv_len = pub->kv_len, shift = pub->shift, j0 = pub->j0, n_max = pub->n_max;
       const int n_t = pub->nt[t], tile_row0 = pub->row0[t], head = pub->h[t];
+      const int q0 = PACKED ? pub->q0 : 0, lq = PACKED ? pub->lq : a.Lq;
+      const CUtensorMap* mo = &tmO;
+      if constexpr (PACKED) mo = map_of(pub->seq, kMapO);
       const bool use_mask = GEN == 2 && pub->mask;
       if (!KEYS) ptx::mbar_arrive(&ctl->item_empty[slot]);  // (KEYS: read again after the walk, and then handed back)
       if (n_max < 0) break;
-      const int row = tile_row0 + r_in;  // global query row of this thread
-      T* orow = reinterpret_cast<T*>(a.o) + b * a.os.b + head * a.os.h + static_cast<int64_t>(row) * a.os.s;
-      float* lse_row = a.lse ? a.lse + (static_cast<int64_t>(b) * a.Hq + head) * a.Lq + row : nullptr;
+      const int row = tile_row0 + r_in;  // query row of this thread
+      T* orow = reinterpret_cast<T*>(a.o) + b * a.os.b + head * a.os.h + static_cast<int64_t>(q0 + row) * a.os.s;
+      float* lse_row = a.lse ? a.lse + (static_cast<int64_t>(b) * a.Hq + head) * a.Lq + q0 + row : nullptr;
+      if (PACKED && n_max > 0 && r_in == 0) ptx::tensormap_acquire(mo);
 
       if (KEYS ? cluster == 1 && n_max == 0 : n_t == 0) {
         if (KEYS) ptx::mbar_arrive(&ctl->item_empty[slot]);
         // no participating key (or tile beyond Lq): O = 0, LSE = -inf
-        if (row < a.Lq && (!KEYS || t == 0)) {
+        if (row < lq && (!KEYS || t == 0)) {
 #pragma unroll
           for (int e = 0; e < D; e += 8) *reinterpret_cast<uint4*>(orow + e) = make_uint4(0, 0, 0, 0);
           if (lse_row) *lse_row = -INFINITY;
@@ -914,11 +936,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           ptx::fence_proxy_async_smem();
           ptx::named_barrier(1 + t, BM);
           if (r_in == 0) {
-            ptx::tma_store_4d(&tmO, stage, c0, tile_row0, head, b);
+            ptx::tma_store_4d(mo, stage, c0, tile_row0, head, b);
             ptx::bulk_commit();
           }
         }
-        if (t == 0 && row < a.Lq && lse_row) *lse_row = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        if (t == 0 && row < lq && lse_row) *lse_row = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
         continue;
       }
 
@@ -959,16 +981,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::fence_proxy_async_smem();
         ptx::named_barrier(1 + t, BM);
         if (r_in == 0 && ok) {
-          ptx::tma_store_4d(&tmO, stage, hf * 64, tile_row0, head, b);
+          ptx::tma_store_4d(mo, stage, hf * 64, tile_row0, head, b);
           ptx::bulk_commit();
         }
       }
-      if (ok && row < a.Lq && lse_row) *lse_row = l > 0.f ? (m_ref + log2f(l)) * kLn2 : -INFINITY;
+      if (ok && row < lq && lse_row) *lse_row = l > 0.f ? (m_ref + log2f(l)) * kLn2 : -INFINITY;
     }
     if (r_in == 0) ptx::bulk_wait_all();
   }
 
-  if (KEYS && cluster > 1) {
+  if (KEYS && !PACKED && cluster > 1) {
     __syncwarp();
     ptx::cluster_sync();
     if (warp < 8 && *abort_flag == 0) {
@@ -995,13 +1017,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------ host ----
-template <int D, bool BF16, int GEN, bool KEYS>
+template <int D, bool BF16, int GEN, bool KEYS, bool PACKED = false>
 cudaError_t launch_k(const FwdArgs& a, int dtype, int grid, int cluster, cudaStream_t stream) {
   CUtensorMap tq, tk, tv, to;
   if (!make_map(&tq, dtype, a.q, D, a.Lq, a.Hq, a.B, a.qs) || !make_map(&tk, dtype, a.k, D, a.Skv, a.Hkv, a.B, a.ks) ||
       !make_map(&tv, dtype, a.v, D, a.Skv, a.Hkv, a.B, a.vs) || !make_map(&to, dtype, a.o, D, a.Lq, a.Hq, a.B, a.os))
     return cudaErrorInvalidValue;
-  auto kern = fwd_tc_kernel<D, BF16, GEN, KEYS>;
+  auto kern = fwd_tc_kernel<D, BF16, GEN, KEYS, PACKED>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D, GEN>());
   if (e != cudaSuccess) return e;
   return launch_early(kern, dim3(grid), dim3(kThreads), smem_bytes<D, GEN>(), stream, cluster, tq, tk, tv, to, a, cluster);
@@ -1016,7 +1038,7 @@ int cluster_slots(int device, int cluster) {
   std::atomic<int>& k = known[device][cluster == 2 ? 0 : (cluster == 4 ? 1 : 2)];
   int n = k.load(std::memory_order_relaxed);
   if (n == 0) {
-    auto kern = fwd_tc_kernel<D, BF16, GEN, true>;
+    auto kern = fwd_tc_kernel<D, BF16, GEN, true, false>;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
@@ -1116,7 +1138,46 @@ cudaError_t launch_t(FwdArgs a, int dtype, int device, cudaStream_t stream) {
                 : launch_k<D, BF16, GEN, false>(a, dtype, grid, 1, stream);
 }
 
+// Packed sequences.  The host does not know their lengths: it divides the work into single blocks, half the steps each, where
+// there are few for the machine even if the rows were one sequence, else into pairs.
+template <int D, bool BF16, int GEN>
+cudaError_t launch_packed(FwdArgs a, const PackedCall& c, int dtype, int device, cudaStream_t stream) {
+  const int group = a.Hq / a.Hkv, sms = sm_count(device);
+  const size_t blocks = packed_items(c.n, a.Lq, group, 1) * a.Hkv;
+  const bool keys = false;
+  PackedPlan p{};
+  p.cu_q = c.cu_q, p.cu_k = c.cu_k, p.n = c.n, p.total_q = a.Lq, p.total_k = c.total_k;
+  p.group = group, p.causal = a.causal, p.step = keys ? 1 : QT, p.sched = a.sched, p.status = a.status;
+  const void* ptr[kPackedFwdMaps] = {a.q, a.k, a.v, a.o};
+  const Str3* st[kPackedFwdMaps] = {&a.qs, &a.ks, &a.vs, &a.os};
+  for (int m = 0; m < kPackedFwdMaps; ++m) {
+    p.of_k[m] = m == kMapK || m == kMapV;
+    if (!make_map(&p.base[m], dtype, ptr[m], D, p.of_k[m] ? a.Skv : a.Lq, p.of_k[m] ? a.Hkv : a.Hq, 1, *st[m])) return cudaErrorInvalidValue;
+    p.address[m] = static_cast<const char*>(ptr[m]), p.row_bytes[m] = st[m]->s * 2;
+  }
+  p.n_maps = kPackedFwdMaps;
+  p.zero[0] = PackedPlan::Rows{static_cast<char*>(a.o), a.os.s * 2, a.os.h * 2, a.Hq, D * 2, false};
+  p.n_zero = 1, p.lse = a.lse;
+  cudaError_t e = launch_packed_plan(p, c.scratch, &a.packed, stream);
+  if (e != cudaSuccess) return e;
+  const int grid = static_cast<int>(blocks < static_cast<size_t>(sms) ? blocks : sms);
+  return keys ? launch_k<D, BF16, GEN, true, true>(a, dtype, grid, 1, stream) : launch_k<D, BF16, GEN, false, true>(a, dtype, grid, 1, stream);
+}
+
 }  // namespace
+
+cudaError_t launch_fwd_packed(int dtype, int D, const FwdArgs& a, const PackedCall& c, int device, cudaStream_t stream) {
+  auto go = [&](auto d, auto bf) {
+    constexpr int DD = decltype(d)::value;
+    constexpr bool BF = decltype(bf)::value;
+    return a.causal == TT_ATTN_CAUSAL_BOTTOM_RIGHT ? launch_packed<DD, BF, 1>(a, c, dtype, device, stream)
+                                                   : launch_packed<DD, BF, 0>(a, c, dtype, device, stream);
+  };
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
+  if (dtype == TT_ATTN_BF16) return D == 64 ? go(D64{}, std::true_type{}) : go(D128{}, std::true_type{});
+  return D == 64 ? go(D64{}, std::false_type{}) : go(D128{}, std::false_type{});
+}
 
 template <int GEN>
 cudaError_t launch_g(int dtype, int D, const FwdArgs& a, int device, cudaStream_t stream) {

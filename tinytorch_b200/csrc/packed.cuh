@@ -1,0 +1,59 @@
+// Packed sequences: what the planning kernel (packed_plan.cu) is asked for by the forward's and the backward's launcher.
+#pragma once
+#include <cuda.h>
+
+#include "common.cuh"
+
+namespace ttattn {
+
+struct PackedPlan {
+  const int32_t* cu_q;  // [n + 1] device
+  const int32_t* cu_k;
+  int n, total_q, total_k;
+  int group, causal;
+  // items: of the forward `step` query blocks (128 rows of one head of a group); of the backward a key tile of 128
+  bool bwd;
+  int step;
+  int shift;            // levels of the sort: key or query tiles of a walk >> shift
+  PackedEntry* items;
+  int* n_items;
+  int* sched;           // set to zero, or null
+  int32_t* status;
+  // tensor maps: those of the whole tensors, and which of them go along with k; rows are dimension 1
+  CUtensorMap base[kPackedBwdMaps];
+  const char* address[kPackedBwdMaps];
+  int64_t row_bytes[kPackedBwdMaps];
+  bool of_k[kPackedBwdMaps];
+  int n_maps;
+  CUtensorMap* maps;
+  // rows behind the last sequence: zeros in these (of 16-byte multiples), and -inf in lse
+  struct Rows {
+    char* ptr;
+    int64_t row_bytes, head_bytes;
+    int heads, bytes;  // bytes of a row of one head
+    bool of_k;
+  } zero[3];
+  int n_zero;
+  float* lse;  // [heads of zero[0]][total_q]
+};
+
+// A call over packed sequences.
+struct PackedCall {
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int n, total_k;
+  void* scratch;  // packed_plan_bytes
+};
+
+// Upper bounds of what a plan takes in scratch memory.
+size_t packed_items(int n, int total, int group, int step);
+size_t packed_plan_bytes(int n, int total_q, int total_k, int group, bool bwd);
+
+// Fills in items, maps and args from `scratch` and enqueues the planning kernel.
+cudaError_t launch_packed_plan(PackedPlan p, void* scratch, PackedArgs* args, cudaStream_t stream);
+
+// The forward and the backward; a's B is 1, its Lq and Skv are the rows of all sequences.
+cudaError_t launch_fwd_packed(int dtype, int D, const FwdArgs& a, const PackedCall& c, int device, cudaStream_t stream);
+cudaError_t launch_bwd_packed(int dtype, int D, const BwdArgs& a, const PackedCall& c, int device, cudaStream_t stream);
+
+}  // namespace ttattn

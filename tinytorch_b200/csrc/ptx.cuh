@@ -164,6 +164,30 @@ __device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* map, int c0, 
                : "memory");
 }
 
+// ----------------------------------------------------- tensor maps in memory --
+// A copy of a tensor map in shared memory (128 bytes, aligned to that) is given another base address or extent by one
+// thread, then goes to global memory by a whole warp.  Whoever uses it there acquires it first, per thread.
+__device__ __forceinline__ void tensormap_set_address(uint32_t smem_map, const void* address) {
+  asm volatile("tensormap.replace.tile.global_address.shared::cta.b1024.b64 [%0], %1;" ::"r"(smem_map),
+               "l"(reinterpret_cast<uint64_t>(address))
+               : "memory");
+}
+template <int DIM>
+__device__ __forceinline__ void tensormap_set_extent(uint32_t smem_map, uint32_t extent) {
+  asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], %1, %2;" ::"r"(smem_map), "n"(DIM), "r"(extent)
+               : "memory");
+}
+__device__ __forceinline__ void tensormap_release(void* global_map, uint32_t smem_map) {
+  asm volatile(
+      "tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned [%0], [%1], 128;" ::"l"(
+          __cvta_generic_to_global(global_map)),
+      "r"(smem_map)
+      : "memory");
+}
+__device__ __forceinline__ void tensormap_acquire(const void* global_map) {
+  asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(reinterpret_cast<uint64_t>(global_map)) : "memory");
+}
+
 // -------------------------------------------------------- thread-block clusters --
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;

@@ -50,6 +50,42 @@ class FuncSDPAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None
 
 
+class FuncSDPAttentionPacked(torch.autograd.Function):
+    """As FuncSDPAttention, for packed sequences (the native node is PackedBackward)."""
+
+    @staticmethod
+    def forward(ctx, query, key, value, cuSeqlens, cuSeqlensK, isCausal, scale):
+        needs_grad = any(ctx.needs_input_grad[:3])
+        o, lse = op.sdpAttentionPackedFwd(query, key, value, cuSeqlens, isCausal, scale, cuSeqlensK, needLse=needs_grad)
+        if needs_grad:
+            ctx.save_for_backward(query, key, value, o, lse, cuSeqlens, cuSeqlensK)
+            ctx.isCausal, ctx.scale = isCausal, scale
+        return o
+
+    @staticmethod
+    def backward(ctx, grad):
+        query, key, value, o, lse, cuSeqlens, cuSeqlensK = ctx.saved_tensors
+        dq, dk, dv = op.sdpAttentionPackedBwd(grad, query, key, value, o, lse, cuSeqlens, ctx.isCausal, ctx.scale, cuSeqlensK,
+                                              needs=ctx.needs_input_grad[:3])
+        return dq, dk, dv, None, None, None, None
+
+
+def sdpAttentionPacked(query, key, value, cuSeqlens, isCausal=False, scale=None, cuSeqlensK=None):
+    """Attention over sequences packed behind one another without padding, differentiable: query [rows, Hq, D], key and
+    value [rows, Hkv, D], float16 / bfloat16; sequence n is the rows cuSeqlens[n] to cuSeqlens[n + 1] (int32 [N + 1] on the device).
+
+    With cuSeqlensK keys have lengths of their own, and isCausal="bottom-right" aligns each sequence's queries to the end of its
+    keys.  Sequences may be empty; rows of no sequence (behind the last, say) give O = 0 and zero gradients.  The reference has padded
+    batches only; each sequence here is what sdpAttention makes of it alone."""
+    if not isinstance(isCausal, str):
+        isCausal = bool(isCausal)
+    o = _capi.native().sdp_attention_packed(query, key, value, cuSeqlens, cuSeqlensK, op._causal_mode(isCausal), scale)
+    if o is NotImplemented:
+        scale = op.default_scale(query.shape[-1]) if scale is None else float(scale)
+        o = FuncSDPAttentionPacked.apply(query, key, value, cuSeqlens, cuSeqlensK, isCausal, scale)
+    return o
+
+
 def sdpAttention(query, key, value, isCausal=False, attnMask=None, dropoutP=0.0, scale=None, kvLens=None):
     """Drop-in for function::sdpAttention (src/Function/FuncNNLayer.h:298-302)."""
     if isCausal and attnMask is not None:

@@ -11,6 +11,9 @@ reference's names, argument meaning and in-place behaviour:
       float16 / bfloat16 on the tensor cores (float32 stays on the library gemm and is refused here),
       with the reference's backward (dX = dY W, dW = dY^T X, db = sum dY) through the same kernel
 
+  qkNormRope(q, k, ...)                       (no counterpart in the reference)
+      the RMS norm of every head of q and k and the rotation to their positions, in one pass, with gradients
+
 All go through the C ABI of libtt_attn.so (include/tt_fused.h) and launch on the
 current CUDA stream of the tensors' device.  None has a CPU implementation here, and - as
 in the reference (FuncFused.h:18,27) - siluMul and fusedAddRmsNorm have no backward.
@@ -28,6 +31,40 @@ def siluMul(x):
 def fusedAddRmsNorm(input, residual, weight, eps):
     """In place: residual += input; input = rmsnorm(residual) * weight.  Returns None, like the reference."""
     _capi.native().add_rms_norm(input, residual, weight, eps)
+
+
+class FuncQkNormRope(torch.autograd.Function):
+    """qkNormRope as a Python autograd function, for what the native node (NormRopeBackward in csrc/binding.cpp) does not do;
+    see function.FuncSDPAttention."""
+
+    @staticmethod
+    def forward(ctx, q, k, qWeight, kWeight, cos, sin, positions, eps, interleaved, sections, status):
+        ctx.save_for_backward(q, k, qWeight, kWeight, cos, sin, positions)
+        ctx.how = eps, interleaved, sections
+        return _capi.native().qk_norm_rope_raw(q, k, qWeight, kWeight, cos, sin, positions, eps, interleaved, sections, status)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        q, k, *rest = ctx.saved_tensors
+        gq = torch.zeros_like(q) if gq is None else gq
+        gk = torch.zeros_like(k) if gk is None else gk
+        return (*_capi.native().qk_norm_rope_bwd(gq, gk, q, k, *rest, *ctx.how, *ctx.needs_input_grad[:4]),) + (None,) * 7
+
+
+def qkNormRope(q, k, qWeight=None, kWeight=None, cos=None, sin=None, positions=None, eps=1e-6, interleaved=False, sections=None,
+               status=None):
+    """The RMS norm of every head of q and k, times a weight [D], and the rotation to the rows' positions -> (q', k').
+
+    q [B, Hq, S, D] and k [B, Hkv, S, D], or packed rows [T, Hq, D] and [T, Hkv, D], with any strides (parts of the projection's
+    output, say); the results are dense in the same order.  Without a weight an operand is not normalised.  cos, sin: fp32
+    tables [positions, D/2] as op.ropeTables makes them, or None for no rotation; positions: int32 [S] or [B, S] ([T]
+    for packed rows).  Pairs are the channels (i, i + D/2), or (2i, 2i + 1) if interleaved.  Positions of several axes (time, height,
+    width): positions [axes, ...] and sections, how many of the D/2 pairs belong to each axis, in order.  A position outside the
+    tables leaves its pairs unrotated and sets bit 8 of status (int32 [1]).  fp32 arithmetic, one rounding."""
+    r = _capi.native().qk_norm_rope(q, k, qWeight, kWeight, cos, sin, positions, eps, interleaved, sections, status)
+    if r is NotImplemented:
+        r = FuncQkNormRope.apply(q, k, qWeight, kWeight, cos, sin, positions, float(eps), bool(interleaved), sections, status)
+    return r
 
 
 def _linear_raw(x2, w, bias, status=None):

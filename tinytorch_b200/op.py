@@ -49,6 +49,19 @@ def sdpAttentionBwd(dO, q, k, v, o, lse, isCausal=False, scale=None, kvLens=None
                                    needs[2], attnMask)
 
 
+def sdpAttentionPackedFwd(q, k, v, cuSeqlens, isCausal=False, scale=None, cuSeqlensK=None, needLse=True, status=None):
+    """Packed sequences (see function.sdpAttentionPacked) -> (O [rows, Hq, D], LSE [Hq, rows] fp32 or None).
+
+    status (int32 [1]): bit 16 is set where the offsets fall, are negative or lie beyond the rows; the result is then zeros."""
+    return _capi.native().packed_fwd(q, k, v, cuSeqlens, cuSeqlensK, _causal_mode(isCausal), scale, needLse, status)
+
+
+def sdpAttentionPackedBwd(dO, q, k, v, o, lse, cuSeqlens, isCausal=False, scale=None, cuSeqlensK=None, needs=(True, True, True)):
+    """Gradients (dQ, dK, dV); entries of `needs` that are False come back as None."""
+    return _capi.native().packed_bwd(dO, q, k, v, o, lse, cuSeqlens, cuSeqlensK, _causal_mode(isCausal), scale, needs[0], needs[1],
+                                     needs[2])
+
+
 def sdpAttentionDecode(q, kCache, vCache, kvLens=None, scale=None, needLse=False, workspace=None):
     """One query per sequence against a KV cache [B,Hkv,capacity,D] -> (O [B,Hq,1,D], LSE [B,Hq] or None)."""
     return _capi.native().decode(q, kCache, vCache, kvLens, scale, needLse, workspace)
