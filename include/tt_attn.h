@@ -312,6 +312,68 @@ TT_ATTN_API int tt_attn_packed_bwd(const tt_attn_packed_bwd_params* p);
 /* kind: TT_ATTN_KIND_FWD or TT_ATTN_KIND_BWD; 0 for any other. */
 TT_ATTN_API size_t tt_attn_packed_workspace_bytes(int kind, int n_seqs, int Hq, int Hkv, int total_q, int total_k, int D);
 
+/* Drafted tokens, arranged in a tree, over a KV cache (speculative decoding's verification step; no counterpart in the
+ * reference): T queries per sequence, each of which sees the first kv_lens[b] rows of the cache and those of the sequence's T
+ * drafts that the mask says (their keys and values, k_draft and v_draft, are not in the cache yet; what is accepted goes there
+ * by tt_attn_cache_accept).  The softmax runs over both.
+ *  - mask: device uint8 [B or 1, T, T], non-zero where draft t (row) sees draft j, its ancestors and itself as a rule;
+ *    columns contiguous, strides in elements (batch 0: the same for all).  NULL: a chain, draft t sees the drafts up to itself.
+ *  - A query that sees nothing gives O = 0, LSE = -inf.  Cache rows at or beyond the length may hold anything; keys and values
+ *    of drafts must be finite (a draft that a query does not see may be multiplied by an exact 0).
+ *  - lse is [B, Hq, T].
+ *  - Limits: T up to TT_ATTN_MAX_DRAFTS, Hq / Hkv up to 128 (Float32: 32); TT_ATTN_ERR_TOO_LARGE beyond.
+ *  - Scratch: tt_attn_tree_workspace_bytes.  Results repeat bit for bit. */
+#define TT_ATTN_MAX_DRAFTS 128
+typedef struct tt_attn_tree_params {
+  uint32_t struct_size;
+  int32_t dtype;
+  int32_t B, Hq, Hkv, T, capacity, D;
+  const void* q;       /* [B, Hq, T, D] */
+  const void* k_draft; /* [B, Hkv, T, D] */
+  const void* v_draft;
+  const void* k; /* [B, Hkv, capacity, D] */
+  const void* v;
+  void* o;    /* [B, Hq, T, D] */
+  float* lse; /* or NULL */
+  tt_attn_strides q_strides, k_draft_strides, v_draft_strides, k_strides, v_strides, o_strides;
+  const int32_t* kv_lens; /* device [B]; NULL: every row of the cache is valid */
+  const void* mask;       /* or NULL */
+  int64_t mask_strides[2]; /* for (b, row) */
+  float scale;
+  int32_t device;
+  void* stream;
+  void* workspace;
+  size_t workspace_bytes;
+  const tt_attn_alloc_hook* alloc;
+  int32_t* status;
+} tt_attn_tree_params;
+
+/* The keys and values of accepted drafts go behind the valid rows of the caches: row path[b][i] of k_draft / v_draft to row
+ * kv_lens[b] + i, for i < counts[b].  new_lens[b] = kv_lens[b] + the rows written (it may be neither kv_lens nor counts).  A path ends at
+ * the first draft that does not exist (bit 16 of *status, as for a count outside [0, N]) and where the cache is full (bit 4).
+ * The same draft may be taken twice.  k_draft and v_draft may not overlap the caches. */
+typedef struct tt_attn_cache_accept_params {
+  uint32_t struct_size;
+  int32_t dtype;
+  int32_t B, Hkv, T, capacity, D, N;
+  const void* k_draft; /* [B, Hkv, T, D] */
+  const void* v_draft;
+  void* k; /* [B, Hkv, capacity, D] */
+  void* v;
+  tt_attn_strides k_draft_strides, v_draft_strides, k_strides, v_strides;
+  const int32_t* kv_lens; /* device [B] */
+  const int32_t* path;    /* device [B, N] */
+  const int32_t* counts;  /* device [B] */
+  int32_t* new_lens;      /* device [B] */
+  int32_t device;
+  void* stream;
+  int32_t* status;
+} tt_attn_cache_accept_params;
+
+TT_ATTN_API int tt_attn_tree(const tt_attn_tree_params* p);
+TT_ATTN_API int tt_attn_cache_accept(const tt_attn_cache_accept_params* p);
+TT_ATTN_API size_t tt_attn_tree_workspace_bytes(int dtype, int B, int Hq, int Hkv, int T, int capacity, int D);
+
 enum tt_attn_kind {
   TT_ATTN_KIND_FWD = 0,
   TT_ATTN_KIND_BWD = 1,

@@ -228,3 +228,96 @@ def test_the_forms_gradients_against_differences():
             d = r(*y.shape)
             f = lambda s: (ref.norm_rope(x + s * d if i == 0 else x, w + s * d if i == 1 else w, cs, 1e-3, interleaved) * go).sum()
             assert abs((f(1e-6) - f(-1e-6)) / 2e-6 - (want * d).sum()) <= 1e-7
+
+
+# ---------------------------------------------------------------------------------------------- tree and accept --
+def tree_args(**kw):
+    a = dict(q=t(3, 8, 5, 64), kDraft=t(3, 2, 5, 64), vDraft=t(3, 2, 5, 64), kCache=t(3, 2, 90, 64), vCache=t(3, 2, 90, 64), kvLens=ints(3),
+             treeMask=t(3, 5, 5, dtype=torch.bool))
+    a.update({n: f() if callable(f) else f for n, f in kw.items()})
+    return a
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q=lambda: t(3, 8, 5, 64, device="cpu")), dict(q=lambda: t(3, 8, 64)), dict(kDraft=lambda: t(3, 2, 4, 64)), dict(vDraft=lambda: t(3, 2, 6, 64)),
+    dict(kDraft=lambda: t(3, 4, 5, 64)), dict(kDraft=lambda: t(2, 2, 5, 64)), dict(vDraft=lambda: t(3, 2, 5, 64, dtype=torch.float16)),
+    dict(kCache=lambda: t(2, 2, 90, 64)), dict(vCache=lambda: t(3, 2, 89, 64)), dict(kCache=lambda: t(3, 2, 90, 128)), dict(kCache=lambda: t(3, 2, 64, 90).transpose(2, 3)),
+    dict(kvLens=lambda: ints(2)), dict(kvLens=lambda: ints(3, dtype=torch.int64)), dict(treeMask=lambda: t(3, 5, 5)), dict(treeMask=lambda: t(3, 4, 5, dtype=torch.bool)),
+    dict(treeMask=lambda: t(2, 5, 5, dtype=torch.bool)), dict(treeMask=lambda: t(3, 1, 5, 5, dtype=torch.bool)), dict(treeMask=lambda: t(5, 5, dtype=torch.bool, device="cpu")),
+    dict(workspace=lambda: t(99, device="cpu")), dict(status=lambda: ints(0)),
+])
+def test_tree_refuses(fake, kw):
+    with pytest.raises(ValueError):
+        op.sdpAttentionTree(**tree_args(**kw))
+
+
+def accept_args(**kw):
+    a = dict(kDraft=t(3, 2, 5, 64), vDraft=t(3, 2, 5, 64), kCache=t(3, 2, 90, 64), vCache=t(3, 2, 90, 64), kvLens=ints(3), path=ints(3, 4), counts=ints(3))
+    a.update({n: f() if callable(f) else f for n, f in kw.items()})
+    return a
+
+
+@pytest.mark.parametrize("kw", [
+    dict(kDraft=lambda: t(3, 4, 5, 64)), dict(vDraft=lambda: t(3, 2, 4, 64)), dict(kCache=lambda: t(2, 2, 90, 64)), dict(vCache=lambda: t(3, 2, 91, 64)),
+    dict(kvLens=lambda: ints(2)), dict(kvLens=lambda: ints(3, device="cpu")), dict(counts=lambda: ints(4)), dict(counts=lambda: ints(3, dtype=torch.int64)),
+    dict(path=lambda: ints(2, 4)), dict(path=lambda: ints(3)), dict(path=lambda: ints(3, 8)[:, ::2]), dict(path=lambda: ints(3, 4, device="cpu")),
+    dict(kCache=lambda: t(1, 2, 90, 64).expand(3, -1, -1, -1)), dict(vCache=lambda: t(3, 1, 90, 64).expand(-1, 2, -1, -1)),
+])
+def test_accept_refuses(fake, kw):
+    with pytest.raises(ValueError):
+        op.cacheAccept(**accept_args(**kw))
+
+
+def test_accept_refuses_drafts_that_lie_in_the_cache(fake):
+    c = t(3, 2, 90, 64)
+    with pytest.raises(ValueError, match="memory"):
+        op.cacheAccept(**accept_args(kCache=c, kDraft=c[:, :, 80:85]))
+
+
+def tree_params(cls, **kw):
+    p = cls()
+    p.struct_size = C.sizeof(p)
+    p.dtype, p.B, p.Hkv, p.T, p.capacity, p.D = 2, 3, 2, 5, 90, 64
+    p.k_draft = p.v_draft = p.k = p.v = 0x1000
+    if cls is _capi.TreeParams:
+        p.Hq, p.q, p.o = 8, 0x1000, 0x1000
+    else:
+        p.N, p.kv_lens, p.path, p.counts, p.new_lens = 4, 0x1000, 0x1000, 0x1000, 0x2000
+    for n, v in kw.items():
+        setattr(p, n, v)
+    return C.byref(p)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(struct_size=8), -8), (dict(dtype=3), -2), (dict(B=0), -3), (dict(T=0), -3), (dict(capacity=0), -3), (dict(D=96), -4), (dict(k_draft=None), -1),
+    (dict(v=0x1008), -5), (dict(k_strides=_capi.Strides(0, 64, 60)), -5), (dict(B=70000), -10),
+])
+def test_tree_and_accept_abi(kw, code):
+    lib = _capi.lib()
+    assert lib.tt_attn_tree(tree_params(_capi.TreeParams, **kw)) == code
+    assert lib.tt_attn_cache_accept(tree_params(_capi.CacheAcceptParams, **kw)) == code
+    assert lib.tt_attn_tree(None) == -1 and lib.tt_attn_cache_accept(None) == -1
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(T=129), -10), (dict(Hq=258), -10), (dict(dtype=0, Hq=66), -10), (dict(Hq=9), -3), (dict(q=None), -1), (dict(o=0x1004), -5),
+    (dict(mask=0x1000, mask_strides=(C.c_int64 * 2)(-1, 5)), -3), (dict(B=60000, capacity=2 ** 31 - 200), -10),
+])
+def test_tree_abi(kw, code):
+    assert _capi.lib().tt_attn_tree(tree_params(_capi.TreeParams, **kw)) == code
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(N=-1), -3), (dict(path=None), -1), (dict(counts=None), -1), (dict(new_lens=0x1000), -3), (dict(N=2 ** 30), -10),
+    (dict(k_strides=_capi.Strides(0, 128, 64)), -3), (dict(v_strides=_capi.Strides(11520, 0, 64)), -3),
+])
+def test_accept_abi(kw, code):
+    assert _capi.lib().tt_attn_cache_accept(tree_params(_capi.CacheAcceptParams, **kw)) == code
+
+
+def test_tree_workspace():
+    """Two partial results of 128 rows for each of up to 148 CTAs, and a line for each."""
+    w = _capi.lib().tt_attn_tree_workspace_bytes
+    assert w(2, 32, 32, 8, 32, 8192, 128) == 148 * 2 * 128 * 130 * 4 + 2560
+    assert 0 < w(2, 1, 1, 1, 1, 1, 64) <= 256 + 2 * 2 * 128 * 66 * 4
+    assert w(2, 1, 1, 1, 129, 1, 64) == 0 and w(0, 1, 64, 1, 1, 1, 64) == 0 and w(2, 0, 1, 1, 1, 1, 64) == 0

@@ -153,6 +153,33 @@ class PackedBwdParams(C.Structure):
     ]
 
 
+class TreeParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32),
+        ("B", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("T", C.c_int32), ("capacity", C.c_int32), ("D", C.c_int32),
+        ("q", C.c_void_p), ("k_draft", C.c_void_p), ("v_draft", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("q_strides", Strides), ("k_draft_strides", Strides), ("v_draft_strides", Strides), ("k_strides", Strides),
+        ("v_strides", Strides), ("o_strides", Strides),
+        ("kv_lens", C.c_void_p), ("mask", C.c_void_p), ("mask_strides", C.c_int64 * 2), ("scale", C.c_float),
+        ("device", C.c_int32), ("stream", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("alloc", C.POINTER(AllocHook)), ("status", C.c_void_p),
+    ]
+
+
+class CacheAcceptParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32),
+        ("B", C.c_int32), ("Hkv", C.c_int32), ("T", C.c_int32), ("capacity", C.c_int32), ("D", C.c_int32), ("N", C.c_int32),
+        ("k_draft", C.c_void_p), ("v_draft", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("k_draft_strides", Strides), ("v_draft_strides", Strides), ("k_strides", Strides), ("v_strides", Strides),
+        ("kv_lens", C.c_void_p), ("path", C.c_void_p), ("counts", C.c_void_p), ("new_lens", C.c_void_p),
+        ("device", C.c_int32), ("stream", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
+MAX_DRAFTS = 128  # TT_ATTN_MAX_DRAFTS
 MAX_ROPE_AXES = 4  # TT_ATTN_MAX_ROPE_AXES
 
 
@@ -184,7 +211,7 @@ FUSED_EXPORTS = ("tt_fused_add_rms_norm", "tt_silu_mul", "tt_linear", "tt_linear
 EXPORTS = ("tt_attn_fwd", "tt_attn_bwd", "tt_attn_decode", "tt_attn_decode_append", "tt_attn_decode_static",
            "tt_attn_selftest_wait_expiry", "tt_attn_bwd_selftest", "tt_attn_workspace_bytes", "tt_attn_strerror",
            "tt_attn_last_cuda_error", "tt_attn_version", "tt_attn_packed_fwd", "tt_attn_packed_bwd",
-           "tt_attn_packed_workspace_bytes")
+           "tt_attn_packed_workspace_bytes", "tt_attn_tree", "tt_attn_cache_accept", "tt_attn_tree_workspace_bytes")
 
 _lib = None
 _native = None
@@ -223,10 +250,13 @@ def lib():
         L.tt_attn_bwd_selftest.argtypes = [C.POINTER(BwdParams), C.c_int32, C.POINTER(C.c_int32)]
         L.tt_attn_bwd_selftest.restype = C.c_int
         for n, params in (("tt_attn_packed_fwd", PackedFwdParams), ("tt_attn_packed_bwd", PackedBwdParams),
+                          ("tt_attn_tree", TreeParams), ("tt_attn_cache_accept", CacheAcceptParams),
                           ("tt_qk_norm_rope", QkNormRopeParams), ("tt_qk_norm_rope_bwd", QkNormRopeBwdParams)):
             getattr(L, n).argtypes, getattr(L, n).restype = [C.POINTER(params)], C.c_int
         L.tt_attn_packed_workspace_bytes.argtypes = [C.c_int] * 7
         L.tt_attn_packed_workspace_bytes.restype = C.c_size_t
+        L.tt_attn_tree_workspace_bytes.argtypes = [C.c_int] * 7
+        L.tt_attn_tree_workspace_bytes.restype = C.c_size_t
         L.tt_qk_norm_rope_workspace_bytes.argtypes = [C.c_int] * 5
         L.tt_qk_norm_rope_workspace_bytes.restype = C.c_size_t
         for n in ("tt_attn_fwd", "tt_attn_bwd", "tt_attn_decode", "tt_attn_version"):

@@ -9,6 +9,7 @@
 #include "common.cuh"
 #include "norm_rope.cuh"
 #include "packed.cuh"
+#include "tree.cuh"
 #include "tma_host.cuh"
 
 namespace ttattn {
@@ -178,6 +179,11 @@ Str3 packed_strides(const tt_attn_strides& st, int64_t H, int64_t total, int64_t
   if (st.h == 0 && st.s == 0) return Str3{total * H * D, D, H * D};
   // (a batch of one: its stride is not used, but a tensor map wants one that is no smaller than the others)
   return Str3{st.s * total > st.h * H ? st.s * total : st.h * H, st.h, st.s};
+}
+
+int tree_limits(int dtype, int Hq, int Hkv, int T) {
+  const int rows = dtype == TT_ATTN_F32 ? 32 : 128;  // of a block, which holds whole groups
+  return T > TT_ATTN_MAX_DRAFTS || Hq / Hkv > rows ? TT_ATTN_ERR_TOO_LARGE : TT_ATTN_OK;
 }
 
 // Checks what the forward and the backward of tt_qk_norm_rope share and fills in the arguments.
@@ -618,6 +624,75 @@ int tt_attn_packed_bwd(const tt_attn_packed_bwd_params* p) {
   a.dq_accum = reinterpret_cast<float*>(at + 256 + plan + delta);
   const PackedCall c{p->cu_q, p->cu_k ? p->cu_k : p->cu_q, p->n_seqs, p->total_k, at + 256};
   cudaError_t e = launch_bwd_packed(p->dtype, p->D, a, c, p->device, static_cast<cudaStream_t>(p->stream));
+  return e == cudaSuccess ? TT_ATTN_OK : launch_failed(e);
+}
+
+size_t tt_attn_tree_workspace_bytes(int dtype, int B, int Hq, int Hkv, int T, int capacity, int D) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || T <= 0 || capacity <= 0 || D <= 0 || tree_limits(dtype, Hq, Hkv, T) != TT_ATTN_OK) return 0;
+  return tree_scratch_bytes(dtype, B, Hq, Hkv, T, capacity, D);
+}
+
+int tt_attn_tree(const tt_attn_tree_params* p) {
+  if (!p) return TT_ATTN_ERR_NULL;
+  if (p->struct_size != sizeof(tt_attn_tree_params)) return TT_ATTN_ERR_STRUCT;
+  if (int rc = check_common(p->dtype, p->B, p->Hq, p->Hkv, p->T, p->capacity, p->D)) return rc;
+  if (int rc = tree_limits(p->dtype, p->Hq, p->Hkv, p->T)) return rc;
+  if (tree_line(p->dtype, p->B, p->Hq, p->Hkv, p->T, p->capacity) > 1e9) return TT_ATTN_ERR_TOO_LARGE;  // (tiles are counted in 32 bits)
+  if (!p->q || !p->k_draft || !p->v_draft || !p->k || !p->v || !p->o) return TT_ATTN_ERR_NULL;
+  const size_t es = elem_size(p->dtype);
+  TreeArgs a{};
+  a.q = p->q, a.kd = p->k_draft, a.vd = p->v_draft, a.kc = p->k, a.vc = p->v, a.o = p->o, a.lse = p->lse;
+  a.qs = dense_or(p->q_strides, p->Hq, p->T, p->D);
+  a.kds = dense_or(p->k_draft_strides, p->Hkv, p->T, p->D);
+  a.vds = dense_or(p->v_draft_strides, p->Hkv, p->T, p->D);
+  a.kcs = dense_or(p->k_strides, p->Hkv, p->capacity, p->D);
+  a.vcs = dense_or(p->v_strides, p->Hkv, p->capacity, p->D);
+  a.os = dense_or(p->o_strides, p->Hq, p->T, p->D);
+  const void* ptrs[] = {p->q, p->k_draft, p->v_draft, p->k, p->v, p->o};
+  for (const void* q : ptrs)
+    if (!aligned16(q)) return TT_ATTN_ERR_ALIGN;
+  const Str3* sts[] = {&a.qs, &a.kds, &a.vds, &a.kcs, &a.vcs, &a.os};
+  for (const Str3* s : sts)
+    if (!strides_ok(*s, es)) return TT_ATTN_ERR_ALIGN;
+  if (p->mask && (p->mask_strides[0] < 0 || p->mask_strides[1] < 0)) return TT_ATTN_ERR_SHAPE;
+  a.B = p->B, a.Hq = p->Hq, a.Hkv = p->Hkv, a.T = p->T, a.capacity = p->capacity;
+  a.scale = p->scale, a.kv_lens = p->kv_lens, a.status = p->status;
+  a.mask = static_cast<const uint8_t*>(p->mask), a.mask_b = p->mask_strides[0], a.mask_t = p->mask_strides[1];
+  DeviceGuard guard(p->device);
+  if (!guard.ok) return TT_ATTN_ERR_NO_DEVICE;
+  Workspace ws;
+  if (int rc = ws.acquire(tree_scratch_bytes(p->dtype, p->B, p->Hq, p->Hkv, p->T, p->capacity, p->D), p->workspace, p->workspace_bytes, p->alloc,
+                          p->device))
+    return rc;
+  cudaError_t e = launch_tree(p->dtype, p->D, a, ws.ptr, p->device, static_cast<cudaStream_t>(p->stream));
+  return e == cudaSuccess ? TT_ATTN_OK : launch_failed(e);
+}
+
+int tt_attn_cache_accept(const tt_attn_cache_accept_params* p) {
+  if (!p) return TT_ATTN_ERR_NULL;
+  if (p->struct_size != sizeof(tt_attn_cache_accept_params)) return TT_ATTN_ERR_STRUCT;
+  if (int rc = check_common(p->dtype, p->B, p->Hkv, p->Hkv, p->T, p->capacity, p->D)) return rc;
+  if (p->N < 0) return TT_ATTN_ERR_SHAPE;
+  if (2.0 * p->Hkv * p->N * p->D > 1e9) return TT_ATTN_ERR_TOO_LARGE;  // (vectors of a sequence are counted in 32 bits)
+  if (!p->k_draft || !p->v_draft || !p->k || !p->v || !p->kv_lens || !p->counts || !p->new_lens || (p->N > 0 && !p->path)) return TT_ATTN_ERR_NULL;
+  if (p->new_lens == p->kv_lens || p->new_lens == p->counts) return TT_ATTN_ERR_SHAPE;
+  const size_t es = elem_size(p->dtype);
+  AcceptArgs a{};
+  a.kd = p->k_draft, a.vd = p->v_draft, a.kc = p->k, a.vc = p->v;
+  a.kds = dense_or(p->k_draft_strides, p->Hkv, p->T, p->D);
+  a.vds = dense_or(p->v_draft_strides, p->Hkv, p->T, p->D);
+  a.kcs = dense_or(p->k_strides, p->Hkv, p->capacity, p->D);
+  a.vcs = dense_or(p->v_strides, p->Hkv, p->capacity, p->D);
+  if (!aligned16(a.kd) || !aligned16(a.vd) || !aligned16(a.kc) || !aligned16(a.vc) || !strides_ok(a.kds, es) || !strides_ok(a.vds, es) ||
+      !strides_ok(a.kcs, es) || !strides_ok(a.vcs, es))
+    return TT_ATTN_ERR_ALIGN;
+  for (const Str3* s : {&a.kcs, &a.vcs})  // (sequences or heads that share rows would be written twice)
+    if ((p->B > 1 && s->b == 0) || (p->Hkv > 1 && s->h == 0)) return TT_ATTN_ERR_SHAPE;
+  a.B = p->B, a.Hkv = p->Hkv, a.T = p->T, a.capacity = p->capacity, a.N = p->N;
+  a.kv_lens = p->kv_lens, a.path = p->path, a.counts = p->counts, a.new_lens = p->new_lens, a.status = p->status;
+  DeviceGuard guard(p->device);
+  if (!guard.ok) return TT_ATTN_ERR_NO_DEVICE;
+  cudaError_t e = launch_cache_accept(p->dtype, p->D, a, static_cast<cudaStream_t>(p->stream));
   return e == cudaSuccess ? TT_ATTN_OK : launch_failed(e);
 }
 

@@ -50,6 +50,8 @@ struct Api {
   int (*linear)(const tt_linear_params*);
   int (*packed_fwd)(const tt_attn_packed_fwd_params*);
   int (*packed_bwd)(const tt_attn_packed_bwd_params*);
+  int (*tree)(const tt_attn_tree_params*);
+  int (*cache_accept)(const tt_attn_cache_accept_params*);
   int (*qk_norm_rope)(const tt_qk_norm_rope_params*);
   int (*qk_norm_rope_bwd)(const tt_qk_norm_rope_bwd_params*);
   const char* (*strerror)(int);
@@ -1148,6 +1150,112 @@ PyObject* py_packed_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// k and v of drafts [B, Hkv, T, D] beside caches [B, Hkv, capacity, D]
+void check_drafts(const Tensor& kd, const Tensor& vd, const Tensor& kc, const Tensor& vc, const Tensor& like, int64_t T) {
+  check_attn_tensor(kd, "kDraft");
+  check_attn_tensor(vd, "vDraft");
+  check_attn_tensor(kc, "kCache");
+  check_attn_tensor(vc, "vCache");
+  const at::DimVector drafts = {like.size(0), kc.size(1), T, like.size(3)};
+  for (const Tensor* t : {&kd, &vd, &kc, &vc})
+    if (t->scalar_type() != like.scalar_type() || t->device() != like.device()) raise(PyExc_ValueError, "drafts and caches must share dtype and device");
+  if (kd.sizes() != at::IntArrayRef(drafts) || vd.sizes() != kd.sizes())
+    raise(PyExc_ValueError, "kDraft and vDraft must be [B, Hkv, drafts, D], with the heads of the caches");
+  if (kc.size(0) != like.size(0) || kc.size(3) != like.size(3) || vc.sizes() != kc.sizes())
+    raise(PyExc_ValueError, "kCache and vCache must be [B, Hkv, capacity, D]");
+}
+
+// tree(q, kDraft, vDraft, kCache, vCache, kvLens, treeMask, scale, needLse, workspace, status) -> (O, LSE or None)
+PyObject* py_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 11);
+  const Tensor &q = tensor_of(a[0], "q"), &kd = tensor_of(a[1], "kDraft"), &vd = tensor_of(a[2], "vDraft"), &kc = tensor_of(a[3], "kCache"),
+               &vc = tensor_of(a[4], "vCache");
+  check_attn_tensor(q, "q");
+  check_drafts(kd, vd, kc, vc, q, q.size(2));
+  const Tensor kv_lens = optional_of(a[5], "kvLens"), ws = optional_of(a[9], "workspace"), status = optional_of(a[10], "status");
+  Tensor mask = optional_of(a[6], "treeMask");
+  check_ints(kv_lens, status, q);
+  const int64_t B = q.size(0), Hq = q.size(1), T = q.size(2), D = q.size(3);
+  if (mask.defined()) {
+    const int64_t m = mask.dim();
+    if (mask.scalar_type() != at::kBool || mask.device() != q.device() || (m != 2 && m != 3) || mask.size(-1) != T || mask.size(-2) != T ||
+        (m == 3 && mask.size(0) != B && mask.size(0) != 1))
+      raise(PyExc_ValueError, "treeMask must be bool [drafts, drafts] or [B, drafts, drafts] on the device of q");
+    if (T > 1 && mask.stride(-1) != 1) mask = mask.contiguous();
+  }
+  if (ws.defined() && (ws.device() != q.device() || !ws.is_contiguous()))
+    raise(PyExc_ValueError, "workspace must be a contiguous tensor on the device of q");
+  const float scale = scale_or_default(scale_arg(a[7]), D);
+  const bool need_lse = bool_arg(a[8]);
+  Tensor o, lse;
+  {
+    NoGil nogil;
+    tt_attn_tree_params p{};
+    set_common(&p, q);
+    o = empty(q.sizes(), q.scalar_type(), q.device());
+    if (need_lse) lse = empty({B, Hq, T}, at::kFloat, q.device());
+    p.dtype = dtype_of(q.scalar_type());
+    p.B = B, p.Hq = Hq, p.Hkv = kc.size(1), p.T = T, p.capacity = kc.size(2), p.D = D;
+    p.q = q.data_ptr(), p.k_draft = kd.data_ptr(), p.v_draft = vd.data_ptr(), p.k = kc.data_ptr(), p.v = vc.data_ptr(), p.o = o.data_ptr();
+    p.lse = need_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
+    p.q_strides = head_strides_of(q), p.k_draft_strides = head_strides_of(kd), p.v_draft_strides = head_strides_of(vd);
+    p.k_strides = head_strides_of(kc), p.v_strides = head_strides_of(vc), p.o_strides = head_strides_of(o);
+    p.kv_lens = ints_ptr(kv_lens), p.scale = scale;
+    if (mask.defined()) {
+      p.mask = mask.data_ptr();
+      p.mask_strides[0] = mask.dim() == 3 && mask.size(0) > 1 ? mask.stride(0) : 0, p.mask_strides[1] = T > 1 ? mask.stride(-2) : 0;
+    }
+    p.alloc = &hook, p.status = ints_ptr(status);
+    if (ws.defined()) p.workspace = ws.data_ptr(), p.workspace_bytes = ws.numel() * ws.element_size();
+    check(api.tree(&p));
+  }
+  return tuple_of({&o, &lse});
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_accept(kDraft, vDraft, kCache, vCache, kvLens, path, counts, status) -> newLens
+PyObject* py_cache_accept(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 8);
+  const Tensor &kd = tensor_of(a[0], "kDraft"), &vd = tensor_of(a[1], "vDraft"), &kc = tensor_of(a[2], "kCache"), &vc = tensor_of(a[3], "vCache"),
+               &lens = tensor_of(a[4], "kvLens"), &path = tensor_of(a[5], "path"), &counts = tensor_of(a[6], "counts");
+  check_attn_tensor(kd, "kDraft");
+  check_drafts(kd, vd, kc, vc, kd, kd.size(2));
+  const Tensor status = optional_of(a[7], "status");
+  const int64_t B = kd.size(0);
+  if (!lens.is_cuda() || !counts.is_cuda() || lens.numel() != B || counts.numel() != B)
+    raise(PyExc_ValueError, "kvLens and counts must be int32 [B] on the device of the caches");
+  check_ints(lens, "kvLens", B, kd);
+  check_ints(counts, "counts", B, kd);
+  if (path.dim() != 2 || path.size(0) != B || !path.is_cuda()) raise(PyExc_ValueError, "path must be int32 [B, N] on the device of the caches");
+  check_ints(path, "path", path.numel(), kd);
+  check_ints(status, "status", 1, kd);
+  for (const Tensor* from : {&kd, &vd})
+    for (const Tensor* to : {&kc, &vc})
+      if (from->storage().is_alias_of(to->storage())) raise(PyExc_ValueError, "drafts must not lie in a cache's memory");
+  for (const Tensor* c : {&kc, &vc})
+    for (int d = 0; d < 3; ++d)
+      if (c->size(d) > 1 && c->stride(d) == 0) raise(PyExc_ValueError, "sequences, heads and rows of a cache that is written must have their own memory");
+  Tensor new_lens;
+  {
+    NoGil nogil;
+    new_lens = empty(lens.sizes(), at::kInt, lens.device());
+    tt_attn_cache_accept_params p{};
+    set_common(&p, kd);
+    p.dtype = dtype_of(kd.scalar_type());
+    p.B = B, p.Hkv = kc.size(1), p.T = kd.size(2), p.capacity = kc.size(2), p.D = kd.size(3), p.N = path.size(1);
+    p.k_draft = kd.data_ptr(), p.v_draft = vd.data_ptr(), p.k = kc.data_ptr(), p.v = vc.data_ptr();
+    p.k_draft_strides = head_strides_of(kd), p.v_draft_strides = head_strides_of(vd);
+    p.k_strides = head_strides_of(kc), p.v_strides = head_strides_of(vc);
+    p.kv_lens = ints_ptr(lens), p.path = ints_ptr(path), p.counts = ints_ptr(counts), p.new_lens = ints_ptr(new_lens);
+    p.status = ints_ptr(status);
+    check(api.cache_accept(&p));
+  }
+  return wrap(new_lens);
+  END_HANDLE_TH_ERRORS
+}
+
 // cos, sin, positions, eps, interleaved, sections (None or a sequence of integers)
 Rope rope_args(PyObject* const* a) {
   Rope r;
@@ -1247,6 +1355,8 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   sym(api.linear, "tt_linear");
   sym(api.packed_fwd, "tt_attn_packed_fwd");
   sym(api.packed_bwd, "tt_attn_packed_bwd");
+  sym(api.tree, "tt_attn_tree");
+  sym(api.cache_accept, "tt_attn_cache_accept");
   sym(api.qk_norm_rope, "tt_qk_norm_rope");
   sym(api.qk_norm_rope_bwd, "tt_qk_norm_rope_bwd");
   sym(api.strerror, "tt_attn_strerror");
@@ -1277,6 +1387,8 @@ PyMethodDef methods[] = {
     {"sdp_attention_packed", fast(py_sdp_attention_packed), METH_FASTCALL, nullptr},
     {"packed_fwd", fast(py_packed_fwd), METH_FASTCALL, nullptr},
     {"packed_bwd", fast(py_packed_bwd), METH_FASTCALL, nullptr},
+    {"tree", fast(py_tree), METH_FASTCALL, nullptr},
+    {"cache_accept", fast(py_cache_accept), METH_FASTCALL, nullptr},
     {"qk_norm_rope", fast(py_qk_norm_rope), METH_FASTCALL, nullptr},
     {"qk_norm_rope_raw", fast(py_qk_norm_rope_raw), METH_FASTCALL, nullptr},
     {"qk_norm_rope_bwd", fast(py_qk_norm_rope_bwd), METH_FASTCALL, nullptr},

@@ -1,0 +1,437 @@
+// Drafted tokens over a KV cache for fp16 / bf16 on sm_100a tensor cores (see tree.cuh for how the work is divided).
+//
+// Bound by memory: every cache row is read once for the up to 128 rows of a block (2 D keys and values of 16 bits for 4 D
+// operations a row), so the loop has to keep the loads going and to do a tile's two products and 128 x 128 exponentials in the time
+// that its 64 KB (D = 128) take to arrive, 2800 cycles of an SM's share of the bandwidth.  The key tiles of a walk go to the
+// two halves of the CTA in turn:
+//   warp 8     producer: publishes the segments, loads Q (one 5-D box: heads of the group inside drafts) and streams K and V tiles
+//              of 128 keys through rings of three stages (six for D = 64), the cache's and then the drafts'; it runs ahead across segments
+//   warp 9     issuer: S_t = Q K^T and O_t += P_t V with tcgen05.mma, P_t from TMEM
+//   warps 0-3 / 4-7: softmax of half t.  Thread r owns row r (TMEM lane): scores, running maximum and sum, P written over S;
+//              warps without rows skip all of it but the barriers.  V rows behind a sequence's length may hold anything and are
+//              zeroed in shared memory before the product.  The halves' accumulators, in the same lanes, are put together at the end of a
+//              segment by both warpgroups, each for half of the channels.
+// Every mbarrier wait is bounded.
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "ptx.cuh"
+#include "tma_host.cuh"
+#include "tree.cuh"
+
+namespace ttattn {
+namespace {
+
+constexpr int BM = 128, BN = 128, kThreads = 384, kTmemCols = 512;
+constexpr int kHalfBytes = BM * 128;  // a block of 64 channels of a tile
+constexpr int kSoft = 2 * BM;
+constexpr int kProducer = 8, kIssuer = 9;
+
+template <int D>
+struct Cfg {
+  static constexpr int kTile = BM * D * 2, kStages = D == 128 ? 3 : 6;
+  static constexpr int kSmem = kTile + 2 * kStages * kTile + 512 /* control block */ + 2 * BM * 8 /* statistics */;
+  static_assert(kSmem <= 232448, "exceeds the shared memory a CTA may request");
+};
+
+struct __align__(16) Ctl {
+  uint64_t q_full, q_empty;
+  uint64_t k_full[6], k_empty[6], v_full[6], v_empty[6];
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t seg_full[2], seg_empty[2];
+  TreeSegment seg[2];
+  int scratch[kThreads / 32 + 2];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(Ctl) <= 512, "control block");
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                   const __grid_constant__ CUtensorMap tmKd, const __grid_constant__ CUtensorMap tmVd, const TreeArgs a) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  constexpr int kTile = Cfg<D>::kTile, kStages = Cfg<D>::kStages, kHalves = D / 64;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((ptx::smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0 && a.status) atomicOr(a.status, kStatusBadSmemAlign);
+    return;
+  }
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + kTile;
+  uint8_t* sV = sK + kStages * kTile;
+  Ctl* ctl = reinterpret_cast<Ctl*>(sV + kStages * kTile);
+  volatile int* abort_flag = &ctl->abort_flag;
+  float2* s_stat = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(ctl) + 512);  // [half][row]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = a.Hq / a.Hkv;
+
+  if (warp == kProducer && lane == 0) {
+    ptx::mbar_init(&ctl->q_full, 1);
+    ptx::mbar_init(&ctl->q_empty, 1);
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) {
+      ptx::mbar_init(&ctl->k_full[i], 1);
+      ptx::mbar_init(&ctl->k_empty[i], 1);
+      ptx::mbar_init(&ctl->v_full[i], 1);
+      ptx::mbar_init(&ctl->v_empty[i], 1);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&ctl->s_full[i], 1);
+      ptx::mbar_init(&ctl->p_full[i], BM);
+      ptx::mbar_init(&ctl->o_full[i], 1);
+      ptx::mbar_init(&ctl->seg_full[i], 1);
+      ptx::mbar_init(&ctl->seg_empty[i], 1 + kSoft);
+    }
+    ctl->abort_flag = 0;
+    ptx::fence_barrier_init();
+    ptx::tma_prefetch_desc(&tmQ);
+    ptx::tma_prefetch_desc(&tmK);
+    ptx::tma_prefetch_desc(&tmV);
+    ptx::tma_prefetch_desc(&tmKd);
+    ptx::tma_prefetch_desc(&tmVd);
+  }
+  if (warp == kIssuer) {
+    ptx::tmem_alloc(&ctl->tmem_base, kTmemCols);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = ctl->tmem_base;
+  ptx::grid_dep_launch();
+  ptx::grid_dep_wait();
+  TreeWalk walk;
+  walk.start<BN, kThreads>(a, ctl->scratch);
+
+  if (warp >= 8) {
+    ptx::setmaxnreg_dec<72>();  // (216 + 216 + 72 registers: the 168 x 384 that the CTA was launched with)
+    if (warp == kProducer && lane == 0) {
+      // -------------------------------------------------------------- producer --
+      uint32_t g = 0;  // tiles requested so far
+      a.pieces[blockIdx.x] = make_int4(0, 0, 0, 0);
+      bool ok = true;
+      for (uint32_t i = 0; ok; ++i) {
+        TreeSegment s;
+        const int begin = walk.at;
+        const bool some = walk.next<BN>(a, &s);
+        if (!some) s.n = -1;
+        const int slot = i & 1;
+        if (!ptx::mbar_wait(&ctl->seg_empty[slot], ((i >> 1) & 1) ^ 1, abort_flag)) break;
+        ctl->seg[slot] = s;
+        ptx::mbar_arrive(&ctl->seg_full[slot]);
+        if (!some) break;
+        if (s.piece == 1) a.pieces[blockIdx.x] = make_int4(walk.pieces(begin, s.n_all), s.b, s.hk, s.block);
+        if (!ptx::mbar_wait(&ctl->q_empty, (i & 1) ^ 1, abort_flag)) break;
+        ptx::mbar_arrive_expect_tx(&ctl->q_full, kHalves * group * a.block * 128);
+#pragma unroll
+        for (int hf = 0; hf < kHalves; ++hf)
+          ptx::tma_load_5d(sQ + hf * kHalfBytes, &tmQ, &ctl->q_full, hf * 64, 0, s.block * a.block, s.hk, s.b);
+        auto load = [&](uint8_t* dst, const CUtensorMap* cache, const CUtensorMap* drafts, uint64_t* full, uint64_t* empty, int j) {
+          const uint32_t gj = g + j;
+          const int st = gj % kStages, tile = s.j0 + j;
+          if (!ptx::mbar_wait(&empty[st], ((gj / kStages) & 1) ^ 1, abort_flag)) return false;
+          ptx::mbar_arrive_expect_tx(&full[st], kTile);
+          const CUtensorMap* map = tile < s.n_ctx ? cache : drafts;
+          const int row = (tile < s.n_ctx ? tile : tile - s.n_ctx) * BN;
+#pragma unroll
+          for (int hf = 0; hf < kHalves; ++hf) ptx::tma_load_4d(dst + st * kTile + hf * kHalfBytes, map, &full[st], hf * 64, row, s.hk, s.b);
+          return true;
+        };
+        // K a tile ahead of V, as the products consume them
+        ok = load(sK, &tmK, &tmKd, ctl->k_full, ctl->k_empty, 0);
+        for (int j = 0; j < s.n && ok; ++j) {
+          if (j + 1 < s.n) ok = load(sK, &tmK, &tmKd, ctl->k_full, ctl->k_empty, j + 1);
+          if (ok) ok = load(sV, &tmV, &tmVd, ctl->v_full, ctl->v_empty, j);
+        }
+        g += s.n;
+      }
+    } else if (warp == kIssuer) {
+      // ---------------------------------------------------------------- issuer --
+      // The whole warp runs the loop; one elected lane issues.  Half t takes the tiles t, t + 2, ... of a segment, in the order
+      // PV(0) QK(0)' PV(1) QK(1)': MMAs execute in issue order, so QK(t)' cannot pass the PV(t) that still reads P_t.
+      const bool leader = ptx::elect_one();
+      auto uwait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag)) != 0; };
+      // (a negative scale is folded into the sign of Q: the softmax multiplies by a non-negative one)
+      const uint32_t idesc_qk = ptx::make_idesc_f16(BM, BN, BF16 ? 1 : 0, 0, 0) | (a.scale < 0.f ? (1u << 13) : 0u);
+      const uint32_t idesc_pv = ptx::make_idesc_f16(BM, D, BF16 ? 1 : 0, 0, 1);
+      constexpr uint32_t kHi = ptx::smem_desc_hi_sw128(1024);
+      const uint32_t qlo = ptx::smem_desc_lo(ptx::smem_u32(sQ), 16), klo = ptx::smem_desc_lo(ptx::smem_u32(sK), 16);
+      const uint32_t vlo = ptx::smem_desc_lo(ptx::smem_u32(sV), kHalfBytes);
+      uint32_t g0 = 0, done[2] = {0, 0};  // ring position of the segment; softmax iterations of each half (p_full phases)
+      bool ok = true;
+      for (uint32_t i = 0; ok; ++i) {
+        const int slot = i & 1;
+        if (!uwait(&ctl->seg_full[slot], (i >> 1) & 1)) break;
+        const int n = ctl->seg[slot].n;
+        __syncwarp();
+        if (leader) ptx::mbar_arrive(&ctl->seg_empty[slot]);
+        if (n < 0) break;
+        auto qk = [&](int t, int j) {
+          const uint32_t b0 = klo + ((g0 + j) % kStages) * (kTile >> 4), d = tmem + t * BN;
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
+            if (leader) ptx::mma_ss2(d, qlo + off, kHi, b0 + off, kHi, idesc_qk, ks > 0 ? 1u : 0u);
+          }
+          if (leader) ptx::mma_commit(&ctl->s_full[t]);
+          if (leader) ptx::mma_commit(&ctl->k_empty[(g0 + j) % kStages]);
+          if (leader && j == n - 1) ptx::mma_commit(&ctl->q_empty);
+        };
+        auto wait_k = [&](int j) { return uwait(&ctl->k_full[(g0 + j) % kStages], ((g0 + j) / kStages) & 1); };
+        if (!(ok = uwait(&ctl->q_full, i & 1))) break;
+        for (int t = 0; t < 2 && t < n; ++t) {
+          if (!(ok = wait_k(t))) break;
+          ptx::tc_fence_after();
+          qk(t, t);
+        }
+        for (int j = 0; j < n && ok; ++j) {
+          const int t = j & 1;
+          const uint32_t g = g0 + j;
+          bool all = ptx::mbar_wait(&ctl->v_full[g % kStages], (g / kStages) & 1, abort_flag);
+          if (j + 2 < n && all) all = ptx::mbar_wait(&ctl->k_full[(g + 2) % kStages], ((g + 2) / kStages) & 1, abort_flag);
+          if (all) all = ptx::mbar_wait(&ctl->p_full[t], ((t == 0 ? done[0] : done[1]) + (j >> 1)) & 1, abort_flag);
+          if (!(ok = __all_sync(0xffffffffu, all) != 0)) break;
+          ptx::tc_fence_after();
+          const uint32_t b0 = vlo + (g % kStages) * (kTile >> 4), d = tmem + 256 + t * D, a0 = tmem + t * BN;
+#pragma unroll
+          for (int ks = 0; ks < BN / 16; ++ks)
+            if (leader) ptx::mma_ts2(d, a0 + ks * 8, b0 + ks * (2048 >> 4), kHi, idesc_pv, (j >= 2 || ks > 0) ? 1u : 0u);
+          if (leader && j + 2 >= n) ptx::mma_commit(&ctl->o_full[t]);
+          if (leader) ptx::mma_commit(&ctl->v_empty[g % kStages]);
+          if (j + 2 < n) qk(t, j + 2);
+        }
+        g0 += n, done[0] += (n + 1) / 2, done[1] += n / 2;
+      }
+    }
+  } else {
+    ptx::setmaxnreg_inc<216>();
+    // ------------------------------------------------------------- softmax --
+    const int t = warp >> 2, r = tid & (BM - 1);
+    const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + t * BN + lane_addr, tO = tmem + 256 + t * D + lane_addr;
+    const float c = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);  // > 0, so that a hidden score stays -inf
+    const float2 c2 = make_float2(c, c);
+    uint32_t cnt = 0, tiles = 0, ends[2] = {0, 0};  // phases of s_full, ring position, phases of o_full
+    uint32_t s[BN];
+    bool ok = true;
+    // Threads meet at named barriers within a segment: an expired wait is voted on, and all leave together.
+    for (uint32_t i = 0;; ++i) {
+      const int slot = i & 1;
+      ok = ptx::mbar_wait(&ctl->seg_full[slot], (i >> 1) & 1, abort_flag);
+      if (ptx::named_barrier_or(3, kSoft, !ok)) break;
+      const TreeSegment g = ctl->seg[slot];
+      ptx::mbar_arrive(&ctl->seg_empty[slot]);
+      if (g.n < 0) break;
+      const int draft0 = g.block * a.block, drafts = a.T - draft0 < a.block ? a.T - draft0 : a.block, rows = drafts * group;
+      const bool mine = r < rows, warp_has = (warp & 3) * 32 < rows;
+      const int draft = draft0 + r / group, head = g.hk * group + r % group;
+      uint32_t sees[4] = {0, 0, 0, 0};
+      if (mine && g.j0 + g.n == g.n_all) tree_mask_row<4>(a, g.b, draft, sees);
+
+      float m_ref = mine ? -INFINITY : 0.f;  // reference maximum, in log2 units
+      float2 l2 = make_float2(0.f, 0.f);
+      const int n_t = (g.n + 1 - t) / 2;
+      for (int jj = 0; jj < n_t && ok; ++jj) {
+        const int j = 2 * jj + t, tile = g.j0 + j;
+        ok = ptx::mbar_wait(&ctl->s_full[t], (cnt + jj) & 1, abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const int left = tile < g.n_ctx ? g.len - tile * BN : BN;  // valid keys of a tile of the cache
+        if (left < BN) {
+          // what lies behind the length may be infinite: exact zeros, so that 0 times it is 0
+          const uint32_t gj = tiles + j;
+          ok = ptx::mbar_wait(&ctl->v_full[gj % kStages], (gj / kStages) & 1, abort_flag);
+          if (ok && r >= left) {
+            uint8_t* v = sV + (gj % kStages) * kTile + r * 128;
+#pragma unroll
+            for (int hf = 0; hf < kHalves; ++hf)
+#pragma unroll
+              for (int ch = 0; ch < 8; ++ch) *reinterpret_cast<uint4*>(v + hf * kHalfBytes + ch * 16) = make_uint4(0, 0, 0, 0);
+          }
+          ptx::fence_proxy_async_smem();
+        }
+        if (warp_has) {
+#pragma unroll
+          for (int cc = 0; cc < 4; ++cc) ptx::tmem_ld32p(tS + cc * 32, s + cc * 32);
+          ptx::tmem_wait_ld();
+          if (tile >= g.n_ctx) {
+#pragma unroll
+            for (int e = 0; e < BN; ++e)
+              if (!((sees[e / 32] >> (e % 32)) & 1)) s[e] = 0xff800000u;
+          } else if (left < BN || !mine) {
+            const int lim = mine ? left : 0;
+#pragma unroll
+            for (int e = 0; e < BN; ++e)
+              if (e >= lim) s[e] = 0xff800000u;
+          }
+          // The maximum is only a reference for the exponentials: it is kept while a tile's sum shows that none is large.
+          bool need_max = jj == 0;
+          for (;;) {
+            if (need_max) {
+              float mx[8];
+#pragma unroll
+              for (int q = 0; q < 8; ++q) mx[q] = ptx::max3(__uint_as_float(s[q]), __uint_as_float(s[q + 8]), -INFINITY);
+#pragma unroll
+              for (int e = 16; e < BN; e += 16)
+#pragma unroll
+                for (int q = 0; q < 8; ++q) mx[q] = ptx::max3(mx[q], __uint_as_float(s[e + q]), __uint_as_float(s[e + q + 8]));
+              const float x_max = ptx::max3(ptx::max3(mx[0], mx[1], mx[2]), ptx::max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * c;
+              if (jj == 0) {
+                if (mine) m_ref = x_max;
+              } else if (__any_sync(0xffffffffu, x_max > m_ref)) {
+                const float m_new = fmaxf(m_ref, x_max);
+                const float alpha = m_new == -INFINITY ? 1.f : ptx::ex2(m_ref - m_new);
+                uint32_t x[32];
+#pragma unroll
+                for (int cc = 0; cc < D / 32; ++cc) {
+                  ptx::tmem_ld32(tO + cc * 32, x);
+                  ptx::tmem_wait_ld();
+#pragma unroll
+                  for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
+                  ptx::tmem_st32(tO + cc * 32, x);
+                }
+                l2.x *= alpha, l2.y *= alpha;
+                m_ref = m_new;
+              }
+            }
+            const float m_use = m_ref == -INFINITY ? 0.f : m_ref;  // (nothing seen so far: exponentials of -inf)
+            const float2 nm2 = make_float2(-m_use, -m_use);
+            float2 lt = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              uint32_t pk[32];
+#pragma unroll
+              for (int e2 = 0; e2 < 64; e2 += 2) {
+                const int e = hf * 64 + e2;
+                const float2 x = ptx::fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, nm2);
+                const float2 p = make_float2(ptx::ex2(x.x), ptx::ex2(x.y));
+                lt = ptx::add2(lt, p);
+                pk[e2 >> 1] = pack2<BF16>(p.x, p.y);
+              }
+              ptx::tmem_st32(tS + hf * 32, pk);
+            }
+            const float sum = lt.x + lt.y;
+            const bool redo = !need_max && (!(sum <= 256.f) || m_ref == -INFINITY);
+            if (!__any_sync(0xffffffffu, redo)) {
+              l2 = ptx::add2(l2, lt);
+              break;
+            }
+            need_max = true;
+          }
+          ptx::tmem_wait_st();
+        }
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(&ctl->p_full[t]);
+      }
+      cnt += n_t, tiles += g.n;
+
+      // both halves
+      const bool two = g.n > 1;
+      if (ok) ok = ptx::mbar_wait(&ctl->o_full[0], ends[0] & 1, abort_flag);
+      if (ok && two) ok = ptx::mbar_wait(&ctl->o_full[1], ends[1] & 1, abort_flag);
+      ++ends[0], ends[1] += two;
+      s_stat[t * BM + r] = make_float2(n_t > 0 ? m_ref : -INFINITY, l2.x + l2.y);
+      if (ptx::named_barrier_or(3, kSoft, !ok)) break;
+      ptx::tc_fence_after();
+      if (warp_has && (D == 128 || t == 0)) {
+        const float2 sa = s_stat[r], sb = s_stat[BM + r];
+        const float m = fmaxf(sa.x, sb.x);
+        const float wa = sa.x == -INFINITY ? 0.f : ptx::ex2(sa.x - m), wb = sb.x == -INFINITY ? 0.f : ptx::ex2(sb.x - m);
+        const float l = sa.y * wa + sb.y * wb;
+        const int c0 = D == 128 ? t * 64 : 0;
+        const float inv = g.piece >= 0 ? 1.f : (l > 0.f ? 1.f / l : 0.f);
+        const float ua = wa * inv, ub = wb * inv;
+        float* part = a.partial + (static_cast<size_t>(blockIdx.x) * 2 + (g.piece > 0 ? 1 : 0)) * tree_partial_floats(D);
+        T* orow = reinterpret_cast<T*>(a.o) + g.b * a.os.b + head * a.os.h + draft * a.os.s;
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          ptx::tmem_ld32p(tmem + 256 + lane_addr + c0 + cc * 32, s);
+          if (two) ptx::tmem_ld32p(tmem + 256 + D + lane_addr + c0 + cc * 32, s + 32);
+          ptx::tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            // (a half that has seen no key for the row holds zeros, or nothing at all: it takes no part)
+            float x = ua > 0.f ? __uint_as_float(s[e]) * ua : 0.f;
+            if (two && ub > 0.f) x = fmaf(__uint_as_float(s[32 + e]), ub, x);
+            s[e] = __float_as_uint(x);
+          }
+          if (!mine) continue;
+          if (g.piece >= 0) {
+#pragma unroll
+            for (int ch = 0; ch < 8; ++ch)
+              *reinterpret_cast<uint4*>(part + ((c0 + cc * 32) / 4 + ch) * (kTreeRows * 4) + r * 4) =
+                  make_uint4(s[ch * 4], s[ch * 4 + 1], s[ch * 4 + 2], s[ch * 4 + 3]);
+          } else {
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) {
+              uint4 w;
+              w.x = pack2<BF16>(__uint_as_float(s[ch * 8 + 0]), __uint_as_float(s[ch * 8 + 1]));
+              w.y = pack2<BF16>(__uint_as_float(s[ch * 8 + 2]), __uint_as_float(s[ch * 8 + 3]));
+              w.z = pack2<BF16>(__uint_as_float(s[ch * 8 + 4]), __uint_as_float(s[ch * 8 + 5]));
+              w.w = pack2<BF16>(__uint_as_float(s[ch * 8 + 6]), __uint_as_float(s[ch * 8 + 7]));
+              *reinterpret_cast<uint4*>(orow + c0 + cc * 32 + ch * 8) = w;
+            }
+          }
+        }
+        if (mine && t == 0) {
+          if (g.piece >= 0)
+            *reinterpret_cast<float2*>(part + kTreeRows * D + r * 2) = make_float2(l > 0.f ? m : -INFINITY, l);
+          else if (a.lse)
+            a.lse[(static_cast<int64_t>(g.b) * a.Hq + head) * a.T + draft] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        }
+      }
+      ptx::tc_fence_before();
+      ptx::named_barrier(3, kSoft);  // both accumulators and the statistics have been read
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == kIssuer) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, kTmemCols);
+  }
+  if (tid == 0 && ctl->abort_flag && a.status) atomicOr(a.status, kStatusWaitExpired);
+}
+
+// Q as [B][kv head][draft][head of the group][D]: a box is all heads of the group, the drafts of a block and 64 channels.
+bool make_map_q(CUtensorMap* m, int dtype, const TreeArgs& a, int D) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const int group = a.Hq / a.Hkv;
+  cuuint64_t dims[5] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(group), static_cast<cuuint64_t>(a.T),
+                        static_cast<cuuint64_t>(a.Hkv), static_cast<cuuint64_t>(a.B)};
+  cuuint64_t strides[4] = {static_cast<cuuint64_t>(a.qs.h) * 2, static_cast<cuuint64_t>(a.qs.s) * 2, static_cast<cuuint64_t>(a.qs.h) * group * 2,
+                           static_cast<cuuint64_t>(a.qs.b) * 2};
+  cuuint32_t box[5] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(a.block), 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return fn(m, dtype == TT_ATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(a.q), dims, strides,
+            box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool BF16>
+cudaError_t launch_t(int dtype, const TreeArgs& a, int ctas, cudaStream_t stream) {
+  CUtensorMap tq, tk, tv, tkd, tvd;
+  if (!make_map_q(&tq, dtype, a, D) || !make_map(&tk, dtype, a.kc, D, a.capacity, a.Hkv, a.B, a.kcs) ||
+      !make_map(&tv, dtype, a.vc, D, a.capacity, a.Hkv, a.B, a.vcs) || !make_map(&tkd, dtype, a.kd, D, a.T, a.Hkv, a.B, a.kds) ||
+      !make_map(&tvd, dtype, a.vd, D, a.T, a.Hkv, a.B, a.vds))
+    return cudaErrorInvalidValue;
+  auto kern = tree_tc_kernel<D, BF16>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
+  if (e != cudaSuccess) return e;
+  return launch_early(kern, dim3(ctas), dim3(kThreads), Cfg<D>::kSmem, stream, 1, tq, tk, tv, tkd, tvd, a);
+}
+
+}  // namespace
+
+cudaError_t launch_tree_tc(int dtype, int D, const TreeArgs& a, int ctas, cudaStream_t stream) {
+  const bool bf = dtype == TT_ATTN_BF16;
+  if (D == 128) return bf ? launch_t<128, true>(dtype, a, ctas, stream) : launch_t<128, false>(dtype, a, ctas, stream);
+  return bf ? launch_t<64, true>(dtype, a, ctas, stream) : launch_t<64, false>(dtype, a, ctas, stream);
+}
+
+}  // namespace ttattn

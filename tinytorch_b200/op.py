@@ -84,5 +84,21 @@ def sdpAttentionDecodeAppend(q, kNew, vNew, kCache, vCache, kvLens, ropeCos=None
                                         needLse, status)
 
 
+def sdpAttentionTree(q, kDraft, vDraft, kCache, vCache, kvLens=None, treeMask=None, scale=None, needLse=False, workspace=None,
+                     status=None):
+    """Attention of drafted tokens that form a tree (the verification step of speculative decoding): q [B, Hq, T, D] sees the first
+    kvLens[b] rows of the caches [B, Hkv, capacity, D] and, of the T drafts' own keys and values [B, Hkv, T, D], those that
+    treeMask (bool [T, T] or [B, T, T]; row: draft, column: what it sees, itself included as a rule) says; None: a chain.
+    T up to 128.  -> (O [B, Hq, T, D], LSE [B, Hq, T] or None).  The caches are not written: see cacheAccept."""
+    return _capi.native().tree(q, kDraft, vDraft, kCache, vCache, kvLens, treeMask, scale, needLse, workspace, status)
+
+
+def cacheAccept(kDraft, vDraft, kCache, vCache, kvLens, path, counts, status=None):
+    """Accepted drafts go behind the rows of the caches, in place: draft path[b, i] to row kvLens[b] + i for i < counts[b] (int32
+    [B, N] and [B]).  -> newLens = kvLens + the rows written.  A path ends at a draft that does not exist (bit 16 of status) and
+    where the cache is full (bit 4)."""
+    return _capi.native().cache_accept(kDraft, vDraft, kCache, vCache, kvLens, path, counts, status)
+
+
 def workspaceBytes(kind, dtype, B, Hq, Hkv, Lq, Skv, D):
     return int(_capi.lib().tt_attn_workspace_bytes(kind, _DTYPES[dtype], B, Hq, Hkv, Lq, Skv, D))
