@@ -28,7 +28,7 @@ struct NormRopeArgs {
   int axes;
   int axis_end[kMaxAxes];    // the first pair behind an axis's section
   int32_t* status;
-  int split[2], ctas[2];     // set by the launcher: warps to a token, CTAs
+  int split[2], ctas[2];     // set by the launcher: warps to a token (forward), CTAs
 };
 
 cudaError_t launch_norm_rope(int dtype, int D, const NormRopeArgs& a, int device, cudaStream_t stream);
