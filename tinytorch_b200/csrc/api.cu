@@ -637,7 +637,7 @@ int tt_attn_tree(const tt_attn_tree_params* p) {
   if (p->struct_size != sizeof(tt_attn_tree_params)) return TT_ATTN_ERR_STRUCT;
   if (int rc = check_common(p->dtype, p->B, p->Hq, p->Hkv, p->T, p->capacity, p->D)) return rc;
   if (int rc = tree_limits(p->dtype, p->Hq, p->Hkv, p->T)) return rc;
-  if (tree_line(p->dtype, p->B, p->Hq, p->Hkv, p->T, p->capacity) > 1e9) return TT_ATTN_ERR_TOO_LARGE;  // (tiles are counted in 32 bits)
+  if (tree_line(p->dtype, p->B, p->Hq, p->Hkv, p->T, p->capacity, p->D) > 1e9) return TT_ATTN_ERR_TOO_LARGE;  // (tiles are counted in 32 bits)
   if (!p->q || !p->k_draft || !p->v_draft || !p->k || !p->v || !p->o) return TT_ATTN_ERR_NULL;
   const size_t es = elem_size(p->dtype);
   TreeArgs a{};

@@ -3,8 +3,9 @@
 //
 // The rows of one (sequence, kv head) are its T drafts times the G query heads of the group, row t * G + g, in blocks of whole
 // drafts.  Their keys are the tiles of the cache's valid rows, then those of the drafts themselves, of which a row sees what
-// the mask says.  All tiles of all (sequence, kv head, block) stand in one line, and every CTA takes an equal piece of it: the whole
-// machine reads to the end whatever the lengths are, and a walk is broken only where a piece ends.  A broken walk leaves unnormalised
+// the mask says.  All tiles of all (sequence, kv head, block) stand in one line, the end of each walk counting
+// for some more, and every CTA takes an equal piece of it: the whole machine reads to the end whatever the lengths are, and a
+// walk is broken only where a piece ends.  A broken walk leaves unnormalised
 // sums, maxima and weights in scratch memory, two at most to a CTA (one that it goes on with, one that it leaves to others),
 // and a second kernel puts them together in order.
 #pragma once
@@ -28,7 +29,8 @@ struct TreeArgs {
   int64_t mask_b, mask_t;
   int32_t* status;
   int block, n_blocks;  // drafts of a block, blocks
-  int least;            // tiles of a CTA's piece, at least
+  int least;            // tiles of a CTA's piece, about, at least
+  int ends;             // what the end of a walk counts for in the line, in tiles
   float* partial;       // [CTAs][2] of tree_partial_floats
   int4* pieces;         // [CTAs]: pieces of the walk that begins in this CTA and goes on, sequence, kv head, block
 };
@@ -41,6 +43,7 @@ __host__ __device__ constexpr size_t tree_partial_floats(int D) { return static_
 // A CTA's part of one walk: tiles [j0, j0 + n) of n_all, the first n_ctx of which are the cache's.
 struct TreeSegment {
   int b, hk, block, j0, n, n_all, n_ctx, len;
+  int at;     // where it begins in the line
   int piece;  // the CTA's first, if it goes on with a walk (0), or the last, if it leaves one (1); -1: whole
 };
 
@@ -58,7 +61,7 @@ __device__ __forceinline__ int tree_tiles(const TreeArgs& a, int b, int* len) {
 // Where a CTA's piece begins and ends in the line.
 struct TreeWalk {
   int at, end;       // tiles of the line
-  int per;           // tiles of a piece
+  int line, ctas;    // tiles of the line; CTAs that have a piece
   int b, unit, j;    // the sequence, (kv head, block) and tile of `at`
   int n_all, len;
 
@@ -69,25 +72,11 @@ struct TreeWalk {
     constexpr int kW = THREADS / 32;
     int* s_found = s_sum + kW;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, units = a.Hkv * a.n_blocks;
-    int own = 0, l;
-    for (int i = tid; i < a.B; i += THREADS) own += tree_tiles<KT>(a, i, &l);
-    own = __reduce_add_sync(0xffffffffu, own);
-    if (lane == 0) s_sum[warp] = own;
-    __syncthreads();
-    int total = 0;
-    for (int w = 0; w < kW; ++w) total += s_sum[w];
-    const int line = total * units, ctas = gridDim.x;
-    per = (line + ctas - 1) / ctas;
-    if (per < a.least) per = a.least;
-    // (32 bits: the launcher has seen to it that the line, and with it every product here, fits)
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * per;
-    at = first < line ? static_cast<int>(first) : line;
-    end = first + per < line ? static_cast<int>(first + per) : line;
-    int before = 0;
-    for (int base = 0; base < a.B; base += THREADS) {
-      const int i = base + tid;
-      const int n = i < a.B ? tree_tiles<KT>(a, i, &l) : 0;
-      int upto = n;
+    // totals up to every sequence: in one go where there are no more sequences than threads
+    int total = 0, l, upto = 0, n = 0;
+    auto scan = [&](int base) {  // of the sequences base ...: `n` and `upto` of this thread's, and what all of them come to
+      n = base + tid < a.B ? tree_tiles<KT>(a, base + tid, &l) + a.ends : 0;
+      upto = n;
 #pragma unroll
       for (int of = 1; of < 32; of <<= 1) {
         const int o = __shfl_up_sync(0xffffffffu, upto, of);
@@ -97,12 +86,25 @@ struct TreeWalk {
       if (lane == 31) s_sum[warp] = upto;
       __syncthreads();
       int all = 0;
+#pragma unroll
       for (int w = 0; w < kW; ++w) {
-        if (w < warp) upto += s_sum[w];
-        all += s_sum[w];
+        const int x = s_sum[w];
+        if (w < warp) upto += x;
+        all += x;
       }
+      return all;
+    };
+    for (int base = 0; base < a.B; base += THREADS) total += scan(base);
+    line = total * units;  // (the launcher has seen to it that it fits 32 bits)
+    ctas = line / a.least < static_cast<int>(gridDim.x) ? line / a.least + 1 : gridDim.x;
+    const int me = static_cast<int>(blockIdx.x) < ctas ? blockIdx.x : ctas;
+    at = static_cast<int>(static_cast<int64_t>(line) * me / ctas);
+    end = me < ctas ? static_cast<int>(static_cast<int64_t>(line) * (me + 1) / ctas) : at;
+    int before = 0;
+    for (int base = 0; base < a.B; base += THREADS) {
+      const int all = a.B > THREADS ? scan(base) : total;
       const int lo = (before + upto - n) * units, hi = (before + upto) * units;
-      if (at >= lo && at < hi) s_found[0] = i, s_found[1] = lo;
+      if (at >= lo && at < hi) s_found[0] = base + tid, s_found[1] = lo;
       before += all;
       if (at < before * units) break;  // (the same for every thread)
     }
@@ -112,29 +114,41 @@ struct TreeWalk {
       b = s_found[0];
       n_all = tree_tiles<KT>(a, b, &len);
       const int off = at - s_found[1];
-      unit = off / n_all, j = off - unit * n_all;
+      unit = off / (n_all + a.ends), j = off - unit * (n_all + a.ends);
     }
   }
 
   // The next part of a walk, or false.
   template <int KT>
   __device__ bool next(const TreeArgs& a, TreeSegment* s) {
+    if (j >= n_all) {  // (the piece begins in the end of a walk)
+      at += n_all + a.ends - j;
+      advance<KT>(a);
+    }
     if (at >= end) return false;
     s->b = b, s->hk = unit / a.n_blocks, s->block = unit - s->hk * a.n_blocks;
     s->j0 = j, s->n_all = n_all, s->len = len, s->n_ctx = (len + KT - 1) / KT;
+    s->at = at;
     const int left = n_all - j, room = end - at;
     s->n = left < room ? left : room;
     s->piece = j > 0 ? 0 : (s->n < n_all ? 1 : -1);
-    at += s->n, j = 0;
+    at += s->n + (s->n == left ? a.ends : 0);
+    advance<KT>(a);
+    return true;
+  }
+  template <int KT>
+  __device__ void advance(const TreeArgs& a) {
+    j = 0;
     if (++unit == a.Hkv * a.n_blocks) {
       unit = 0;
       if (++b < a.B) n_all = tree_tiles<KT>(a, b, &len);
     }
-    return true;
   }
 
-  // CTAs that a walk takes which has `left` tiles from tile `begin` of the line on, `begin` lying in this CTA's piece
-  __device__ int pieces(int begin, int left) const { return (begin + left - 1) / per - static_cast<int>(blockIdx.x) + 1; }
+  // CTAs that the walk takes which begins with this segment
+  __device__ int pieces(const TreeSegment& s) const {
+    return static_cast<int>((static_cast<int64_t>(s.at + s.n_all) * ctas - 1) / line) - static_cast<int>(blockIdx.x) + 1;
+  }
 };
 
 // What draft t sees of the drafts: bit j of words[j / 32].
@@ -179,7 +193,7 @@ void tree_plan(int dtype, int Hq, int Hkv, int T, int* block, int* n_blocks);
 int tree_ctas(int dtype, int B, int Hq, int Hkv, int T, int capacity, int D);
 size_t tree_scratch_bytes(int dtype, int B, int Hq, int Hkv, int T, int capacity, int D);
 // longest line that a call can have; the launchers take up to 2^31 - 1
-double tree_line(int dtype, int B, int Hq, int Hkv, int T, int capacity);
+double tree_line(int dtype, int B, int Hq, int Hkv, int T, int capacity, int D);
 
 cudaError_t launch_tree(int dtype, int D, TreeArgs a, void* scratch, int device, cudaStream_t stream);
 cudaError_t launch_tree_tc(int dtype, int D, const TreeArgs& a, int ctas, cudaStream_t stream);

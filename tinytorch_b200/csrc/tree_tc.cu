@@ -115,7 +115,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (uint32_t i = 0; ok; ++i) {
         TreeSegment s;
-        const int begin = walk.at;
         const bool some = walk.next<BN>(a, &s);
         if (!some) s.n = -1;
         const int slot = i & 1;
@@ -123,12 +122,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ctl->seg[slot] = s;
         ptx::mbar_arrive(&ctl->seg_full[slot]);
         if (!some) break;
-        if (s.piece == 1) a.pieces[blockIdx.x] = make_int4(walk.pieces(begin, s.n_all), s.b, s.hk, s.block);
-        if (!ptx::mbar_wait(&ctl->q_empty, (i & 1) ^ 1, abort_flag)) break;
-        ptx::mbar_arrive_expect_tx(&ctl->q_full, kHalves * group * a.block * 128);
-#pragma unroll
-        for (int hf = 0; hf < kHalves; ++hf)
-          ptx::tma_load_5d(sQ + hf * kHalfBytes, &tmQ, &ctl->q_full, hf * 64, 0, s.block * a.block, s.hk, s.b);
+        if (s.piece == 1) a.pieces[blockIdx.x] = make_int4(walk.pieces(s), s.b, s.hk, s.block);
         auto load = [&](uint8_t* dst, const CUtensorMap* cache, const CUtensorMap* drafts, uint64_t* full, uint64_t* empty, int j) {
           const uint32_t gj = g + j;
           const int st = gj % kStages, tile = s.j0 + j;
@@ -140,11 +134,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int hf = 0; hf < kHalves; ++hf) ptx::tma_load_4d(dst + st * kTile + hf * kHalfBytes, map, &full[st], hf * 64, row, s.hk, s.b);
           return true;
         };
-        // K a tile ahead of V, as the products consume them
-        ok = load(sK, &tmK, &tmKd, ctl->k_full, ctl->k_empty, 0);
+        // The first two K tiles under the segment before, whose last products still need its Q; then K two tiles ahead of V, as the
+        // products consume them
+        for (int j = 0; j < 2 && j < s.n && ok; ++j) ok = load(sK, &tmK, &tmKd, ctl->k_full, ctl->k_empty, j);
+        if (!ok || !ptx::mbar_wait(&ctl->q_empty, (i & 1) ^ 1, abort_flag)) break;
+        ptx::mbar_arrive_expect_tx(&ctl->q_full, kHalves * group * a.block * 128);
+#pragma unroll
+        for (int hf = 0; hf < kHalves; ++hf)
+          ptx::tma_load_5d(sQ + hf * kHalfBytes, &tmQ, &ctl->q_full, hf * 64, 0, s.block * a.block, s.hk, s.b);
         for (int j = 0; j < s.n && ok; ++j) {
-          if (j + 1 < s.n) ok = load(sK, &tmK, &tmKd, ctl->k_full, ctl->k_empty, j + 1);
-          if (ok) ok = load(sV, &tmV, &tmVd, ctl->v_full, ctl->v_empty, j);
+          ok = load(sV, &tmV, &tmVd, ctl->v_full, ctl->v_empty, j);
+          if (j + 2 < s.n && ok) ok = load(sK, &tmK, &tmKd, ctl->k_full, ctl->k_empty, j + 2);
         }
         g += s.n;
       }
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool mine = r < rows, warp_has = (warp & 3) * 32 < rows;
       const int draft = draft0 + r / group, head = g.hk * group + r % group;
       uint32_t sees[4] = {0, 0, 0, 0};
-      if (mine && g.j0 + g.n == g.n_all) tree_mask_row<4>(a, g.b, draft, sees);
+      if (mine && g.j0 + g.n == g.n_all && ((g.n - 1) & 1) == t) tree_mask_row<4>(a, g.b, draft, sees);
 
       float m_ref = mine ? -INFINITY : 0.f;  // reference maximum, in log2 units
       float2 l2 = make_float2(0.f, 0.f);
@@ -328,63 +328,65 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       cnt += n_t, tiles += g.n;
 
-      // both halves
-      const bool two = g.n > 1;
+      // Both halves, in the same lanes: warpgroup t puts the channels [64 t, 64 t + 64) together (D = 64: warpgroup 0 all of them).  It holds them in
+      // registers before the barrier, behind which the accumulators may be overwritten while it still works on them.
+      const bool two = g.n > 1, puts = warp_has && (D == 128 || t == 0);
+      const int c0 = D == 128 ? t * 64 : 0;
       if (ok) ok = ptx::mbar_wait(&ctl->o_full[0], ends[0] & 1, abort_flag);
       if (ok && two) ok = ptx::mbar_wait(&ctl->o_full[1], ends[1] & 1, abort_flag);
       ++ends[0], ends[1] += two;
-      s_stat[t * BM + r] = make_float2(n_t > 0 ? m_ref : -INFINITY, l2.x + l2.y);
-      if (ptx::named_barrier_or(3, kSoft, !ok)) break;
       ptx::tc_fence_after();
-      if (warp_has && (D == 128 || t == 0)) {
+      // (with tiles for both halves, the products that were waited for say that the other has read the statistics of the segment before)
+      if (!two) ptx::named_barrier(3, kSoft);
+      s_stat[t * BM + r] = make_float2(n_t > 0 ? m_ref : -INFINITY, l2.x + l2.y);
+      if (puts) {
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          ptx::tmem_ld32p(tmem + 256 + lane_addr + c0 + cc * 32, s + cc * 32);
+          if (two) ptx::tmem_ld32p(tmem + 256 + D + lane_addr + c0 + cc * 32, s + 64 + cc * 32);
+        }
+        ptx::tmem_wait_ld();
+      }
+      ptx::tc_fence_before();
+      if (ptx::named_barrier_or(3, kSoft, !ok)) break;
+      if (puts && mine) {
         const float2 sa = s_stat[r], sb = s_stat[BM + r];
         const float m = fmaxf(sa.x, sb.x);
         const float wa = sa.x == -INFINITY ? 0.f : ptx::ex2(sa.x - m), wb = sb.x == -INFINITY ? 0.f : ptx::ex2(sb.x - m);
         const float l = sa.y * wa + sb.y * wb;
-        const int c0 = D == 128 ? t * 64 : 0;
         const float inv = g.piece >= 0 ? 1.f : (l > 0.f ? 1.f / l : 0.f);
         const float ua = wa * inv, ub = wb * inv;
         float* part = a.partial + (static_cast<size_t>(blockIdx.x) * 2 + (g.piece > 0 ? 1 : 0)) * tree_partial_floats(D);
         T* orow = reinterpret_cast<T*>(a.o) + g.b * a.os.b + head * a.os.h + draft * a.os.s;
 #pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          ptx::tmem_ld32p(tmem + 256 + lane_addr + c0 + cc * 32, s);
-          if (two) ptx::tmem_ld32p(tmem + 256 + D + lane_addr + c0 + cc * 32, s + 32);
-          ptx::tmem_wait_ld();
+        for (int e = 0; e < 64; ++e) {
+          // (a half that has seen no key for the row holds zeros, or nothing at all: it takes no part)
+          float x = ua > 0.f ? __uint_as_float(s[e]) * ua : 0.f;
+          if (two && ub > 0.f) x = fmaf(__uint_as_float(s[64 + e]), ub, x);
+          s[e] = __float_as_uint(x);
+        }
+        if (g.piece >= 0) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            // (a half that has seen no key for the row holds zeros, or nothing at all: it takes no part)
-            float x = ua > 0.f ? __uint_as_float(s[e]) * ua : 0.f;
-            if (two && ub > 0.f) x = fmaf(__uint_as_float(s[32 + e]), ub, x);
-            s[e] = __float_as_uint(x);
-          }
-          if (!mine) continue;
-          if (g.piece >= 0) {
+          for (int ch = 0; ch < 16; ++ch)
+            *reinterpret_cast<uint4*>(part + (c0 / 4 + ch) * (kTreeRows * 4) + r * 4) = make_uint4(s[ch * 4], s[ch * 4 + 1], s[ch * 4 + 2], s[ch * 4 + 3]);
+        } else {
 #pragma unroll
-            for (int ch = 0; ch < 8; ++ch)
-              *reinterpret_cast<uint4*>(part + ((c0 + cc * 32) / 4 + ch) * (kTreeRows * 4) + r * 4) =
-                  make_uint4(s[ch * 4], s[ch * 4 + 1], s[ch * 4 + 2], s[ch * 4 + 3]);
-          } else {
-#pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-              uint4 w;
-              w.x = pack2<BF16>(__uint_as_float(s[ch * 8 + 0]), __uint_as_float(s[ch * 8 + 1]));
-              w.y = pack2<BF16>(__uint_as_float(s[ch * 8 + 2]), __uint_as_float(s[ch * 8 + 3]));
-              w.z = pack2<BF16>(__uint_as_float(s[ch * 8 + 4]), __uint_as_float(s[ch * 8 + 5]));
-              w.w = pack2<BF16>(__uint_as_float(s[ch * 8 + 6]), __uint_as_float(s[ch * 8 + 7]));
-              *reinterpret_cast<uint4*>(orow + c0 + cc * 32 + ch * 8) = w;
-            }
+          for (int ch = 0; ch < 8; ++ch) {
+            uint4 w;
+            w.x = pack2<BF16>(__uint_as_float(s[ch * 8 + 0]), __uint_as_float(s[ch * 8 + 1]));
+            w.y = pack2<BF16>(__uint_as_float(s[ch * 8 + 2]), __uint_as_float(s[ch * 8 + 3]));
+            w.z = pack2<BF16>(__uint_as_float(s[ch * 8 + 4]), __uint_as_float(s[ch * 8 + 5]));
+            w.w = pack2<BF16>(__uint_as_float(s[ch * 8 + 6]), __uint_as_float(s[ch * 8 + 7]));
+            *reinterpret_cast<uint4*>(orow + c0 + ch * 8) = w;
           }
         }
-        if (mine && t == 0) {
+        if (t == 0) {
           if (g.piece >= 0)
             *reinterpret_cast<float2*>(part + kTreeRows * D + r * 2) = make_float2(l > 0.f ? m : -INFINITY, l);
           else if (a.lse)
             a.lse[(static_cast<int64_t>(g.b) * a.Hq + head) * a.T + draft] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
         }
       }
-      ptx::tc_fence_before();
-      ptx::named_barrier(3, kSoft);  // both accumulators and the statistics have been read
     }
   }
 
