@@ -160,7 +160,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t kHi = ptx::smem_desc_hi_sw128(1024);
       const uint32_t qlo = ptx::smem_desc_lo(ptx::smem_u32(sQ), 16), klo = ptx::smem_desc_lo(ptx::smem_u32(sK), 16);
       const uint32_t vlo = ptx::smem_desc_lo(ptx::smem_u32(sV), kHalfBytes);
-      uint32_t g0 = 0, done[2] = {0, 0};  // ring position of the segment; softmax iterations of each half (p_full phases)
+      // Tiles are used in order, so stages and phases are counted up: this warp sets the pace of a tile, and a remainder by
+      // three for each of them shows.
+      int kst = 0, vst = 0;
+      uint32_t kph = 0, vph = 0, done0 = 0, done1 = 0;  // done: softmax iterations of each half (p_full phases)
       bool ok = true;
       for (uint32_t i = 0; ok; ++i) {
         const int slot = i & 1;
@@ -169,41 +172,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (leader) ptx::mbar_arrive(&ctl->seg_empty[slot]);
         if (n < 0) break;
-        auto qk = [&](int t, int j) {
-          const uint32_t b0 = klo + ((g0 + j) % kStages) * (kTile >> 4), d = tmem + t * BN;
+        auto qk = [&](int t, bool last) {
+          const uint32_t b0 = klo + kst * (kTile >> 4), d = tmem + t * BN;
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks) {
             const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
             if (leader) ptx::mma_ss2(d, qlo + off, kHi, b0 + off, kHi, idesc_qk, ks > 0 ? 1u : 0u);
           }
           if (leader) ptx::mma_commit(&ctl->s_full[t]);
-          if (leader) ptx::mma_commit(&ctl->k_empty[(g0 + j) % kStages]);
-          if (leader && j == n - 1) ptx::mma_commit(&ctl->q_empty);
+          if (leader) ptx::mma_commit(&ctl->k_empty[kst]);
+          if (leader && last) ptx::mma_commit(&ctl->q_empty);
+          if (++kst == kStages) kst = 0, kph ^= 1;
         };
-        auto wait_k = [&](int j) { return uwait(&ctl->k_full[(g0 + j) % kStages], ((g0 + j) / kStages) & 1); };
         if (!(ok = uwait(&ctl->q_full, i & 1))) break;
-        for (int t = 0; t < 2 && t < n; ++t) {
-          if (!(ok = wait_k(t))) break;
-          ptx::tc_fence_after();
-          qk(t, t);
-        }
-        for (int j = 0; j < n && ok; ++j) {
-          const int t = j & 1;
-          const uint32_t g = g0 + j;
-          bool all = ptx::mbar_wait(&ctl->v_full[g % kStages], (g / kStages) & 1, abort_flag);
-          if (j + 2 < n && all) all = ptx::mbar_wait(&ctl->k_full[(g + 2) % kStages], ((g + 2) / kStages) & 1, abort_flag);
-          if (all) all = ptx::mbar_wait(&ctl->p_full[t], ((t == 0 ? done[0] : done[1]) + (j >> 1)) & 1, abort_flag);
-          if (!(ok = __all_sync(0xffffffffu, all) != 0)) break;
-          ptx::tc_fence_after();
-          const uint32_t b0 = vlo + (g % kStages) * (kTile >> 4), d = tmem + 256 + t * D, a0 = tmem + t * BN;
 #pragma unroll
-          for (int ks = 0; ks < BN / 16; ++ks)
-            if (leader) ptx::mma_ts2(d, a0 + ks * 8, b0 + ks * (2048 >> 4), kHi, idesc_pv, (j >= 2 || ks > 0) ? 1u : 0u);
-          if (leader && j + 2 >= n) ptx::mma_commit(&ctl->o_full[t]);
-          if (leader) ptx::mma_commit(&ctl->v_empty[g % kStages]);
-          if (j + 2 < n) qk(t, j + 2);
+        for (int t = 0; t < 2; ++t) {
+          if (t >= n || !ok) continue;
+          if (!(ok = uwait(&ctl->k_full[kst], kph))) continue;
+          ptx::tc_fence_after();
+          qk(t, t == n - 1);
         }
-        g0 += n, done[0] += (n + 1) / 2, done[1] += n / 2;
+        for (int j0 = 0; j0 < n && ok; j0 += 2) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int j = j0 + t;
+            if (j >= n || !ok) continue;
+            const bool more = j + 2 < n;
+            // (the wait for P comes last: it is the one on the critical path)
+            bool all = ptx::mbar_wait(&ctl->v_full[vst], vph, abort_flag);
+            if (more && all) all = ptx::mbar_wait(&ctl->k_full[kst], kph, abort_flag);
+            if (all) all = ptx::mbar_wait(&ctl->p_full[t], (t == 0 ? done0 : done1) & 1, abort_flag);
+            if (!(ok = __all_sync(0xffffffffu, all) != 0)) continue;
+            ptx::tc_fence_after();
+            (t == 0 ? done0 : done1) += 1;
+            const uint32_t b0 = vlo + vst * (kTile >> 4), d = tmem + 256 + t * D, a0 = tmem + t * BN;
+#pragma unroll
+            for (int ks = 0; ks < BN / 16; ++ks)
+              if (leader) ptx::mma_ts2(d, a0 + ks * 8, b0 + ks * (2048 >> 4), kHi, idesc_pv, (j0 > 0 || ks > 0) ? 1u : 0u);
+            if (leader && !more) ptx::mma_commit(&ctl->o_full[t]);
+            if (leader) ptx::mma_commit(&ctl->v_empty[vst]);
+            if (++vst == kStages) vst = 0, vph ^= 1;
+            if (more) qk(t, j + 3 == n);
+          }
+        }
       }
     }
   } else {
