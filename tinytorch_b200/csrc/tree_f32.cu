@@ -303,7 +303,8 @@ cudaError_t launch_combine(int D, const TreeArgs& a, int ctas, cudaStream_t stre
 
 void tree_plan(int dtype, int Hq, int Hkv, int T, int* block, int* n_blocks) {
   const int group = Hq / Hkv, most = dtype == TT_ATTN_F32 ? 32 : kTreeRows;
-  *block = most / group < T ? most / group : T;  // (groups of more heads than rows are refused)
+  const int fit = most / group < T ? most / group : T;  // (groups of more heads than rows are refused)
+  *block = (T + (T + fit - 1) / fit - 1) / ((T + fit - 1) / fit);  // as equal as can be
   *n_blocks = (T + *block - 1) / *block;
 }
 

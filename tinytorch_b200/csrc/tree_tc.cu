@@ -5,12 +5,16 @@
 // that its 64 KB (D = 128) take to arrive, 2800 cycles of an SM's share of the bandwidth.  The key tiles of a walk go to the
 // two halves of the CTA in turn:
 //   warp 8     producer: publishes the segments, loads Q (one 5-D box: heads of the group inside drafts) and streams K and V tiles
-//              of 128 keys through rings of three stages (six for D = 64), the cache's and then the drafts'; it runs ahead across segments
+//              of 128 keys, the cache's and then the drafts', through a ring in the order in which the products take them; it runs ahead
+//              across segments
 //   warp 9     issuer: S_t = Q K^T and O_t += P_t V with tcgen05.mma, P_t from TMEM
 //   warps 0-3 / 4-7: softmax of half t.  Thread r owns row r (TMEM lane): scores, running maximum and sum, P written over S;
 //              warps without rows skip all of it but the barriers.  V rows behind a sequence's length may hold anything and are
 //              zeroed in shared memory before the product.  The halves' accumulators, in the same lanes, are put together at the end of a
 //              segment by both warpgroups, each for half of the channels.
+// R: a block of up to 32 rows lies in the 128 lanes four times, of up to 64 twice, and each copy takes 32 or 64 keys of every tile (its P is zero
+// for the others): a tile's exponentials then are the work of all four warps of a warpgroup, on all four of an SM's
+// special-function units, instead of one warp's.  The copies are added up through shared memory at the end of a segment.
 // Every mbarrier wait is bounded.
 #include <cuda.h>
 
@@ -28,16 +32,18 @@ constexpr int kHalfBytes = BM * 128;  // a block of 64 channels of a tile
 constexpr int kSoft = 2 * BM;
 constexpr int kProducer = 8, kIssuer = 9;
 
-template <int D>
+template <int D, int R>
 struct Cfg {
-  static constexpr int kTile = BM * D * 2, kStages = D == 128 ? 3 : 6;
-  static constexpr int kSmem = kTile + 2 * kStages * kTile + 512 /* control block */ + 2 * BM * 8 /* statistics */;
+  static constexpr int kTile = BM * D * 2, kRing = (R == 1 ? 6 : 5) * 128 / D;  // tiles of the ring
+  static constexpr int kLanes = BM / R, kKeys = BN / R;                          // lanes of a copy of the rows, its keys of a tile
+  static constexpr int kAddUp = R == 1 ? 0 : 2 * (BM - kLanes) * 32 * 4;         // 32 channels of all copies but the first, for either warpgroup
+  static constexpr int kSmem = kTile + kRing * kTile + 512 /* control block */ + 2 * BM * 8 /* statistics */ + kAddUp;
   static_assert(kSmem <= 232448, "exceeds the shared memory a CTA may request");
 };
 
 struct __align__(16) Ctl {
   uint64_t q_full, q_empty;
-  uint64_t k_full[6], k_empty[6], v_full[6], v_empty[6];
+  uint64_t full[12], empty[12];
   uint64_t s_full[2], p_full[2], o_full[2];
   uint64_t seg_full[2], seg_empty[2];
   TreeSegment seg[2];
@@ -47,23 +53,24 @@ struct __align__(16) Ctl {
 };
 static_assert(sizeof(Ctl) <= 512, "control block");
 
-template <int D, bool BF16>
+template <int D, bool BF16, int R>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const __grid_constant__ CUtensorMap tmKd, const __grid_constant__ CUtensorMap tmVd, const TreeArgs a) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  constexpr int kTile = Cfg<D>::kTile, kStages = Cfg<D>::kStages, kHalves = D / 64;
+  using C = Cfg<D, R>;
+  constexpr int kTile = C::kTile, kRing = C::kRing, kHalves = D / 64, kLanes = C::kLanes, kKeys = C::kKeys;
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((ptx::smem_u32(smem) & 1023u) != 0) {
     if (threadIdx.x == 0 && a.status) atomicOr(a.status, kStatusBadSmemAlign);
     return;
   }
   uint8_t* sQ = smem;
-  uint8_t* sK = sQ + kTile;
-  uint8_t* sV = sK + kStages * kTile;
-  Ctl* ctl = reinterpret_cast<Ctl*>(sV + kStages * kTile);
+  uint8_t* ring = sQ + kTile;
+  Ctl* ctl = reinterpret_cast<Ctl*>(ring + kRing * kTile);
   volatile int* abort_flag = &ctl->abort_flag;
-  float2* s_stat = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(ctl) + 512);  // [half][row]
+  float2* s_stat = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(ctl) + 512);  // [half][lane]
+  float* s_add = reinterpret_cast<float*>(s_stat + 2 * BM);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = a.Hq / a.Hkv;
 
@@ -71,11 +78,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     ptx::mbar_init(&ctl->q_full, 1);
     ptx::mbar_init(&ctl->q_empty, 1);
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) {
-      ptx::mbar_init(&ctl->k_full[i], 1);
-      ptx::mbar_init(&ctl->k_empty[i], 1);
-      ptx::mbar_init(&ctl->v_full[i], 1);
-      ptx::mbar_init(&ctl->v_empty[i], 1);
+    for (int i = 0; i < kRing; ++i) {
+      ptx::mbar_init(&ctl->full[i], 1);
+      ptx::mbar_init(&ctl->empty[i], 1);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -110,7 +115,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     ptx::setmaxnreg_dec<72>();  // (216 + 216 + 72 registers: the 168 x 384 that the CTA was launched with)
     if (warp == kProducer && lane == 0) {
       // -------------------------------------------------------------- producer --
-      uint32_t g = 0;  // tiles requested so far
+      int st = 0;
+      uint32_t ph = 0;  // of the ring
       a.pieces[blockIdx.x] = make_int4(0, 0, 0, 0);
       bool ok = true;
       for (uint32_t i = 0; ok; ++i) {
@@ -123,30 +129,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::mbar_arrive(&ctl->seg_full[slot]);
         if (!some) break;
         if (s.piece == 1) a.pieces[blockIdx.x] = make_int4(walk.pieces(s), s.b, s.hk, s.block);
-        auto load = [&](uint8_t* dst, const CUtensorMap* cache, const CUtensorMap* drafts, uint64_t* full, uint64_t* empty, int j) {
-          const uint32_t gj = g + j;
-          const int st = gj % kStages, tile = s.j0 + j;
-          if (!ptx::mbar_wait(&empty[st], ((gj / kStages) & 1) ^ 1, abort_flag)) return false;
-          ptx::mbar_arrive_expect_tx(&full[st], kTile);
+        auto load = [&](const CUtensorMap* cache, const CUtensorMap* drafts, int j) {
+          const int tile = s.j0 + j;
+          if (!ptx::mbar_wait(&ctl->empty[st], ph ^ 1, abort_flag)) return false;
+          ptx::mbar_arrive_expect_tx(&ctl->full[st], kTile);
           const CUtensorMap* map = tile < s.n_ctx ? cache : drafts;
           const int row = (tile < s.n_ctx ? tile : tile - s.n_ctx) * BN;
 #pragma unroll
-          for (int hf = 0; hf < kHalves; ++hf) ptx::tma_load_4d(dst + st * kTile + hf * kHalfBytes, map, &full[st], hf * 64, row, s.hk, s.b);
+          for (int hf = 0; hf < kHalves; ++hf) ptx::tma_load_4d(ring + st * kTile + hf * kHalfBytes, map, &ctl->full[st], hf * 64, row, s.hk, s.b);
+          if (++st == kRing) st = 0, ph ^= 1;
           return true;
         };
-        // The first two K tiles under the segment before, whose last products still need its Q; then K two tiles ahead of V, as the
-        // products consume them
-        for (int j = 0; j < 2 && j < s.n && ok; ++j) ok = load(sK, &tmK, &tmKd, ctl->k_full, ctl->k_empty, j);
+        // In the order of the products: K0 K1 V0 K2 V1 ...  The first two go under the segment before, whose last products still need its Q.
+        for (int j = 0; j < 2 && j < s.n && ok; ++j) ok = load(&tmK, &tmKd, j);
         if (!ok || !ptx::mbar_wait(&ctl->q_empty, (i & 1) ^ 1, abort_flag)) break;
-        ptx::mbar_arrive_expect_tx(&ctl->q_full, kHalves * group * a.block * 128);
+        ptx::mbar_arrive_expect_tx(&ctl->q_full, R * kHalves * group * a.block * 128);
 #pragma unroll
-        for (int hf = 0; hf < kHalves; ++hf)
-          ptx::tma_load_5d(sQ + hf * kHalfBytes, &tmQ, &ctl->q_full, hf * 64, 0, s.block * a.block, s.hk, s.b);
+        for (int c = 0; c < R; ++c)
+#pragma unroll
+          for (int hf = 0; hf < kHalves; ++hf)
+            ptx::tma_load_5d(sQ + hf * kHalfBytes + c * kLanes * 128, &tmQ, &ctl->q_full, hf * 64, 0, s.block * a.block, s.hk, s.b);
         for (int j = 0; j < s.n && ok; ++j) {
-          ok = load(sV, &tmV, &tmVd, ctl->v_full, ctl->v_empty, j);
-          if (j + 2 < s.n && ok) ok = load(sK, &tmK, &tmKd, ctl->k_full, ctl->k_empty, j + 2);
+          ok = load(&tmV, &tmVd, j);
+          if (j + 2 < s.n && ok) ok = load(&tmK, &tmKd, j + 2);
         }
-        g += s.n;
       }
     } else if (warp == kIssuer) {
       // ---------------------------------------------------------------- issuer --
@@ -158,12 +164,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t idesc_qk = ptx::make_idesc_f16(BM, BN, BF16 ? 1 : 0, 0, 0) | (a.scale < 0.f ? (1u << 13) : 0u);
       const uint32_t idesc_pv = ptx::make_idesc_f16(BM, D, BF16 ? 1 : 0, 0, 1);
       constexpr uint32_t kHi = ptx::smem_desc_hi_sw128(1024);
-      const uint32_t qlo = ptx::smem_desc_lo(ptx::smem_u32(sQ), 16), klo = ptx::smem_desc_lo(ptx::smem_u32(sK), 16);
-      const uint32_t vlo = ptx::smem_desc_lo(ptx::smem_u32(sV), kHalfBytes);
-      // Tiles are used in order, so stages and phases are counted up: this warp sets the pace of a tile, and a remainder by
-      // three for each of them shows.
-      int kst = 0, vst = 0;
-      uint32_t kph = 0, vph = 0, done0 = 0, done1 = 0;  // done: softmax iterations of each half (p_full phases)
+      const uint32_t qlo = ptx::smem_desc_lo(ptx::smem_u32(sQ), 16), klo = ptx::smem_desc_lo(ptx::smem_u32(ring), 16);
+      const uint32_t vlo = ptx::smem_desc_lo(ptx::smem_u32(ring), kHalfBytes);
+      int st = 0;  // the next tile of the ring
+      uint32_t ph = 0, done0 = 0, done1 = 0;  // done: softmax iterations of each half (p_full phases)
       bool ok = true;
       for (uint32_t i = 0; ok; ++i) {
         const int slot = i & 1;
@@ -173,22 +177,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (leader) ptx::mbar_arrive(&ctl->seg_empty[slot]);
         if (n < 0) break;
         auto qk = [&](int t, bool last) {
-          const uint32_t b0 = klo + kst * (kTile >> 4), d = tmem + t * BN;
+          const uint32_t b0 = klo + st * (kTile >> 4), d = tmem + t * BN;
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks) {
             const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
             if (leader) ptx::mma_ss2(d, qlo + off, kHi, b0 + off, kHi, idesc_qk, ks > 0 ? 1u : 0u);
           }
           if (leader) ptx::mma_commit(&ctl->s_full[t]);
-          if (leader) ptx::mma_commit(&ctl->k_empty[kst]);
+          if (leader) ptx::mma_commit(&ctl->empty[st]);
           if (leader && last) ptx::mma_commit(&ctl->q_empty);
-          if (++kst == kStages) kst = 0, kph ^= 1;
+          if (++st == kRing) st = 0, ph ^= 1;
         };
         if (!(ok = uwait(&ctl->q_full, i & 1))) break;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (t >= n || !ok) continue;
-          if (!(ok = uwait(&ctl->k_full[kst], kph))) continue;
+          if (!(ok = uwait(&ctl->full[st], ph))) continue;
           ptx::tc_fence_after();
           qk(t, t == n - 1);
         }
@@ -199,19 +203,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (j >= n || !ok) continue;
             const bool more = j + 2 < n;
             // (the wait for P comes last: it is the one on the critical path)
-            bool all = ptx::mbar_wait(&ctl->v_full[vst], vph, abort_flag);
-            if (more && all) all = ptx::mbar_wait(&ctl->k_full[kst], kph, abort_flag);
+            bool all = ptx::mbar_wait(&ctl->full[st], ph, abort_flag);  // V, and the K behind it
+            if (more && all) all = st + 1 < kRing ? ptx::mbar_wait(&ctl->full[st + 1], ph, abort_flag) : ptx::mbar_wait(&ctl->full[0], ph ^ 1, abort_flag);
             if (all) all = ptx::mbar_wait(&ctl->p_full[t], (t == 0 ? done0 : done1) & 1, abort_flag);
             if (!(ok = __all_sync(0xffffffffu, all) != 0)) continue;
             ptx::tc_fence_after();
             (t == 0 ? done0 : done1) += 1;
-            const uint32_t b0 = vlo + vst * (kTile >> 4), d = tmem + 256 + t * D, a0 = tmem + t * BN;
+            const uint32_t b0 = vlo + st * (kTile >> 4), d = tmem + 256 + t * D, a0 = tmem + t * BN;
 #pragma unroll
             for (int ks = 0; ks < BN / 16; ++ks)
               if (leader) ptx::mma_ts2(d, a0 + ks * 8, b0 + ks * (2048 >> 4), kHi, idesc_pv, (j0 > 0 || ks > 0) ? 1u : 0u);
             if (leader && !more) ptx::mma_commit(&ctl->o_full[t]);
-            if (leader) ptx::mma_commit(&ctl->v_empty[vst]);
-            if (++vst == kStages) vst = 0, vph ^= 1;
+            if (leader) ptx::mma_commit(&ctl->empty[st]);
+            if (++st == kRing) st = 0, ph ^= 1;
             if (more) qk(t, j + 3 == n);
           }
         }
@@ -225,8 +229,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tS = tmem + t * BN + lane_addr, tO = tmem + 256 + t * D + lane_addr;
     const float c = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);  // > 0, so that a hidden score stays -inf
     const float2 c2 = make_float2(c, c);
-    uint32_t cnt = 0, tiles = 0, ends[2] = {0, 0};  // phases of s_full, ring position, phases of o_full
+    const int copy = r / kLanes, row = r % kLanes, col0 = copy * kKeys;  // this lane's copy of the block's rows, its row, and its keys of a tile
+    uint32_t cnt = 0, used = 0, ends[2] = {0, 0};  // phases of s_full, ring position, phases of o_full
     uint32_t s[BN];
+    auto part_of = [&](const TreeSegment& g) { return a.partial + (static_cast<size_t>(blockIdx.x) * 2 + (g.piece > 0 ? 1 : 0)) * tree_partial_floats(D); };
     bool ok = true;
     // Threads meet at named barriers within a segment: an expired wait is voted on, and all leave together.
     for (uint32_t i = 0;; ++i) {
@@ -237,10 +243,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_arrive(&ctl->seg_empty[slot]);
       if (g.n < 0) break;
       const int draft0 = g.block * a.block, drafts = a.T - draft0 < a.block ? a.T - draft0 : a.block, rows = drafts * group;
-      const bool mine = r < rows, warp_has = (warp & 3) * 32 < rows;
-      const int draft = draft0 + r / group, head = g.hk * group + r % group;
-      uint32_t sees[4] = {0, 0, 0, 0};
-      if (mine && g.j0 + g.n == g.n_all && ((g.n - 1) & 1) == t) tree_mask_row<4>(a, g.b, draft, sees);
+      const bool mine = row < rows, warp_has = (warp & 3) * 32 % kLanes < rows;
+      const int draft = draft0 + row / group, head = g.hk * group + row % group;
+      uint32_t sees[kKeys / 32];  // of this copy's keys of the drafts' tile
+#pragma unroll
+      for (int i = 0; i < kKeys / 32; ++i) sees[i] = 0;
+      if (mine && g.j0 + g.n == g.n_all && ((g.n - 1) & 1) == t) {
+        uint32_t words[4];
+        tree_mask_row<4>(a, g.b, draft, words);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i / (kKeys / 32) == copy) sees[i % (kKeys / 32)] = words[i];
+      }
 
       float m_ref = mine ? -INFINITY : 0.f;  // reference maximum, in log2 units
       float2 l2 = make_float2(0.f, 0.f);
@@ -253,10 +267,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int left = tile < g.n_ctx ? g.len - tile * BN : BN;  // valid keys of a tile of the cache
         if (left < BN) {
           // what lies behind the length may be infinite: exact zeros, so that 0 times it is 0
-          const uint32_t gj = tiles + j;
-          ok = ptx::mbar_wait(&ctl->v_full[gj % kStages], (gj / kStages) & 1, abort_flag);
+          const uint32_t at = used + 2 * j + (j == g.n - 1 ? 1 : 2);  // (where V of tile j lies in the order K0 K1 V0 K2 V1 ...)
+          ok = ptx::mbar_wait(&ctl->full[at % kRing], (at / kRing) & 1, abort_flag);
           if (ok && r >= left) {
-            uint8_t* v = sV + (gj % kStages) * kTile + r * 128;
+            uint8_t* v = ring + (at % kRing) * kTile + r * 128;
 #pragma unroll
             for (int hf = 0; hf < kHalves; ++hf)
 #pragma unroll
@@ -266,16 +280,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (warp_has) {
 #pragma unroll
-          for (int cc = 0; cc < 4; ++cc) ptx::tmem_ld32p(tS + cc * 32, s + cc * 32);
+          for (int cc = 0; cc < kKeys / 32; ++cc) ptx::tmem_ld32p(tS + col0 + cc * 32, s + cc * 32);
           ptx::tmem_wait_ld();
           if (tile >= g.n_ctx) {
 #pragma unroll
-            for (int e = 0; e < BN; ++e)
+            for (int e = 0; e < kKeys; ++e)
               if (!((sees[e / 32] >> (e % 32)) & 1)) s[e] = 0xff800000u;
           } else if (left < BN || !mine) {
-            const int lim = mine ? left : 0;
+            const int lim = mine ? left - col0 : 0;
 #pragma unroll
-            for (int e = 0; e < BN; ++e)
+            for (int e = 0; e < kKeys; ++e)
               if (e >= lim) s[e] = 0xff800000u;
           }
           // The maximum is only a reference for the exponentials: it is kept while a tile's sum shows that none is large.
@@ -286,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int q = 0; q < 8; ++q) mx[q] = ptx::max3(__uint_as_float(s[q]), __uint_as_float(s[q + 8]), -INFINITY);
 #pragma unroll
-              for (int e = 16; e < BN; e += 16)
+              for (int e = 16; e < kKeys; e += 16)
 #pragma unroll
                 for (int q = 0; q < 8; ++q) mx[q] = ptx::max3(mx[q], __uint_as_float(s[e + q]), __uint_as_float(s[e + q + 8]));
               const float x_max = ptx::max3(ptx::max3(mx[0], mx[1], mx[2]), ptx::max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * c;
@@ -311,18 +325,29 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float m_use = m_ref == -INFINITY ? 0.f : m_ref;  // (nothing seen so far: exponentials of -inf)
             const float2 nm2 = make_float2(-m_use, -m_use);
             float2 lt = make_float2(0.f, 0.f);
+            constexpr int kPart = kKeys < 64 ? kKeys : 64;  // keys whose P is stored together
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-              uint32_t pk[32];
+            for (int k0 = 0; k0 < kKeys; k0 += kPart) {
+              uint32_t pk[kPart / 2];
 #pragma unroll
-              for (int e2 = 0; e2 < 64; e2 += 2) {
-                const int e = hf * 64 + e2;
-                const float2 x = ptx::fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, nm2);
+              for (int e2 = 0; e2 < kPart; e2 += 2) {
+                const float2 x = ptx::fma2(make_float2(__uint_as_float(s[k0 + e2]), __uint_as_float(s[k0 + e2 + 1])), c2, nm2);
                 const float2 p = make_float2(ptx::ex2(x.x), ptx::ex2(x.y));
                 lt = ptx::add2(lt, p);
                 pk[e2 >> 1] = pack2<BF16>(p.x, p.y);
               }
-              ptx::tmem_st32(tS + hf * 32, pk);
+              if constexpr (R == 4) ptx::tmem_st16(tS + copy * 16, pk);
+              else ptx::tmem_st32(tS + copy * 32 + k0 / 2, pk);
+            }
+            if constexpr (R > 1) {  // the other copies' keys
+              uint32_t zero[kKeys / 2];
+#pragma unroll
+              for (int i = 0; i < kKeys / 2; ++i) zero[i] = 0;
+#pragma unroll
+              for (int i = 1; i < R; ++i) {
+                if constexpr (R == 4) ptx::tmem_st16(tS + (copy + i) % R * 16, zero);
+                else ptx::tmem_st32(tS + (copy + i) % R * 32, zero);
+              }
             }
             const float sum = lt.x + lt.y;
             const bool redo = !need_max && (!(sum <= 256.f) || m_ref == -INFINITY);
@@ -337,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::tc_fence_before();
         ptx::mbar_arrive(&ctl->p_full[t]);
       }
-      cnt += n_t, tiles += g.n;
+      cnt += n_t, used += 2 * g.n;
 
       // Both halves, in the same lanes: warpgroup t puts the channels [64 t, 64 t + 64) together (D = 64: warpgroup 0 all of them).  It holds them in
       // registers before the barrier, behind which the accumulators may be overwritten while it still works on them.
@@ -361,26 +386,62 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::tc_fence_before();
       if (ptx::named_barrier_or(3, kSoft, !ok)) break;
       if (puts && mine) {
-        const float2 sa = s_stat[r], sb = s_stat[BM + r];
-        const float m = fmaxf(sa.x, sb.x);
-        const float wa = sa.x == -INFINITY ? 0.f : ptx::ex2(sa.x - m), wb = sb.x == -INFINITY ? 0.f : ptx::ex2(sb.x - m);
-        const float l = sa.y * wa + sb.y * wb;
+        // over the copies and halves of the row; one that has seen no key for it holds zeros, or nothing at all, and takes no part
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i) m = fmaxf(m, s_stat[i * kLanes + row].x);
+        auto weight = [&](float ref) { return ref == -INFINITY ? 0.f : ptx::ex2(ref - m); };
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i) {
+          const float2 x = s_stat[i * kLanes + row];
+          l = fmaf(x.y, weight(x.x), l);
+        }
         const float inv = g.piece >= 0 ? 1.f : (l > 0.f ? 1.f / l : 0.f);
-        const float ua = wa * inv, ub = wb * inv;
-        float* part = a.partial + (static_cast<size_t>(blockIdx.x) * 2 + (g.piece > 0 ? 1 : 0)) * tree_partial_floats(D);
-        T* orow = reinterpret_cast<T*>(a.o) + g.b * a.os.b + head * a.os.h + draft * a.os.s;
+        const float ua = weight(s_stat[r].x) * inv, ub = weight(s_stat[BM + r].x) * inv;
 #pragma unroll
         for (int e = 0; e < 64; ++e) {
-          // (a half that has seen no key for the row holds zeros, or nothing at all: it takes no part)
           float x = ua > 0.f ? __uint_as_float(s[e]) * ua : 0.f;
           if (two && ub > 0.f) x = fmaf(__uint_as_float(s[64 + e]), ub, x);
           s[e] = __float_as_uint(x);
         }
+        if (t == 0 && copy == 0) {
+          if (g.piece >= 0)
+            *reinterpret_cast<float2*>(part_of(g) + kTreeRows * D + row * 2) = make_float2(l > 0.f ? m : -INFINITY, l);
+          else if (a.lse)
+            a.lse[(static_cast<int64_t>(g.b) * a.Hq + head) * a.T + draft] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        }
+      }
+      if constexpr (R > 1) {
+        if (D == 128 || t == 0) {
+          float* add = s_add + t * (BM - kLanes) * 32;
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {  // 32 channels at a time
+            if (copy > 0 && mine) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) add[e * (BM - kLanes) + r - kLanes] = __uint_as_float(s[cc * 32 + e]);
+            }
+            ptx::named_barrier(1 + t, BM);
+            if (copy == 0 && mine) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                float x = __uint_as_float(s[cc * 32 + e]);
+#pragma unroll
+                for (int i = 0; i < R - 1; ++i) x += add[e * (BM - kLanes) + i * kLanes + row];
+                s[cc * 32 + e] = __float_as_uint(x);
+              }
+            }
+            ptx::named_barrier(1 + t, BM);
+          }
+        }
+      }
+      if (puts && mine && copy == 0) {
         if (g.piece >= 0) {
+          float* part = part_of(g);
 #pragma unroll
           for (int ch = 0; ch < 16; ++ch)
-            *reinterpret_cast<uint4*>(part + (c0 / 4 + ch) * (kTreeRows * 4) + r * 4) = make_uint4(s[ch * 4], s[ch * 4 + 1], s[ch * 4 + 2], s[ch * 4 + 3]);
+            *reinterpret_cast<uint4*>(part + (c0 / 4 + ch) * (kTreeRows * 4) + row * 4) = make_uint4(s[ch * 4], s[ch * 4 + 1], s[ch * 4 + 2], s[ch * 4 + 3]);
         } else {
+          T* orow = reinterpret_cast<T*>(a.o) + g.b * a.os.b + head * a.os.h + draft * a.os.s;
 #pragma unroll
           for (int ch = 0; ch < 8; ++ch) {
             uint4 w;
@@ -390,12 +451,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             w.w = pack2<BF16>(__uint_as_float(s[ch * 8 + 6]), __uint_as_float(s[ch * 8 + 7]));
             *reinterpret_cast<uint4*>(orow + c0 + ch * 8) = w;
           }
-        }
-        if (t == 0) {
-          if (g.piece >= 0)
-            *reinterpret_cast<float2*>(part + kTreeRows * D + r * 2) = make_float2(l > 0.f ? m : -INFINITY, l);
-          else if (a.lse)
-            a.lse[(static_cast<int64_t>(g.b) * a.Hq + head) * a.T + draft] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
         }
       }
     }
@@ -426,17 +481,24 @@ bool make_map_q(CUtensorMap* m, int dtype, const TreeArgs& a, int D) {
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, bool BF16>
-cudaError_t launch_t(int dtype, const TreeArgs& a, int ctas, cudaStream_t stream) {
+template <int D, bool BF16, int R>
+cudaError_t launch_r(int dtype, const TreeArgs& a, int ctas, cudaStream_t stream) {
   CUtensorMap tq, tk, tv, tkd, tvd;
   if (!make_map_q(&tq, dtype, a, D) || !make_map(&tk, dtype, a.kc, D, a.capacity, a.Hkv, a.B, a.kcs) ||
       !make_map(&tv, dtype, a.vc, D, a.capacity, a.Hkv, a.B, a.vcs) || !make_map(&tkd, dtype, a.kd, D, a.T, a.Hkv, a.B, a.kds) ||
       !make_map(&tvd, dtype, a.vd, D, a.T, a.Hkv, a.B, a.vds))
     return cudaErrorInvalidValue;
-  auto kern = tree_tc_kernel<D, BF16>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
+  auto kern = tree_tc_kernel<D, BF16, R>;
+  constexpr int kSmem = Cfg<D, R>::kSmem;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  return launch_early(kern, dim3(ctas), dim3(kThreads), Cfg<D>::kSmem, stream, 1, tq, tk, tv, tkd, tvd, a);
+  return launch_early(kern, dim3(ctas), dim3(kThreads), kSmem, stream, 1, tq, tk, tv, tkd, tvd, a);
+}
+template <int D, bool BF16>
+cudaError_t launch_t(int dtype, const TreeArgs& a, int ctas, cudaStream_t stream) {
+  const int rows = a.block * (a.Hq / a.Hkv);
+  return rows <= 32 ? launch_r<D, BF16, 4>(dtype, a, ctas, stream)
+         : rows <= 64 ? launch_r<D, BF16, 2>(dtype, a, ctas, stream) : launch_r<D, BF16, 1>(dtype, a, ctas, stream);
 }
 
 }  // namespace
