@@ -71,6 +71,25 @@ def test_forward_and_gradients(lens, D, dt, Hq, Hkv, causal):
 
 
 @pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens,Hq,Hkv", [((2000,), 4, 1), ((1500, 3, 700), 8, 1), ((5, 1100, 0, 900), 6, 2)])
+def test_divided_walks(D, causal, lens, Hq, Hkv):
+    """Few key tiles: their walks are divided among the CTAs; dK and dV are the same to the bit every time."""
+    from tinytorch_b200 import op
+    T = sum(lens) + 2
+    q, k, v, g = (make(T, h, D, torch.bfloat16, 30 + i) for i, h in enumerate((Hq, Hkv, Hkv, Hq)))
+    cu = offsets(lens)
+    o, lse = op.sdpAttentionPackedFwd(q, k, v, cu, causal)
+    grads = op.sdpAttentionPackedBwd(g, q, k, v, o, lse, cu, causal)
+    check((o, lse, *grads), q, k, v, lens, causal, g=g)
+    again = op.sdpAttentionPackedBwd(g, q, k, v, o, lse, cu, causal)
+    assert torch.equal(grads[1], again[1]) and torch.equal(grads[2], again[2])
+    for i in (1, 2):
+        one = op.sdpAttentionPackedBwd(g, q, k, v, o, lse, cu, causal, needs=tuple(j == i for j in range(3)))
+        assert torch.equal(one[i], grads[i])
+
+
+@pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("causal", ["bottom-right", True, False])
 @pytest.mark.parametrize("lens,lens_k", [((5, 130, 1), (700, 130, 1)), ((200, 40, 7), (60, 0, 300)), ((0, 300, 1), (9, 299, 1500))])
 def test_keys_with_lengths_of_their_own(D, causal, lens, lens_k):

@@ -175,6 +175,9 @@ int check_packed(int dtype, int n, int Hq, int Hkv, int total_q, int total_k, in
   if (causal < 0 || causal > TT_ATTN_CAUSAL_BOTTOM_RIGHT) return TT_ATTN_ERR_SHAPE;
   return TT_ATTN_OK;
 }
+size_t packed_share_bytes(int n, int Hq, int Hkv, int total_q, int total_k, int D) {
+  return round256(static_cast<size_t>(2) * Hkv * packed_slots(n, total_q, total_k, Hq, Hkv) * 128 * D * sizeof(float));
+}
 Str3 packed_strides(const tt_attn_strides& st, int64_t H, int64_t total, int64_t D) {
   if (st.h == 0 && st.s == 0) return Str3{total * H * D, D, H * D};
   // (a batch of one: its stride is not used, but a tensor map wants one that is no smaller than the others)
@@ -549,7 +552,8 @@ size_t tt_attn_packed_workspace_bytes(int kind, int n, int Hq, int Hkv, int tota
   if (kind == TT_ATTN_KIND_FWD) return 256 + packed_plan_bytes(n, total_q, total_k, Hq / Hkv, false);
   if (kind != TT_ATTN_KIND_BWD) return 0;
   const size_t rows = static_cast<size_t>(Hq) * total_q;
-  return 256 + packed_plan_bytes(n, total_q, total_k, Hq / Hkv, true) + round256(rows * sizeof(float)) + round256(rows * D * sizeof(float));
+  return 256 + packed_plan_bytes(n, total_q, total_k, Hq / Hkv, true) + round256(rows * sizeof(float)) + round256(rows * D * sizeof(float)) +
+         packed_share_bytes(n, Hq, Hkv, total_q, total_k, D);
 }
 
 int tt_attn_packed_fwd(const tt_attn_packed_fwd_params* p) {
@@ -578,7 +582,7 @@ int tt_attn_packed_fwd(const tt_attn_packed_fwd_params* p) {
   const size_t need = 256 + packed_plan_bytes(p->n_seqs, p->total_q, p->total_k, p->Hq / p->Hkv, false);
   if (int rc = ws.acquire(need, p->workspace, p->workspace_bytes, p->alloc, p->device)) return rc;
   a.sched = static_cast<int*>(ws.ptr);
-  const PackedCall c{p->cu_q, p->cu_k ? p->cu_k : p->cu_q, p->n_seqs, p->total_k, static_cast<char*>(ws.ptr) + 256};
+  const PackedCall c{p->cu_q, p->cu_k ? p->cu_k : p->cu_q, p->n_seqs, p->total_k, static_cast<char*>(ws.ptr) + 256, nullptr};
   cudaError_t e = launch_fwd_packed(p->dtype, p->D, a, c, p->device, static_cast<cudaStream_t>(p->stream));
   return e == cudaSuccess ? TT_ATTN_OK : launch_failed(e);
 }
@@ -615,14 +619,16 @@ int tt_attn_packed_bwd(const tt_attn_packed_bwd_params* p) {
   if (rows > 0x7fffffff) return TT_ATTN_ERR_TOO_LARGE;
   DeviceGuard guard(p->device);
   if (!guard.ok) return TT_ATTN_ERR_NO_DEVICE;
-  Workspace ws;  // work counter | plan | delta | dQ accumulator
+  Workspace ws;  // work counter | plan | delta | dQ accumulator | shares of dK and dV
   const size_t plan = packed_plan_bytes(p->n_seqs, p->total_q, p->total_k, p->Hq / p->Hkv, true), delta = round256(rows * sizeof(float));
-  if (int rc = ws.acquire(256 + plan + delta + round256(rows * p->D * sizeof(float)), p->workspace, p->workspace_bytes, p->alloc, p->device)) return rc;
+  const size_t accum = round256(rows * p->D * sizeof(float)), shares = packed_share_bytes(p->n_seqs, p->Hq, p->Hkv, p->total_q, p->total_k, p->D);
+  if (int rc = ws.acquire(256 + plan + delta + accum + shares, p->workspace, p->workspace_bytes, p->alloc, p->device)) return rc;
   char* at = static_cast<char*>(ws.ptr);
   a.sched = reinterpret_cast<int*>(at);
   a.delta = reinterpret_cast<float*>(at + 256 + plan);
   a.dq_accum = reinterpret_cast<float*>(at + 256 + plan + delta);
-  const PackedCall c{p->cu_q, p->cu_k ? p->cu_k : p->cu_q, p->n_seqs, p->total_k, at + 256};
+  const PackedCall c{p->cu_q, p->cu_k ? p->cu_k : p->cu_q, p->n_seqs, p->total_k, at + 256,
+                     shares > 0 ? reinterpret_cast<float*>(at + 256 + plan + delta + accum) : nullptr};
   cudaError_t e = launch_bwd_packed(p->dtype, p->D, a, c, p->device, static_cast<cudaStream_t>(p->stream));
   return e == cudaSuccess ? TT_ATTN_OK : launch_failed(e);
 }

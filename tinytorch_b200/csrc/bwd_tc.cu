@@ -217,7 +217,7 @@ __device__ __forceinline__ void ds_chunk(const uint32_t (&p)[16], const uint32_t
 // GEN: the general variant (a mask and / or a causal triangle that is not top-left
 // aligned); the fast variant compiles all of that out.  PARTS: a key tile's walk is
 // divided among a.parts work items (see bwd_parts).  PACKED: sequences packed behind one another, whose items and tensor
-// maps packed_plan.cu has made; without a mask, undivided.
+// maps packed_plan.cu has made; without a mask; PARTS: some walks are divided (a.parts: slots for shares of dK / dV, per kv head).
 template <bool BF16, bool GEN, bool PARTS, bool PACKED>
 __global__ void __launch_bounds__(Cfg128::kThreads, 1)
     bwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -255,7 +255,8 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
   constexpr bool MASK = GEN && !PACKED;
   const int n_heads = a.Hkv * a.B;
   int n_kt = (a.Skv + BM - 1) / BM, tail_heads = a.tail_heads;  // (packed: the producer asks the plan)
-  int n_items = n_kt * n_heads * (PARTS ? a.parts : 1);
+  constexpr bool EVEN = PARTS && !PACKED;  // every walk is divided into a.parts
+  int n_items = n_kt * n_heads * (EVEN ? a.parts : 1);
   const int n_q_all = (a.Lq + BQ - 1) / BQ;
   auto read_plan = [&]() {
     n_kt = *a.packed.n_items, n_items = n_kt * n_heads;
@@ -266,7 +267,7 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
   auto decode_item = [&](int w) {
     Item it;
     it.part = 0;
-    if (PARTS) it.part = w % a.parts, w /= a.parts;
+    if (EVEN) it.part = w % a.parts, w /= a.parts;
     const int w0 = (n_heads - tail_heads) * n_kt;
     int bh, nt;
     if (w < w0) {
@@ -278,13 +279,15 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
       bh = n_heads - tail_heads + (x - nt * tail_heads);
     }
     it.b = bh / a.Hkv, it.hk = bh - it.b * a.Hkv;
-    int kv_len = a.Skv, Lq = a.Lq, n_q_tiles = n_q_all;
+    int kv_len = a.Skv, Lq = a.Lq, n_q_tiles = n_q_all, from = 0, steps = 0;
+    const int nt0 = nt;
     if constexpr (PACKED) {
       const int4* e = reinterpret_cast<const int4*>(a.packed.items + nt);
       const int4 rows = __ldg(e), place = __ldg(e + 1);
       it.q0 = rows.x, it.lq = Lq = rows.y, it.k0 = rows.z, it.lk = kv_len = rows.w;
       nt = place.x, it.seq = place.y;
       it.n_q = n_q_tiles = (Lq + BQ - 1) / BQ;
+      if (PARTS) from = place.z, steps = place.w, it.part = __ldg(&a.packed.items[nt0].slot);
     }
     it.kv0 = nt * BM;
     if (!PACKED && a.kv_lens) {
@@ -299,8 +302,8 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
     const int per_head = (it.kv0 < kv_len && it.qt_begin < n_q_tiles) ? n_q_tiles - it.qt_begin : 0;
     it.n_steps = per_head * group, it.h = it.hk * group, it.qt = it.qt_begin;
     if (PARTS && per_head > 0) {
-      const int n0 = part_begin(it.n_steps, it.part, a.parts);
-      it.n_steps = part_begin(it.n_steps, it.part + 1, a.parts) - n0;
+      const int n0 = PACKED ? from : part_begin(it.n_steps, it.part, a.parts);
+      it.n_steps = PACKED ? steps : part_begin(it.n_steps, it.part + 1, a.parts) - n0;
       it.h += n0 / per_head, it.qt += n0 % per_head;
     }
     return it;
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
           for (int t = 0; t < 2; ++t) {
             void* base = t == 0 ? a.dv : a.dk;
             const Str3& st = t == 0 ? a.dvs : a.dks;
-            if (!base || PARTS) continue;  // (of a divided key tile the last kernel knows which parts exist)
+            if (!base || EVEN) continue;  // (of a divided key tile the last kernel knows which parts exist)
             T* out = reinterpret_cast<T*>(base) + it.b * st.b + it.hk * st.h + (PACKED ? it.k0 * st.s : 0);
             for (int e = lane; e < BM * (D / 8); e += 32) {
               const int row = it.kv0 + e / (D / 8);
@@ -725,7 +728,7 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
         ptx::tc_fence_after();
         const uint32_t src = (wg == 0 ? tdV : tdK) + lane_addr;
         uint8_t* stage = sdq + wg * (BQ * 128);
-        if constexpr (PARTS) {
+        if (PARTS && (!PACKED || it.part >= 0)) {
           // a part of the key tile's walk: fp32, 32 columns at a time, into its own place in the workspace
 #pragma unroll 1
           for (int cc = 0; cc < D / 32; ++cc) {
@@ -745,7 +748,8 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
             ptx::fence_proxy_async_smem();
             ptx::named_barrier(3 + wg, BM);
             if (r == 0 && ok && wanted) {
-              ptx::tma_store_4d(wg == 0 ? &tmdV : &tmdK, stage, cc * 32, kv0, b * a.Hkv + hk, it.part);
+              if (PACKED) ptx::tma_store_4d(wg == 0 ? &tmdV : &tmdK, stage, cc * 32, 0, hk * a.parts + it.part, 0);
+              else ptx::tma_store_4d(wg == 0 ? &tmdV : &tmdK, stage, cc * 32, kv0, b * a.Hkv + hk, it.part);
               ptx::bulk_commit();
             }
           }
@@ -868,7 +872,8 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
   constexpr bool MASK = GEN && !PACKED;
   const int n_heads = a.Hkv * a.B;
   int n_kt = (a.Skv + BM - 1) / BM, tail_heads = a.tail_heads;  // (packed: the producer asks the plan)
-  int n_items = n_kt * n_heads * (PARTS ? a.parts : 1);
+  constexpr bool EVEN = PARTS && !PACKED;  // every walk is divided into a.parts
+  int n_items = n_kt * n_heads * (EVEN ? a.parts : 1);
   const int n_q_all = (a.Lq + BQ - 1) / BQ;
   auto read_plan = [&]() {
     n_kt = *a.packed.n_items, n_items = n_kt * n_heads;
@@ -879,7 +884,7 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
   auto decode_item = [&](int w) {
     Item it;
     it.part = 0;
-    if (PARTS) it.part = w % a.parts, w /= a.parts;
+    if (EVEN) it.part = w % a.parts, w /= a.parts;
     const int w0 = (n_heads - tail_heads) * n_kt;
     int bh, nt;
     if (w < w0) {
@@ -891,13 +896,15 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
       bh = n_heads - tail_heads + (x - nt * tail_heads);
     }
     it.b = bh / a.Hkv, it.hk = bh - it.b * a.Hkv;
-    int kv_len = a.Skv, Lq = a.Lq, n_q_tiles = n_q_all;
+    int kv_len = a.Skv, Lq = a.Lq, n_q_tiles = n_q_all, from = 0, steps = 0;
+    const int nt0 = nt;
     if constexpr (PACKED) {
       const int4* e = reinterpret_cast<const int4*>(a.packed.items + nt);
       const int4 rows = __ldg(e), place = __ldg(e + 1);
       it.q0 = rows.x, it.lq = Lq = rows.y, it.k0 = rows.z, it.lk = kv_len = rows.w;
       nt = place.x, it.seq = place.y;
       it.n_q = n_q_tiles = (Lq + BQ - 1) / BQ;
+      if (PARTS) from = place.z, steps = place.w, it.part = __ldg(&a.packed.items[nt0].slot);
     }
     it.kv0 = nt * BM;
     if (!PACKED && a.kv_lens) {
@@ -912,8 +919,8 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
     const int per_head = (it.kv0 < kv_len && it.qt_begin < n_q_tiles) ? n_q_tiles - it.qt_begin : 0;
     it.n_steps = per_head * group, it.h = it.hk * group, it.qt = it.qt_begin;
     if (PARTS && per_head > 0) {
-      const int n0 = part_begin(it.n_steps, it.part, a.parts);
-      it.n_steps = part_begin(it.n_steps, it.part + 1, a.parts) - n0;
+      const int n0 = PACKED ? from : part_begin(it.n_steps, it.part, a.parts);
+      it.n_steps = PACKED ? steps : part_begin(it.n_steps, it.part + 1, a.parts) - n0;
       it.h += n0 / per_head, it.qt += n0 % per_head;
     }
     return it;
@@ -1014,7 +1021,7 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
             for (int t = 0; t < 2; ++t) {
               void* base = t == 0 ? a.dv : a.dk;
               const Str3& st = t == 0 ? a.dvs : a.dks;
-              if (!base || PARTS) continue;  // (of a divided key tile the last kernel knows which parts exist)
+              if (!base || EVEN) continue;  // (of a divided key tile the last kernel knows which parts exist)
               T* out = reinterpret_cast<T*>(base) + it.b * st.b + it.hk * st.h + (PACKED ? it.k0 * st.s : 0);
               for (int e = lane; e < BM * (D / 8); e += 32) {
                 const int row = it.kv0 + e / (D / 8);
@@ -1230,6 +1237,7 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
       Item it = ctl->item[slot];
       ptx::mbar_arrive(&ctl->item_empty[slot]);
       if (!ok || it.n_steps < 0) break;
+      const bool share = PARTS && (!PACKED || it.part >= 0);  // fp32, to the workspace
       const CUtensorMap *mdq = &tmdQ, *mdk = &tmdK, *mdv = &tmdV;
       if constexpr (PACKED) {
         mdq = map_of(it.seq, kMapdQ), mdk = map_of(it.seq, kMapdK), mdv = map_of(it.seq, kMapdV);
@@ -1247,7 +1255,7 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
             uint32_t v[32];
             ptx::tmem_ld32(tdV + lane_addr + c * 32, v);
             // the previous store / reduction has read the box (16 bits: both pieces of a tensor go into one)
-            if (lane == 0 && (PARTS || !half)) ptx::bulk_wait_read();
+            if (lane == 0 && (share || !half)) ptx::bulk_wait_read();
             ptx::tmem_wait_ld();
             if (c == 3) {
               // the accumulators may be overwritten by the next item's first products
@@ -1255,7 +1263,7 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
               ptx::mbar_arrive(&ctl->acc_free);
             }
             __syncwarp();
-            if (PARTS) {  // a part of the key tile's walk: fp32, into its own place in the workspace
+            if (share) {  // a part of the key tile's walk: fp32, into its own place in the workspace
 #pragma unroll
               for (int ch = 0; ch < 8; ++ch)
                 *reinterpret_cast<uint4*>(box + lane * 128 + ((ch ^ (lane & 7)) << 4)) =
@@ -1271,11 +1279,13 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
                 *reinterpret_cast<uint4*>(box + lane * 128 + ((((c & 1) * 4 + j) ^ (lane & 7)) << 4)) = w4;
               }
             }
-            if (!PARTS && !half) continue;
+            if (!share && !half) continue;
             ptx::fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0 && ok && (is_v ? a.dv != nullptr : a.dk != nullptr) && it.kv0 + wj * 32 < (PACKED ? it.lk : a.Skv)) {
-              if (PARTS)
+              if (share && PACKED)
+                ptx::tma_store_4d(is_v ? &tmdV : &tmdK, box, (c & 1) * 32, wj * 32, it.hk * a.parts + it.part, 0);
+              else if (share)
                 ptx::tma_store_4d(is_v ? &tmdV : &tmdK, box, (c & 1) * 32, it.kv0 + wj * 32, it.b * a.Hkv + it.hk, it.part);
               else
                 ptx::tma_store_4d(is_v ? mdv : mdk, box, 0, it.kv0 + wj * 32, it.hk, it.b);
@@ -1523,6 +1533,34 @@ cudaError_t launch_t(const BwdArgs& a, int dtype, int device, cudaStream_t strea
   return launch_early(dq_convert_kernel<T, D>, dim3(blocks), dim3(256), 0, stream, 1, a);
 }
 
+// dK and dV of divided key tiles: the sum of their shares, in order.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) packed_sum_kernel(const BwdArgs a) {
+  ptx::grid_dep_wait();
+  const int n = a.packed.n_items[1];
+  const int64_t per_split = 2ll * a.Hkv * BM * (D / 8), step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const int64_t shares = static_cast<int64_t>(a.Hkv) * a.parts * BM * D;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n * per_split; i += step) {
+    const PackedSplit sp = a.packed.splits[i / per_split];
+    int e = static_cast<int>(i % per_split);
+    const int c8 = e % (D / 8), r = (e /= D / 8) % BM, h = (e /= BM) % a.Hkv;
+    const bool v = e / a.Hkv != 0;
+    T* base = reinterpret_cast<T*>(v ? a.dv : a.dk);
+    if (!base || r >= sp.rows) continue;
+    const Str3& st = v ? a.dvs : a.dks;
+    const float* src = a.dkv_part + v * shares + ((static_cast<int64_t>(h) * a.parts + sp.slot) * BM + r) * D + c8 * 8;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+#pragma unroll 4
+    for (int p = 0; p < sp.parts; ++p) {
+      const float4 u = __ldcs(reinterpret_cast<const float4*>(src + static_cast<int64_t>(p) * BM * D));
+      const float4 w = __ldcs(reinterpret_cast<const float4*>(src + static_cast<int64_t>(p) * BM * D) + 1);
+      x.x += u.x, x.y += u.y, x.z += u.z, x.w += u.w;
+      y.x += w.x, y.y += w.y, y.z += w.z, y.w += w.w;
+    }
+    store8(base + h * st.h + static_cast<int64_t>(sp.row + r) * st.s + c8 * 8, x, y);
+  }
+}
+
 // Packed sequences: the plan, the delta pre-pass over all rows as one sequence (it clears dQ's accumulator), the main kernel and
 // the conversion of dQ, again over all rows.
 template <int D, bool BF16, bool GEN>
@@ -1533,6 +1571,7 @@ cudaError_t launch_packed(BwdArgs a, const PackedCall& c, int dtype, int device,
   PackedPlan p{};
   p.cu_q = c.cu_q, p.cu_k = c.cu_k, p.n = c.n, p.total_q = a.Lq, p.total_k = c.total_k;
   p.group = a.Hq / a.Hkv, p.causal = a.causal, p.bwd = true, p.step = 1, p.status = a.status;
+  p.kv_heads = a.Hkv, p.slots = c.shares ? packed_slots(c.n, a.Lq, c.total_k, a.Hq, a.Hkv) : 0;
   // (an absent output gets a map that is never used)
   const Str3 accum{0, static_cast<int64_t>(a.Lq) * D, D};
   const void* ptr[kPackedBwdMaps] = {a.q, a.k, a.v, a.d_o, a.dq_accum, a.dk ? a.dk : a.k, a.dv ? a.dv : a.v};
@@ -1550,22 +1589,28 @@ cudaError_t launch_packed(BwdArgs a, const PackedCall& c, int dtype, int device,
   if (a.dv) p.zero[p.n_zero++] = PackedPlan::Rows{static_cast<char*>(a.dv), a.dvs.s * 2, a.dvs.h * 2, a.Hkv, D * 2, true};
   cudaError_t e = launch_packed_plan(p, c.scratch, &a.packed, stream);
   if (e != cudaSuccess) return e;
-  a.parts = 1;
+  a.parts = p.slots, a.dkv_part = c.shares;
   BwdArgs pre = a;
   pre.zero_dq_accum = 1;
   e = launch_bwd_delta(dtype, D, pre, stream);
   if (e != cudaSuccess) return e;
   void (*kern)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, BwdArgs);
-  if constexpr (D == 64) kern = bwd_tc64_kernel<BF16, GEN, false, true>;
-  else kern = bwd_tc_kernel<BF16, GEN, false, true>;
+  if constexpr (D == 64) kern = p.slots > 0 ? bwd_tc64_kernel<BF16, GEN, true, true> : bwd_tc64_kernel<BF16, GEN, false, true>;
+  else kern = p.slots > 0 ? bwd_tc_kernel<BF16, GEN, true, true> : bwd_tc_kernel<BF16, GEN, false, true>;
+  CUtensorMap tdk = p.base[kMapdK], tdv = p.base[kMapdV];  // (whole walks go through their sequence's)
+  if (p.slots > 0 && (!make_map_f32(&tdk, c.shares, D, BM, a.Hkv * p.slots, 1, kOutRows) ||
+                      !make_map_f32(&tdv, c.shares + static_cast<int64_t>(a.Hkv) * p.slots * BM * D, D, BM, a.Hkv * p.slots, 1, kOutRows)))
+    return cudaErrorInvalidValue;
   constexpr int kSmemBytes = D == 64 ? Cfg64::kSmem : Cfg128::kSmem;
   constexpr int kBlock = D == 64 ? Cfg64::kThreads : Cfg128::kThreads;
   e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   if (e != cudaSuccess) return e;
-  const size_t most = packed_items(c.n, a.Skv, 1, 1) * a.Hkv;
+  const size_t most = (packed_items(c.n, a.Skv, 1, 1) + p.slots) * a.Hkv;
   e = launch_early(kern, dim3(static_cast<unsigned>(most < static_cast<size_t>(sms) ? most : sms)), dim3(kBlock), kSmemBytes, stream, 1,
-                   p.base[kMapQ], p.base[kMapK], p.base[kMapV], p.base[kMapdO], p.base[kMapdQ], p.base[kMapdK], p.base[kMapdV], a);
+                   p.base[kMapQ], p.base[kMapK], p.base[kMapV], p.base[kMapdO], p.base[kMapdQ], tdk, tdv, a);
+  if (e == cudaSuccess && p.slots > 0) e = launch_early(packed_sum_kernel<T, D>, dim3(4 * sms), dim3(256), 0, stream, 1, a);
   if (e != cudaSuccess || !a.dq) return e;
+  a.parts = 1;  // (to the conversion: there is dQ only)
   const int64_t total = static_cast<int64_t>(a.Hq) * a.Lq * (D / 8), blocks = (total + 255) / 256;
   return launch_early(dq_convert_kernel<T, D>, dim3(static_cast<unsigned>(blocks < 8 * sms ? blocks : 8 * sms)), dim3(256), 0, stream, 1, a);
 }

@@ -57,11 +57,19 @@ struct MaskArgs {
 struct PackedEntry {
   int q0, lq, k0, lk;  // the sequence's rows of q and of k
   int x;               // forward: its first query block (query tile * group + head of the group); backward: its key tile
-  int seq, walk, reserved;
+  int seq;
+  int from, steps;     // backward: the item's share of the steps of its key tile,
+  int slot;            // and where its dK and dV go, if it is not the whole: a place in the workspace, of a kv head's (else -1)
+  int reserved[3];
+};
+// A key tile whose walk is divided: its first row of k, rows, first slot and how many.
+struct PackedSplit {
+  int row, rows, slot, parts;
 };
 struct PackedArgs {
   const PackedEntry* items;
-  const int* n_items;
+  const int* n_items;  // [0] items, [1] splits
+  const PackedSplit* splits;
   const void* maps;  // CUtensorMap [sequence][kPackedFwdMaps or kPackedBwdMaps]
 };
 enum PackedMap { kMapQ, kMapK, kMapV, kMapO, kPackedFwdMaps, kMapdO = kMapO, kMapdQ, kMapdK, kMapdV, kPackedBwdMaps };

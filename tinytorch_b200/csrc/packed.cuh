@@ -14,9 +14,12 @@ struct PackedPlan {
   // items: of the forward `step` query blocks (128 rows of one head of a group); of the backward a key tile of 128
   bool bwd;
   int step;
-  int shift;            // levels of the sort: key or query tiles of a walk >> shift
+  int width;            // threads to a sequence (a power of two)
+  int shift, levels;    // of the sort: key tiles (backward: steps) of a walk >> shift
+  int kv_heads, slots;  // backward: places for shares of dK / dV, per kv head (0: no walk is divided)
   PackedEntry* items;
-  int* n_items;
+  PackedSplit* splits;
+  int* n_items;         // [0] items, [1] divided key tiles
   int* sched;           // set to zero, or null
   int32_t* status;
   // tensor maps: those of the whole tensors, and which of them go along with k; rows are dimension 1
@@ -43,11 +46,14 @@ struct PackedCall {
   const int32_t* cu_k;
   int n, total_k;
   void* scratch;  // packed_plan_bytes
+  float* shares;  // backward: [dK, dV][Hkv * slots][128][D], or null
 };
 
 // Upper bounds of what a plan takes in scratch memory.
 size_t packed_items(int n, int total, int group, int step);
 size_t packed_plan_bytes(int n, int total_q, int total_k, int group, bool bwd);
+// Backward: the places that shares of divided walks take at most, per kv head.
+int packed_slots(int n, int total_q, int total_k, int Hq, int Hkv);
 
 // Fills in items, maps and args from `scratch` and enqueues the planning kernel.
 cudaError_t launch_packed_plan(PackedPlan p, void* scratch, PackedArgs* args, cudaStream_t stream);

@@ -5,6 +5,10 @@
 // sequence's rows (which may hold infinities), and stores and reductions behind it are dropped, so that nothing in the kernels'
 // loops knows of packing.  CTA 0 sorts the work items, the longest walks first, so that the CTAs of the attention kernel finish
 // together; the other CTAs make the maps, a warp each, and clear the rows behind the last sequence.
+// In the backward a key tile's walk over the queries of its sequence is one item's; with few key tiles for the machine (the host
+// knows that from the rows and heads) walks that are longer than an SM's share of all steps are divided, into items of half a share
+// at most, each of which leaves dK and dV in a slot of the workspace.  Steps, D = 128, 2.9 us: 8192 rows, 8/1 heads 1397 -> 475 us;
+// 4096, 8/2 heads 365 -> 156; divided without need, 2 x 1000 rows of 16 heads take 72 us instead of 50.
 #include "packed.cuh"
 
 #include "ptx.cuh"
@@ -12,16 +16,12 @@
 namespace ttattn {
 namespace {
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32, kLevels = 4096, kTile = 128;
+constexpr int kThreads = 1024, kWarps = kThreads / 32, kLevels = 4096, kTile = 128, kKept = 1024;
+constexpr int kLeastSteps = 4;  // of an item whose walk is divided: below, its dK / dV cost more to add up than the steps take
 
 struct Seq {
   int q0, lq, k0, lk;
 };
-__device__ __forceinline__ Seq load_seq(const PackedPlan& p, int s) {
-  const int q0 = p.cu_q[s], k0 = p.cu_k[s];
-  return Seq{q0, p.cu_q[s + 1] - q0, k0, p.cu_k[s + 1] - k0};
-}
-
 // Items of a sequence, and the tiles that item i walks over.
 __device__ __forceinline__ int items_of(const PackedPlan& p, const Seq& s) {
   if (p.bwd) return (s.lk + kTile - 1) / kTile;
@@ -43,9 +43,19 @@ __device__ __forceinline__ int walk_of(const PackedPlan& p, const Seq& s, int i)
   return (end + kTile - 1) / kTile;
 }
 
+// Items that a key tile's n steps are divided into, and where one of them begins.  `share`: an SM's of all steps.
+__device__ __forceinline__ int parts_of(int n, int share) {
+  const int most = max((share + 1) / 2, kLeastSteps);
+  return n > max(share, most) ? (n + most - 1) / most : 1;
+}
+__device__ __forceinline__ int part_from(int n, int p, int parts) { return static_cast<int>(static_cast<int64_t>(n) * p / parts); }
+
 __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_constant__ PackedPlan p) {
   __shared__ int s_level[kLevels];  // items of a level; then where its next one goes
   __shared__ int s_warp_sum[kWarps];
+  __shared__ int s_cu[2][kKept];    // the offsets, if they are few
+  __shared__ int s_slots, s_splits;
+  __shared__ unsigned long long s_steps;
   __shared__ __align__(128) uint32_t s_map[kWarps][32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   ptx::grid_dep_launch();
@@ -55,8 +65,19 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
   bool falls = false;
   for (int i = tid; i <= p.n; i += kThreads) {
     const int q = p.cu_q[i], k = p.cu_k[i];
-    falls |= q < 0 || q > p.total_q || k < 0 || k > p.total_k;
-    if (i < p.n) falls |= p.cu_q[i + 1] < q || p.cu_k[i + 1] < k;
+    const int qn = i < p.n ? p.cu_q[i + 1] : q, kn = i < p.n ? p.cu_k[i + 1] : k;
+    falls |= q < 0 || q > p.total_q || k < 0 || k > p.total_k || qn < q || kn < k;
+    if (i < kKept) s_cu[0][i] = q, s_cu[1][i] = k;
+  }
+  const bool kept = p.n < kKept;
+  auto load_seq = [&](int i) {
+    const int q0 = kept ? s_cu[0][i] : p.cu_q[i], q1 = kept ? s_cu[0][i + 1] : p.cu_q[i + 1];
+    const int k0 = kept ? s_cu[1][i] : p.cu_k[i], k1 = kept ? s_cu[1][i + 1] : p.cu_k[i + 1];
+    return Seq{q0, q1 - q0, k0, k1 - k0};
+  };
+  if (blockIdx.x == 0) {
+    for (int i = tid; i < p.levels; i += kThreads) s_level[i] = 0;
+    if (tid == 0) s_slots = s_splits = 0, s_steps = 0;
   }
   const bool bad = __syncthreads_or(falls) != 0;
 
@@ -64,7 +85,7 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
     const int64_t first = (static_cast<int64_t>(blockIdx.x) - 1) * kWarps + warp, step = (static_cast<int64_t>(gridDim.x) - 1) * kWarps;
     for (int64_t i = first; i < static_cast<int64_t>(p.n) * p.n_maps && !bad; i += step) {
       const int s = static_cast<int>(i / p.n_maps), m = static_cast<int>(i - static_cast<int64_t>(s) * p.n_maps);
-      const Seq q = load_seq(p, s);
+      const Seq q = load_seq(s);
       const int row = p.of_k[m] ? q.k0 : q.q0, rows = p.of_k[m] ? q.lk : q.lq;
       if (rows <= 0) continue;
       s_map[warp][lane] = reinterpret_cast<const uint32_t*>(&p.base[m])[lane];
@@ -100,27 +121,41 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
   // ------------------------------------------------------------------ the items --
   if (p.sched && tid == 0) *p.sched = 0;
   if (bad) {
-    if (tid == 0) *p.n_items = 0;
+    if (tid == 0) p.n_items[0] = p.n_items[1] = 0;
     if (tid == 0 && p.status) atomicOr(p.status, kStatusBadOffsets);
     return;
   }
-  for (int i = tid; i < kLevels; i += kThreads) s_level[i] = 0;
-  __syncthreads();
-  // With few sequences several warps share one.
-  int per = 1;
-  while (per < kWarps && p.n * per * 2 <= kWarps) per *= 2;
-  const int mine = warp / per, teams = kWarps / per, id = (warp % per) * 32 + lane, width = per * 32;
+  // A thread to a short sequence, up to all of them to a long one.
+  const int width = p.width, mine = tid / width, teams = kThreads / width, id = tid % width;
+  int share = 0x7fffffff;  // no walk is longer
+  if (p.slots > 0) {
+    unsigned long long steps = 0;
+    for (int s = mine; s < p.n; s += teams) {
+      const Seq q = load_seq(s);
+      const int n = items_of(p, q);
+      for (int i = id; i < n; i += width) steps += static_cast<unsigned>(walk_of(p, q, i) * p.group);
+    }
+    atomicAdd(&s_steps, steps);
+    __syncthreads();
+    share = static_cast<int>((s_steps * p.kv_heads + kSms - 1) / kSms);
+  }
   for (int s = mine; s < p.n; s += teams) {
-    const Seq q = load_seq(p, s);
+    const Seq q = load_seq(s);
     const int n = items_of(p, q);
-    for (int i = id; i < n; i += width) atomicAdd(&s_level[walk_of(p, q, i) >> p.shift], 1);
+    for (int i = id; i < n; i += width) {
+      const int steps = p.bwd ? walk_of(p, q, i) * p.group : walk_of(p, q, i), parts = parts_of(steps, share);
+      for (int k = 0; k < parts; ++k) atomicAdd(&s_level[(part_from(steps, k + 1, parts) - part_from(steps, k, parts)) >> p.shift], 1);
+    }
   }
   __syncthreads();
   // places of the levels, the highest first: thread t has four of them
   constexpr int kMine = kLevels / kThreads;
   int count[kMine], sum = 0;
 #pragma unroll
-  for (int i = 0; i < kMine; ++i) count[i] = s_level[kLevels - 1 - (tid * kMine + i)], sum += count[i];
+  for (int i = 0; i < kMine; ++i) {
+    const int level = p.levels - 1 - (tid * kMine + i);
+    count[i] = level >= 0 ? s_level[level] : 0, sum += count[i];
+  }
   int upto = sum;
 #pragma unroll
   for (int of = 1; of < 32; of <<= 1) {
@@ -143,22 +178,35 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
   int place = upto - sum + (warp > 0 ? s_warp_sum[warp - 1] : 0);
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
-    s_level[kLevels - 1 - (tid * kMine + i)] = place;
+    const int level = p.levels - 1 - (tid * kMine + i);
+    if (level >= 0) s_level[level] = place;
     place += count[i];
   }
   __syncthreads();
   for (int s = mine; s < p.n; s += teams) {
-    const Seq q = load_seq(p, s);
+    const Seq q = load_seq(s);
     const int n = items_of(p, q);
     for (int i = id; i < n; i += width) {
-      const int walk = walk_of(p, q, i);
-      const int at = atomicAdd(&s_level[walk >> p.shift], 1);
-      reinterpret_cast<int4*>(p.items + at)[0] = make_int4(q.q0, q.lq, q.k0, q.lk);
-      reinterpret_cast<int4*>(p.items + at)[1] = make_int4(p.bwd ? i : i * p.step, s, walk, 0);
+      const int steps = p.bwd ? walk_of(p, q, i) * p.group : walk_of(p, q, i), parts = parts_of(steps, share);
+      int slot = -1;
+      if (parts > 1) {
+        slot = atomicAdd(&s_slots, parts);
+        p.splits[atomicAdd(&s_splits, 1)] = PackedSplit{q.k0 + i * kTile, min(kTile, q.lk - i * kTile), slot, parts};
+      }
+      for (int k = 0; k < parts; ++k) {
+        const int from = part_from(steps, k, parts), own = part_from(steps, k + 1, parts) - from;
+        int4* e = reinterpret_cast<int4*>(p.items + atomicAdd(&s_level[own >> p.shift], 1));
+        e[0] = make_int4(q.q0, q.lq, q.k0, q.lk);
+        e[1] = make_int4(p.bwd ? i : i * p.step, s, from, own);
+        if (p.bwd) e[2] = make_int4(slot < 0 ? -1 : slot + k, 0, 0, 0);
+      }
     }
   }
+  __syncthreads();
+  if (tid == 0) p.n_items[1] = s_splits;
 }
 
+constexpr int kMostSlots = 4 * kSms;
 constexpr size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
 }  // namespace
@@ -168,23 +216,43 @@ size_t packed_items(int n, int total, int group, int step) {
   return (static_cast<size_t>(total) / kTile + n) * group / step + n + 1;
 }
 
+// (a divided key tile has several: no more than there are slots for)
 static size_t items_bytes(int n, int total_q, int total_k, int group, bool bwd) {
-  return round256(sizeof(PackedEntry) * (bwd ? packed_items(n, total_k, 1, 1) : packed_items(n, total_q, group, 1)));
+  return round256(sizeof(PackedEntry) * (bwd ? packed_items(n, total_k, 1, 1) + kMostSlots : packed_items(n, total_q, group, 1)));
 }
+static size_t splits_bytes(bool bwd) { return bwd ? round256(sizeof(PackedSplit) * kMostSlots) : 0; }
 
 size_t packed_plan_bytes(int n, int total_q, int total_k, int group, bool bwd) {
-  return 256 + items_bytes(n, total_q, total_k, group, bwd) +
+  return 256 + items_bytes(n, total_q, total_k, group, bwd) + splits_bytes(bwd) +
          round256(sizeof(CUtensorMap) * static_cast<size_t>(n) * (bwd ? kPackedBwdMaps : kPackedFwdMaps));
+}
+
+// With t = max(share / 2, kLeastSteps), and W steps of a kv head, a walk of s > t steps is divided into less than s / t + 1 < 2 s / t items: less than
+// 2 W / t in all, which is at most 4 kSms / Hkv (a share is at least W Hkv / kSms) and 2 W / kLeastSteps.
+int packed_slots(int n, int total_q, int total_k, int Hq, int Hkv) {
+  const double tiles = total_k / kTile + n, walk = (total_q / kTile + 1.0) * (Hq / Hkv);  // at most
+  if (tiles * Hkv > 4 * kSms || walk <= kLeastSteps) return 0;
+  const double few = 2 * tiles * walk / kLeastSteps;
+  const int most = (kMostSlots + Hkv - 1) / Hkv;
+  return few < most ? static_cast<int>(few) + 1 : most;
 }
 
 cudaError_t launch_packed_plan(PackedPlan p, void* scratch, PackedArgs* args, cudaStream_t stream) {
   char* at = static_cast<char*>(scratch);
   p.n_items = reinterpret_cast<int*>(at);
   p.items = reinterpret_cast<PackedEntry*>(at + 256);
-  p.maps = reinterpret_cast<CUtensorMap*>(at + 256 + items_bytes(p.n, p.total_q, p.total_k, p.group, p.bwd));
+  p.splits = reinterpret_cast<PackedSplit*>(at + 256 + items_bytes(p.n, p.total_q, p.total_k, p.group, p.bwd));
+  p.maps = reinterpret_cast<CUtensorMap*>(reinterpret_cast<char*>(p.splits) + splits_bytes(p.bwd));
+  // levels 0 ... the longest walk that there can be
+  const int64_t longest = p.bwd ? (static_cast<int64_t>(p.total_q) + kTile - 1) / kTile * p.group : (static_cast<int64_t>(p.total_k) + kTile - 1) / kTile;
   p.shift = 0;
-  while ((((p.bwd ? p.total_q : p.total_k) + kTile - 1) / kTile >> p.shift) >= kLevels) ++p.shift;
-  *args = PackedArgs{p.items, p.n_items, p.maps};
+  while ((longest >> p.shift) >= kLevels) ++p.shift;
+  p.levels = static_cast<int>(longest >> p.shift) + 1;
+  // threads to a sequence: as many as it has items on the average, unless there are more threads than that takes
+  const size_t items = p.bwd ? packed_items(p.n, p.total_k, 1, 1) : packed_items(p.n, p.total_q, p.group, p.step);
+  p.width = 1;
+  while (p.width < kThreads && (static_cast<size_t>(p.width) * p.n < items || 2ll * p.width * p.n <= kThreads)) p.width *= 2;
+  *args = PackedArgs{p.items, p.n_items, p.splits, p.maps};
   const int64_t warps = static_cast<int64_t>(p.n) * p.n_maps + (p.total_q + p.total_k) / 64;
   const int64_t most = 2 * kSms, ctas = (warps + kWarps - 1) / kWarps;
   return launch_early(packed_plan_kernel, dim3(1 + static_cast<unsigned>(ctas < 1 ? 1 : (ctas < most ? ctas : most))), dim3(kThreads), 0, stream, 1, p);

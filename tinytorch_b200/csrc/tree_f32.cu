@@ -278,9 +278,10 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a) {
 constexpr size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 int tile_keys(int dtype, int D) { return dtype == TT_ATTN_F32 ? 4096 / D : 128; }
 // What the end of a walk counts for, in tiles.  16-bit: the exchange between the halves, the next walk's Q and its first scores take 4 to 6 us, in which
-// half of the next tiles arrive (32 sequences of 1000 to 8160 rows, 32 drafts, 32/8 heads, D = 128, us: 0 142, 2 131, 4 126, 6 119, 8 118; 64 of 500 to
-// 4000, 8 drafts: 135, 116, 108, 106, 106).
-int walk_end(int dtype) { return dtype == TT_ATTN_F32 ? 0 : 6; }
+// some of the next tiles arrive; less with few rows.  Measured, us, for 0, 2, 4, 6, 9: 32 sequences of 1000 to 8160 rows, 32 drafts, 32/8 heads,
+// D = 128: 142, 132, 126, 120, 117; 64 of 500 to 4000, 8 drafts (32 rows): 135, 111, 107, 108, 108; 40 of 100 to 2900, 16 drafts, 12/4
+// heads, D = 64 (48 rows): 30.7 with 2, 26.9, 26.5, 28.2.
+int walk_end(int dtype, int rows) { return dtype == TT_ATTN_F32 ? 0 : (rows > 64 ? 8 : 4); }
 constexpr int kLeast = 2;  // tiles of a piece: below that a piece costs more to begin and to put together than it takes
 constexpr int kF32Ctas = 2;  // of an SM
 
@@ -312,7 +313,7 @@ double tree_line(int dtype, int B, int Hq, int Hkv, int T, int capacity, int D) 
   int block, n;
   tree_plan(dtype, Hq, Hkv, T, &block, &n);
   const int keys = tile_keys(dtype, D);
-  return static_cast<double>(B) * Hkv * n * ((capacity + keys - 1) / keys + (T + keys - 1) / keys + walk_end(dtype));
+  return static_cast<double>(B) * Hkv * n * ((capacity + keys - 1) / keys + (T + keys - 1) / keys + walk_end(dtype, block * (Hq / Hkv)));
 }
 
 int tree_ctas(int dtype, int B, int Hq, int Hkv, int T, int capacity, int D) {
@@ -335,7 +336,7 @@ cudaError_t launch_tree_f32(int D, const TreeArgs& a, int ctas, cudaStream_t str
 cudaError_t launch_tree(int dtype, int D, TreeArgs a, void* scratch, int device, cudaStream_t stream) {
   const int ctas = tree_ctas(dtype, a.B, a.Hq, a.Hkv, a.T, a.capacity, D);
   tree_plan(dtype, a.Hq, a.Hkv, a.T, &a.block, &a.n_blocks);
-  a.least = kLeast, a.ends = walk_end(dtype);
+  a.least = kLeast, a.ends = walk_end(dtype, a.block * (a.Hq / a.Hkv));
   a.pieces = static_cast<int4*>(scratch);
   a.partial = reinterpret_cast<float*>(static_cast<char*>(scratch) + round256(ctas * sizeof(int4)));
   cudaError_t e = dtype == TT_ATTN_F32 ? launch_tree_f32(D, a, ctas, stream) : launch_tree_tc(dtype, D, a, ctas, stream);
