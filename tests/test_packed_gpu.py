@@ -288,6 +288,34 @@ def test_streams_and_graphs():
             assert (gr[3][0] - want[0]).abs().max() <= 2 ** -6 * want[0].abs().max()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_plans_that_follow_one_another(D):
+    """Calls right behind one another, whose plans lie in the same scratch memory and differ, each on operands of its own."""
+    from tinytorch_b200 import op
+
+    g = torch.Generator().manual_seed(D)
+    base = [64, 1, 130, 300, 17, 128, 0, 40]
+    cases = []
+    for i in range(30):
+        lens = [base[j] for j in torch.randperm(len(base), generator=g)]
+        cases.append([make(sum(lens), h, D, torch.bfloat16, 10 * i + h) for h in (8, 2, 2)] + [offsets(lens)])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = [op.sdpAttentionPackedFwd(*c, True) for c in cases]
+        grads = [op.sdpAttentionPackedBwd(c[0], *c[:3], *f, c[3], True) for c, f in zip(cases, got)]
+    side.synchronize()
+    for c, f, b in zip(cases, got, grads):
+        one = op.sdpAttentionPackedFwd(*c, True)
+        torch.cuda.synchronize()
+        assert torch.equal(f[0], one[0]) and torch.equal(f[1], one[1])
+        back = op.sdpAttentionPackedBwd(c[0], *c[:3], *one, c[3], True)
+        torch.cuda.synchronize()
+        # (dq is summed in any order)
+        assert torch.equal(b[1], back[1]) and torch.equal(b[2], back[2])
+        assert (b[0].float() - back[0].float()).abs().max() <= 2 ** -7 * back[0].float().abs().max()
+
+
 def test_offsets_changed_between_the_passes_are_an_error():
     from tinytorch_b200 import function
     q, k, v = (make(64, h, 64, torch.bfloat16, h).requires_grad_() for h in (4, 2, 2))

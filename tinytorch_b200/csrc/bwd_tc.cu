@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
   int n_items = n_kt * n_heads * (EVEN ? a.parts : 1);
   const int n_q_all = (a.Lq + BQ - 1) / BQ;
   auto read_plan = [&]() {
-    n_kt = *a.packed.n_items, n_items = n_kt * n_heads;
+    n_kt = __ldcg(a.packed.n_items), n_items = n_kt * n_heads;
     const int want = n_kt > 0 ? (2 * static_cast<int>(gridDim.x) + n_kt - 1) / n_kt : 0;
     tail_heads = want < n_heads ? want : n_heads;
   };
@@ -283,11 +283,11 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
     const int nt0 = nt;
     if constexpr (PACKED) {
       const int4* e = reinterpret_cast<const int4*>(a.packed.items + nt);
-      const int4 rows = __ldg(e), place = __ldg(e + 1);
+      const int4 rows = __ldcg(e), place = __ldcg(e + 1);
       it.q0 = rows.x, it.lq = Lq = rows.y, it.k0 = rows.z, it.lk = kv_len = rows.w;
       nt = place.x, it.seq = place.y;
       it.n_q = n_q_tiles = (Lq + BQ - 1) / BQ;
-      if (PARTS) from = place.z, steps = place.w, it.part = __ldg(&a.packed.items[nt0].slot);
+      if (PARTS) from = place.z, steps = place.w, it.part = __ldcg(&a.packed.items[nt0].slot);
     }
     it.kv0 = nt * BM;
     if (!PACKED && a.kv_lens) {
@@ -876,7 +876,7 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
   int n_items = n_kt * n_heads * (EVEN ? a.parts : 1);
   const int n_q_all = (a.Lq + BQ - 1) / BQ;
   auto read_plan = [&]() {
-    n_kt = *a.packed.n_items, n_items = n_kt * n_heads;
+    n_kt = __ldcg(a.packed.n_items), n_items = n_kt * n_heads;
     const int want = n_kt > 0 ? (2 * static_cast<int>(gridDim.x) + n_kt - 1) / n_kt : 0;
     tail_heads = want < n_heads ? want : n_heads;
   };
@@ -900,11 +900,11 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
     const int nt0 = nt;
     if constexpr (PACKED) {
       const int4* e = reinterpret_cast<const int4*>(a.packed.items + nt);
-      const int4 rows = __ldg(e), place = __ldg(e + 1);
+      const int4 rows = __ldcg(e), place = __ldcg(e + 1);
       it.q0 = rows.x, it.lq = Lq = rows.y, it.k0 = rows.z, it.lk = kv_len = rows.w;
       nt = place.x, it.seq = place.y;
       it.n_q = n_q_tiles = (Lq + BQ - 1) / BQ;
-      if (PARTS) from = place.z, steps = place.w, it.part = __ldg(&a.packed.items[nt0].slot);
+      if (PARTS) from = place.z, steps = place.w, it.part = __ldcg(&a.packed.items[nt0].slot);
     }
     it.kv0 = nt * BM;
     if (!PACKED && a.kv_lens) {
@@ -1537,7 +1537,7 @@ cudaError_t launch_t(const BwdArgs& a, int dtype, int device, cudaStream_t strea
 template <typename T, int D>
 __global__ void __launch_bounds__(256) packed_sum_kernel(const BwdArgs a) {
   ptx::grid_dep_wait();
-  const int n = a.packed.n_items[1];
+  const int n = __ldcg(a.packed.n_items + 1);
   const int64_t per_split = 2ll * a.Hkv * BM * (D / 8), step = static_cast<int64_t>(gridDim.x) * blockDim.x;
   const int64_t shares = static_cast<int64_t>(a.Hkv) * a.parts * BM * D;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n * per_split; i += step) {
@@ -1578,13 +1578,11 @@ cudaError_t launch_packed(BwdArgs a, const PackedCall& c, int dtype, int device,
   const Str3* st[kPackedBwdMaps] = {&a.qs, &a.ks, &a.vs, &a.dos, &accum, a.dk ? &a.dks : &a.ks, a.dv ? &a.dvs : &a.vs};
   for (int m = 0; m < kPackedBwdMaps; ++m) {
     const bool of_k = m == kMapK || m == kMapV || m == kMapdK || m == kMapdV;
-    const bool made = m == kMapdQ ? make_map_f32(&p.base[m], a.dq_accum, D, a.Lq, a.Hq, 1, D == 64 ? 32 : 128)
-                                  : make_map(&p.base[m], dtype, ptr[m], D, of_k ? a.Skv : a.Lq, of_k ? a.Hkv : a.Hq, 1, *st[m],
-                                             m == kMapdK || m == kMapdV ? kOutRows : 128);
+    const bool made = m == kMapdQ ? packed_map(&p, TT_ATTN_F32, a.dq_accum, D, a.Lq, a.Hq, accum, D == 64 ? 32 : 128, false)
+                                  : packed_map(&p, dtype, ptr[m], D, of_k ? a.Skv : a.Lq, of_k ? a.Hkv : a.Hq, *st[m],
+                                               m == kMapdK || m == kMapdV ? kOutRows : 128, of_k);
     if (!made) return cudaErrorInvalidValue;
-    p.of_k[m] = of_k, p.address[m] = static_cast<const char*>(ptr[m]), p.row_bytes[m] = st[m]->s * (m == kMapdQ ? 4 : 2);
   }
-  p.n_maps = kPackedBwdMaps;
   if (a.dk) p.zero[p.n_zero++] = PackedPlan::Rows{static_cast<char*>(a.dk), a.dks.s * 2, a.dks.h * 2, a.Hkv, D * 2, true};
   if (a.dv) p.zero[p.n_zero++] = PackedPlan::Rows{static_cast<char*>(a.dv), a.dvs.s * 2, a.dvs.h * 2, a.Hkv, D * 2, true};
   cudaError_t e = launch_packed_plan(p, c.scratch, &a.packed, stream);

@@ -128,7 +128,7 @@ __device__ __forceinline__ Item decode_item(const FwdArgs& a, int w, int per_hea
   int kv_len = a.Skv, Lq = a.Lq, first = KEYS ? mp : mp * QT;
   if constexpr (PACKED) {
     const int4* e = reinterpret_cast<const int4*>(a.packed.items + (per_head - 1 - mp));
-    const int4 rows = __ldg(e), place = __ldg(e + 1);
+    const int4 rows = __ldcg(e), place = __ldcg(e + 1);  // (the plan runs while this kernel is coming up)
     it.q0 = rows.x, it.lq = Lq = rows.y, kv_len = rows.w, first = place.x, it.seq = place.y;
   } else if (a.kv_lens) {
     int l = a.kv_lens[it.b];
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         uint32_t g = 0;             // K/V tiles requested so far (ring position)
         uint32_t qc0 = 0, qc1 = 0;  // items whose Q tile 0 / 1 was requested so far
-        if (PACKED) per_head = *a.packed.n_items;
+        if (PACKED) per_head = __ldcg(a.packed.n_items);
         const int n_items = per_head * a.Hkv * a.B;
         for (uint32_t i = 0;; ++i) {
           // the first item is the CTA's own number; the counter, where one is needed, hands out the rest
@@ -1154,11 +1154,9 @@ cudaError_t launch_packed(FwdArgs a, const PackedCall& c, int dtype, int device,
   const void* ptr[kPackedFwdMaps] = {a.q, a.k, a.v, a.o};
   const Str3* st[kPackedFwdMaps] = {&a.qs, &a.ks, &a.vs, &a.os};
   for (int m = 0; m < kPackedFwdMaps; ++m) {
-    p.of_k[m] = m == kMapK || m == kMapV;
-    if (!make_map(&p.base[m], dtype, ptr[m], D, p.of_k[m] ? a.Skv : a.Lq, p.of_k[m] ? a.Hkv : a.Hq, 1, *st[m])) return cudaErrorInvalidValue;
-    p.address[m] = static_cast<const char*>(ptr[m]), p.row_bytes[m] = st[m]->s * 2;
+    const bool of_k = m == kMapK || m == kMapV;
+    if (!packed_map(&p, dtype, ptr[m], D, of_k ? a.Skv : a.Lq, of_k ? a.Hkv : a.Hq, *st[m], 128, of_k)) return cudaErrorInvalidValue;
   }
-  p.n_maps = kPackedFwdMaps;
   p.zero[0] = PackedPlan::Rows{static_cast<char*>(a.o), a.os.s * 2, a.os.h * 2, a.Hq, D * 2, false};
   p.n_zero = 1, p.lse = a.lse;
   cudaError_t e = launch_packed_plan(p, c.scratch, &a.packed, stream);

@@ -22,8 +22,10 @@ struct PackedPlan {
   int* n_items;         // [0] items, [1] divided key tiles
   int* sched;           // set to zero, or null
   int32_t* status;
-  // tensor maps: those of the whole tensors, and which of them go along with k; rows are dimension 1
-  CUtensorMap base[kPackedBwdMaps];
+  // tensor maps (see packed_map): those of the whole tensors, those of one row, and from how many rows on a sequence takes the former;
+  // which of them go along with k; rows are dimension 1
+  CUtensorMap base[kPackedBwdMaps], small[kPackedBwdMaps];
+  int long_rows[kPackedBwdMaps];
   const char* address[kPackedBwdMaps];
   int64_t row_bytes[kPackedBwdMaps];
   bool of_k[kPackedBwdMaps];
@@ -54,6 +56,9 @@ size_t packed_items(int n, int total, int group, int step);
 size_t packed_plan_bytes(int n, int total_q, int total_k, int group, bool bwd);
 // Backward: the places that shares of divided walks take at most, per kv head.
 int packed_slots(int n, int total_q, int total_k, int Hq, int Hkv);
+
+// Adds the map of an operand [rows][H][D] (fp32: dense [H][rows][D]).
+bool packed_map(PackedPlan* p, int dtype, const void* ptr, int D, int rows, int H, const Str3& st, int box_rows, bool of_k);
 
 // Fills in items, maps and args from `scratch` and enqueues the planning kernel.
 cudaError_t launch_packed_plan(PackedPlan p, void* scratch, PackedArgs* args, cudaStream_t stream);

@@ -5,6 +5,10 @@
 // sequence's rows (which may hold infinities), and stores and reductions behind it are dropped, so that nothing in the kernels'
 // loops knows of packing.  CTA 0 sorts the work items, the longest walks first, so that the CTAs of the attention kernel finish
 // together; the other CTAs make the maps, a warp each, and clear the rows behind the last sequence.
+// A copy keeps what the driver has put into a map besides its base and extents, and that depends on how far the tensor reaches: 128
+// KB or more, or less.  A short sequence with the map of a long tensor gets the right rows and zeros behind them, but the hardware
+// also touches addresses behind its last row, which faults where nothing is mapped there (a tensor at the end of an
+// allocator's segment).  So each map comes as two, for short and for long sequences, both made by the driver.
 // In the backward a key tile's walk over the queries of its sequence is one item's; with few key tiles for the machine (the host
 // knows that from the rows and heads) walks that are longer than an SM's share of all steps are divided, into items of half a share
 // at most, each of which leaves dK and dV in a slot of the workspace.  Steps, D = 128, 2.9 us: 8192 rows, 8/1 heads 1397 -> 475 us;
@@ -12,6 +16,7 @@
 #include "packed.cuh"
 
 #include "ptx.cuh"
+#include "tma_host.cuh"
 
 namespace ttattn {
 namespace {
@@ -45,7 +50,7 @@ __device__ __forceinline__ int walk_of(const PackedPlan& p, const Seq& s, int i)
 
 // Items that a key tile's n steps are divided into, and where one of them begins.  `share`: an SM's of all steps.
 __device__ __forceinline__ int parts_of(int n, int share) {
-  const int most = max((share + 1) / 2, kLeastSteps);
+  const int most = max(share / 2 + share % 2, kLeastSteps);
   return n > max(share, most) ? (n + most - 1) / most : 1;
 }
 __device__ __forceinline__ int part_from(int n, int p, int parts) { return static_cast<int>(static_cast<int64_t>(n) * p / parts); }
@@ -64,15 +69,15 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
   // Offsets that fall, or lie outside the rows, would let sequences share rows: then there are no items, and every row is cleared.
   bool falls = false;
   for (int i = tid; i <= p.n; i += kThreads) {
-    const int q = p.cu_q[i], k = p.cu_k[i];
-    const int qn = i < p.n ? p.cu_q[i + 1] : q, kn = i < p.n ? p.cu_k[i + 1] : k;
+    const int q = __ldcg(p.cu_q + i), k = __ldcg(p.cu_k + i);
+    const int qn = i < p.n ? __ldcg(p.cu_q + i + 1) : q, kn = i < p.n ? __ldcg(p.cu_k + i + 1) : k;
     falls |= q < 0 || q > p.total_q || k < 0 || k > p.total_k || qn < q || kn < k;
     if (i < kKept) s_cu[0][i] = q, s_cu[1][i] = k;
   }
   const bool kept = p.n < kKept;
   auto load_seq = [&](int i) {
-    const int q0 = kept ? s_cu[0][i] : p.cu_q[i], q1 = kept ? s_cu[0][i + 1] : p.cu_q[i + 1];
-    const int k0 = kept ? s_cu[1][i] : p.cu_k[i], k1 = kept ? s_cu[1][i + 1] : p.cu_k[i + 1];
+    const int q0 = kept ? s_cu[0][i] : __ldcg(p.cu_q + i), q1 = kept ? s_cu[0][i + 1] : __ldcg(p.cu_q + i + 1);
+    const int k0 = kept ? s_cu[1][i] : __ldcg(p.cu_k + i), k1 = kept ? s_cu[1][i + 1] : __ldcg(p.cu_k + i + 1);
     return Seq{q0, q1 - q0, k0, k1 - k0};
   };
   if (blockIdx.x == 0) {
@@ -88,7 +93,7 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
       const Seq q = load_seq(s);
       const int row = p.of_k[m] ? q.k0 : q.q0, rows = p.of_k[m] ? q.lk : q.lq;
       if (rows <= 0) continue;
-      s_map[warp][lane] = reinterpret_cast<const uint32_t*>(&p.base[m])[lane];
+      s_map[warp][lane] = reinterpret_cast<const uint32_t*>(rows < p.long_rows[m] ? &p.small[m] : &p.base[m])[lane];
       __syncwarp();
       if (lane == 0) {
         const uint32_t at = ptx::smem_u32(s_map[warp]);
@@ -104,7 +109,7 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
       const PackedPlan::Rows& r = p.zero[z];
       const int total = r.of_k ? p.total_k : p.total_q;
       const int32_t* cu = r.of_k ? p.cu_k : p.cu_q;
-      const int head = bad ? 0 : cu[0], tail = bad ? 0 : cu[p.n];
+      const int head = bad ? 0 : __ldcg(cu), tail = bad ? 0 : __ldcg(cu + p.n);
       const int64_t n = static_cast<int64_t>(head + total - tail) * r.heads;
       for (int64_t i = first; i < n; i += step) {
         int row = static_cast<int>(i / r.heads);
@@ -210,6 +215,47 @@ constexpr int kMostSlots = 4 * kSms;
 constexpr size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
 }  // namespace
+
+namespace {
+
+// Whether two maps of the same memory differ in nothing but the number of rows (which lies in one of their words).
+bool same_kind(const CUtensorMap& a, const CUtensorMap& b) {
+  int differ = 0;
+  for (size_t i = 0; i < sizeof(a.opaque) / sizeof(a.opaque[0]); ++i) differ += a.opaque[i] != b.opaque[i];
+  return differ <= 1;
+}
+
+}  // namespace
+
+bool packed_map(PackedPlan* p, int dtype, const void* ptr, int D, int rows, int H, const Str3& st, int box_rows, bool of_k) {
+  const int m = p->n_maps++;
+  const int64_t es = dtype == TT_ATTN_F32 ? 4 : 2;
+  auto encode = [&](CUtensorMap* map, int n) {
+    return dtype == TT_ATTN_F32 ? make_map_f32(map, static_cast<const float*>(ptr), D, rows, H, 1, box_rows, n) : make_map(map, dtype, ptr, D, n, H, 1, st, box_rows);
+  };
+  p->address[m] = static_cast<const char*>(ptr), p->row_bytes[m] = st.s * es, p->of_k[m] = of_k;
+  if (!encode(&p->base[m], rows) || !encode(&p->small[m], 1)) return false;
+  if (same_kind(p->base[m], p->small[m])) {
+    p->long_rows[m] = 1;
+    return true;
+  }
+  // The fewest rows that count as long: those that reach over 128 KB; should a driver see it otherwise, they are searched for.
+  const int64_t first = static_cast<int64_t>(H - 1) * st.h * es + D * es, more = (int64_t(128) << 10) - first;
+  int64_t n = 1 + (more > 0 ? (more + st.s * es - 1) / (st.s * es) : 0);
+  CUtensorMap at, below;
+  if (n < 2 || n > rows || !encode(&at, static_cast<int>(n)) || !encode(&below, static_cast<int>(n - 1)) || !same_kind(at, p->base[m]) ||
+      same_kind(below, p->base[m])) {
+    int64_t lo = 1, hi = rows;
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) / 2;
+      if (!encode(&at, static_cast<int>(mid))) return false;
+      (same_kind(at, p->base[m]) ? hi : lo) = mid;
+    }
+    n = hi;
+  }
+  p->long_rows[m] = static_cast<int>(n);
+  return true;
+}
 
 // Every sequence has at most one item more than its rows fill.
 size_t packed_items(int n, int total, int group, int step) {
