@@ -264,7 +264,7 @@ __device__ __forceinline__ void stream(const NormRopeArgs& a, const Smem<T, D, T
     if (!rotated || token >= a.B * a.S) return;
     const int b = token / a.S;
 #pragma unroll
-    for (int e = 0; e < kMaxAxes; ++e) pos[e] = e < a.axes ? __ldg(a.positions + e * a.pos_axis + b * a.pos_b + (token - b * a.S)) : 0;
+    for (int e = 0; e < kMaxAxes; ++e) pos[e] = e < a.axes ? a.positions[e * a.pos_axis + b * a.pos_b + (token - b * a.S)] : 0;
   };
   Walk ahead(first, per_token), now = ahead;
   const T *x0, *x1;
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas) norm_rope_kernel(const 
   int pos[kMaxAxes];
   if (a.cos && c0 < c1) {
 #pragma unroll
-    for (int e = 0; e < kMaxAxes; ++e) pos[e] = e < a.axes ? __ldg(a.positions + e * a.pos_axis + b * a.pos_b + row) : 0;
+    for (int e = 0; e < kMaxAxes; ++e) pos[e] = e < a.axes ? a.positions[e * a.pos_axis + b * a.pos_b + row] : 0;
   }
   const T* x = reinterpret_cast<const T*>(a.x[t]) + b * a.xs[t].b + row * a.xs[t].s;
   const int64_t xh = a.xs[t].h, yh = a.ys[t].h;

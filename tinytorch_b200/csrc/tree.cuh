@@ -173,7 +173,7 @@ __device__ __forceinline__ void tree_mask_row(const TreeArgs& a, int b, int t, u
 #pragma unroll
   for (int i = 0; i < WORDS * 2 + 1; ++i) {
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (i < n_vec) v = __ldg(p + i);
+    if (i < n_vec) v = p[i];
     const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
