@@ -1570,7 +1570,7 @@ cudaError_t launch_packed(BwdArgs a, const PackedCall& c, int dtype, int device,
   const int sms = sm_count(device);
   PackedPlan p{};
   p.cu_q = c.cu_q, p.cu_k = c.cu_k, p.n = c.n, p.total_q = a.Lq, p.total_k = c.total_k;
-  p.group = a.Hq / a.Hkv, p.causal = a.causal, p.bwd = true, p.step = 1, p.status = a.status;
+  p.group = a.Hq / a.Hkv, p.causal = a.causal, p.bwd = true, p.status = a.status;
   p.kv_heads = a.Hkv, p.slots = c.shares ? packed_slots(c.n, a.Lq, c.total_k, a.Hq, a.Hkv) : 0;
   // (an absent output gets a map that is never used)
   const Str3 accum{0, static_cast<int64_t>(a.Lq) * D, D};

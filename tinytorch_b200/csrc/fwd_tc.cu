@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const CUtensorMap *mq = &tmQ, *mk = &tmK, *mv = &tmV;
           if constexpr (PACKED) {
             mq = map_of(it.seq, kMapQ), mk = map_of(it.seq, kMapK), mv = map_of(it.seq, kMapV);
-            ptx::tensormap_acquire(mq), ptx::tensormap_acquire(mk), ptx::tensormap_acquire(mv);
+            ptx::tensormap_acquire(mq), ptx::tensormap_acquire(mk);  // (V's when Q and K are on their way)
           }
           bool ok = true;
           // a Q tile is loaded only if it has key tiles to walk; tile 0 goes first and, with the first K tile,
@@ -469,6 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               return true;
             };
             ok = load(sK, mk, ctl->k_full, ctl->k_empty, 0);
+            if (PACKED) ptx::tensormap_acquire(mv);
             for (int j = 0; j < n && ok; ++j) {
               if (j + 1 < n) ok = load(sK, mk, ctl->k_full, ctl->k_empty, j + 1);
               if (ok) ok = load(sV, mv, ctl->v_full, ctl->v_empty, j);
@@ -485,6 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int hf = 0; hf < HALVES; ++hf)
                 ptx::tma_load_4d(sK + st * TB + hf * HALF_BYTES, mk, &ctl->k_full[st], hf * 64, (it.j0 + j) * BN, it.hk, it.b);
               if (j == 0 && !(ok = load_q(1, qc1))) break;
+              if (PACKED && j == 0) ptx::tensormap_acquire(mv);
               if (!(ok = ptx::mbar_wait(&ctl->v_empty[st], ph ^ 1, abort_flag))) break;
               ptx::mbar_arrive_expect_tx(&ctl->v_full[st], TB);
 #pragma unroll
@@ -1150,7 +1152,7 @@ cudaError_t launch_packed(FwdArgs a, const PackedCall& c, int dtype, int device,
   const bool keys = est <= 2.0 * sms && c.total_k >= 256ll * c.n;
   PackedPlan p{};
   p.cu_q = c.cu_q, p.cu_k = c.cu_k, p.n = c.n, p.total_q = a.Lq, p.total_k = c.total_k;
-  p.group = group, p.causal = a.causal, p.step = keys ? 1 : QT, p.sched = a.sched, p.status = a.status;
+  p.group = group, p.causal = a.causal, p.step_log = keys ? 0 : 1, p.sched = a.sched, p.status = a.status;
   const void* ptr[kPackedFwdMaps] = {a.q, a.k, a.v, a.o};
   const Str3* st[kPackedFwdMaps] = {&a.qs, &a.ks, &a.vs, &a.os};
   for (int m = 0; m < kPackedFwdMaps; ++m) {

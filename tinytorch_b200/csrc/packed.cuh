@@ -11,10 +11,11 @@ struct PackedPlan {
   const int32_t* cu_k;
   int n, total_q, total_k;
   int group, causal;
-  // items: of the forward `step` query blocks (128 rows of one head of a group); of the backward a key tile of 128
+  uint64_t per_group;   // ceil(2^40 / group)
+  // items: of the forward 1 << step_log query blocks (128 rows of one head of a group); of the backward a key tile of 128
   bool bwd;
-  int step;
-  int width;            // threads to a sequence (a power of two)
+  int step_log;
+  int width_log;        // threads to a sequence
   int shift, levels;    // of the sort: key tiles (backward: steps) of a walk >> shift
   int kv_heads, slots;  // backward: places for shares of dK / dV, per kv head (0: no walk is divided)
   PackedEntry* items;

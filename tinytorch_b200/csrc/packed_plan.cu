@@ -21,16 +21,18 @@
 namespace ttattn {
 namespace {
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32, kLevels = 4096, kTile = 128, kKept = 1024;
+constexpr int kTile = 128, kKept = 1024, kMine = 4;  // (levels of a thread)
 constexpr int kLeastSteps = 4;  // of an item whose walk is divided: below, its dK / dV cost more to add up than the steps take
 
 struct Seq {
   int q0, lq, k0, lk;
 };
+// x / group, exact up to 2^40 / group: a division by a variable takes as long as the rest of an item's plan
+__device__ __forceinline__ int by_group(const PackedPlan& p, int x) { return static_cast<int>(static_cast<uint64_t>(x) * p.per_group >> 40); }
 // Items of a sequence, and the tiles that item i walks over.
 __device__ __forceinline__ int items_of(const PackedPlan& p, const Seq& s) {
   if (p.bwd) return (s.lk + kTile - 1) / kTile;
-  return ((s.lq + kTile - 1) / kTile * p.group + p.step - 1) / p.step;
+  return ((s.lq + kTile - 1) / kTile * p.group + (1 << p.step_log) - 1) >> p.step_log;
 }
 __device__ __forceinline__ int walk_of(const PackedPlan& p, const Seq& s, int i) {  // (query tiles of one head; key tiles of the longer of a pair)
   const int shift = causal_shift(p.causal, s.lk, s.lq);
@@ -39,7 +41,7 @@ __device__ __forceinline__ int walk_of(const PackedPlan& p, const Seq& s, int i)
     const int from = p.causal && first > 0 ? first / kTile : 0;
     return from < nq ? nq - from : 0;
   }
-  const int nq = (s.lq + kTile - 1) / kTile, last = (i * p.step + p.step - 1) / p.group;
+  const int nq = (s.lq + kTile - 1) / kTile, last = by_group(p, ((i + 1) << p.step_log) - 1);
   int end = s.lk;
   if (p.causal) {
     const int seen = ((last < nq ? last : nq - 1) + 1) * kTile + shift;
@@ -53,9 +55,11 @@ __device__ __forceinline__ int parts_of(int n, int share) {
   const int most = max(share / 2 + share % 2, kLeastSteps);
   return n > max(share, most) ? (n + most - 1) / most : 1;
 }
-__device__ __forceinline__ int part_from(int n, int p, int parts) { return static_cast<int>(static_cast<int64_t>(n) * p / parts); }
+__device__ __forceinline__ int part_from(int n, int p, int parts) { return parts == 1 ? n * p : static_cast<int>(static_cast<int64_t>(n) * p / parts); }
 
+template <int kThreads>
 __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_constant__ PackedPlan p) {
+  constexpr int kWarps = kThreads / 32, kLevels = kMine * kThreads;
   __shared__ int s_level[kLevels];  // items of a level; then where its next one goes
   __shared__ int s_warp_sum[kWarps];
   __shared__ int s_cu[2][kKept];    // the offsets, if they are few
@@ -87,9 +91,9 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
   const bool bad = __syncthreads_or(falls) != 0;
 
   if (blockIdx.x > 0) {
-    const int64_t first = (static_cast<int64_t>(blockIdx.x) - 1) * kWarps + warp, step = (static_cast<int64_t>(gridDim.x) - 1) * kWarps;
-    for (int64_t i = first; i < static_cast<int64_t>(p.n) * p.n_maps && !bad; i += step) {
-      const int s = static_cast<int>(i / p.n_maps), m = static_cast<int>(i - static_cast<int64_t>(s) * p.n_maps);
+    const unsigned first = (blockIdx.x - 1) * kWarps + warp, step = (gridDim.x - 1) * kWarps;
+    for (unsigned i = first; i < static_cast<unsigned>(p.n) * p.n_maps && !bad; i += step) {
+      const int s = p.bwd ? i / kPackedBwdMaps : i / kPackedFwdMaps, m = i - s * p.n_maps;
       const Seq q = load_seq(s);
       const int row = p.of_k[m] ? q.k0 : q.q0, rows = p.of_k[m] ? q.lk : q.lq;
       if (rows <= 0) continue;
@@ -131,7 +135,7 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
     return;
   }
   // A thread to a short sequence, up to all of them to a long one.
-  const int width = p.width, mine = tid / width, teams = kThreads / width, id = tid % width;
+  const int width = 1 << p.width_log, mine = tid >> p.width_log, teams = kThreads >> p.width_log, id = tid & (width - 1);
   int share = 0x7fffffff;  // no walk is longer
   if (p.slots > 0) {
     unsigned long long steps = 0;
@@ -154,7 +158,6 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
   }
   __syncthreads();
   // places of the levels, the highest first: thread t has four of them
-  constexpr int kMine = kLevels / kThreads;
   int count[kMine], sum = 0;
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
@@ -170,13 +173,13 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
   if (lane == 31) s_warp_sum[warp] = upto;
   __syncthreads();
   if (warp == 0) {
-    int w = s_warp_sum[lane];
+    int w = lane < kWarps ? s_warp_sum[lane] : 0;
 #pragma unroll
     for (int of = 1; of < 32; of <<= 1) {
       const int o = __shfl_up_sync(0xffffffffu, w, of);
       if (lane >= of) w += o;
     }
-    s_warp_sum[lane] = w;
+    if (lane < kWarps) s_warp_sum[lane] = w;
     if (lane == 31) *p.n_items = w;
   }
   __syncthreads();
@@ -202,7 +205,7 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
         const int from = part_from(steps, k, parts), own = part_from(steps, k + 1, parts) - from;
         int4* e = reinterpret_cast<int4*>(p.items + atomicAdd(&s_level[own >> p.shift], 1));
         e[0] = make_int4(q.q0, q.lq, q.k0, q.lk);
-        e[1] = make_int4(p.bwd ? i : i * p.step, s, from, own);
+        e[1] = make_int4(p.bwd ? i : i << p.step_log, s, from, own);
         if (p.bwd) e[2] = make_int4(slot < 0 ? -1 : slot + k, 0, 0, 0);
       }
     }
@@ -289,19 +292,24 @@ cudaError_t launch_packed_plan(PackedPlan p, void* scratch, PackedArgs* args, cu
   p.items = reinterpret_cast<PackedEntry*>(at + 256);
   p.splits = reinterpret_cast<PackedSplit*>(at + 256 + items_bytes(p.n, p.total_q, p.total_k, p.group, p.bwd));
   p.maps = reinterpret_cast<CUtensorMap*>(reinterpret_cast<char*>(p.splits) + splits_bytes(p.bwd));
+  p.per_group = ((uint64_t(1) << 40) + p.group - 1) / p.group;
+  // A large CTA sorts many items quickly, but each of its barriers takes longer: 677 rows of 5 sequences, 32/8 heads, 26 items: the plan
+  // 2.6 us with 256 threads.
+  const size_t items = p.bwd ? packed_items(p.n, p.total_k, 1, 1) : packed_items(p.n, p.total_q, p.group, 1 << p.step_log);
+  const int threads = items <= 512 && p.n <= 256 ? 256 : 1024, warps = threads / 32;
   // levels 0 ... the longest walk that there can be
   const int64_t longest = p.bwd ? (static_cast<int64_t>(p.total_q) + kTile - 1) / kTile * p.group : (static_cast<int64_t>(p.total_k) + kTile - 1) / kTile;
   p.shift = 0;
-  while ((longest >> p.shift) >= kLevels) ++p.shift;
+  while ((longest >> p.shift) >= kMine * threads) ++p.shift;
   p.levels = static_cast<int>(longest >> p.shift) + 1;
   // threads to a sequence: as many as it has items on the average, unless there are more threads than that takes
-  const size_t items = p.bwd ? packed_items(p.n, p.total_k, 1, 1) : packed_items(p.n, p.total_q, p.group, p.step);
-  p.width = 1;
-  while (p.width < kThreads && (static_cast<size_t>(p.width) * p.n < items || 2ll * p.width * p.n <= kThreads)) p.width *= 2;
+  p.width_log = 0;
+  for (int width = 1; width < threads && (static_cast<size_t>(width) * p.n < items || 2ll * width * p.n <= threads); width *= 2) ++p.width_log;
   *args = PackedArgs{p.items, p.n_items, p.splits, p.maps};
-  const int64_t warps = static_cast<int64_t>(p.n) * p.n_maps + (p.total_q + p.total_k) / 64;
-  const int64_t most = 2 * kSms, ctas = (warps + kWarps - 1) / kWarps;
-  return launch_early(packed_plan_kernel, dim3(1 + static_cast<unsigned>(ctas < 1 ? 1 : (ctas < most ? ctas : most))), dim3(kThreads), 0, stream, 1, p);
+  const int64_t maps = static_cast<int64_t>(p.n) * p.n_maps + (p.total_q + p.total_k) / 64;  // a warp each, and one to 64 rows, which may have to be cleared
+  const int64_t most = 2 * kSms * (1024 / threads), ctas = (maps + warps - 1) / warps;
+  const dim3 grid(1 + static_cast<unsigned>(ctas < 1 ? 1 : (ctas < most ? ctas : most)));
+  return threads == 256 ? launch_early(packed_plan_kernel<256>, grid, dim3(256), 0, stream, 1, p) : launch_early(packed_plan_kernel<1024>, grid, dim3(1024), 0, stream, 1, p);
 }
 
 }  // namespace ttattn
