@@ -36,6 +36,8 @@
 // steps of an item run one after the other; D = 64 (bwd_tc64_kernel) overlaps the two
 // element-wise phases of a step with the MMAs of the neighbouring phases and gives the
 // read-out of results to a warpgroup of its own.
+// PACKED: sequences behind one another, with items and tensor maps from packed_plan.cu.  6 documents of 255 to 3000 rows, 32/8 heads, D = 128, bf16: 470 us in
+// all (700 TFLOP/s, as unpacked); 8 of 517 to 3096, 16 heads, D = 64, fp16: 205 us.
 #include <type_traits>
 
 #include "common.cuh"

@@ -3,7 +3,8 @@
 // fp32 has no tensor-core product of its own precision, so products are FMAs from shared memory: a CTA, one of two on an SM, holds a block of
 // R = 8 or 32 rows and walks over tiles of 4096 / D keys (cp.async, a tile or two ahead, on into the next walk).  With 8 rows a tile's arithmetic is
 // less than the time its keys take to arrive, with 32 rows, whose loads from shared memory set the pace, about twice that; more rows are more
-// blocks, which find the keys in L2.
+// blocks, which find the keys in L2.  4 sequences of 500 to 1003 rows, 5 drafts, 16 heads, D = 64: 19.5 us, of which the keys' bytes take 4: each CTA's few tiles
+// follow one another (with one CTA to an SM 20.7).
 #include <type_traits>
 
 #include "ptx.cuh"

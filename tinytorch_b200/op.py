@@ -1,7 +1,8 @@
-"""Operator layer: the three attention ops a TinyTorch build registers in its
+"""Operator layer: the attention ops a TinyTorch build registers in its
 dispatch tables (reference mechanism: DEFINE_OP / REGISTER_OP_IMPL,
-src/Tensor/Dispatch.h:21-142), here bound to torch tensors used purely as
-device-memory handles.  Every op goes through the C ABI of libtt_attn.so and
+src/Tensor/Dispatch.h:21-142), and those of a language model around them (packed
+sequences, trees of drafted tokens, accepted drafts), here bound to torch tensors
+used purely as device-memory handles.  Every op goes through the C ABI of libtt_attn.so and
 launches on the current CUDA stream of the tensors' device, as reference ops do
 (src/Utils/CUDAUtils.cpp:123-135).  No op has a CPU implementation.
 
