@@ -211,3 +211,23 @@ def test_python_function_has_the_same_results():
     b = fused.FuncQkNormRope.apply(q, k, *w, cos, sin, pos, 1e-6, False, (12, 20), None)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
     assert all(torch.equal(x, y) for x, y in zip(torch.autograd.grad(a, (q, k, *w), gs), torch.autograd.grad(b, (q, k, *w), gs)))
+
+
+@pytest.mark.parametrize("dt,D", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 128)])
+def test_operands_that_end_where_their_memory_does(dt, D):
+    from tinytorch_b200 import fused, op
+
+    g = torch.Generator(device="cuda").manual_seed(D)
+    q, k, gq, gk, wq, wk = (torch.randn(*s, generator=g, device="cuda").to(dt) for s in ((37, 5, D), (37, 2, D), (37, 5, D), (37, 2, D), (D,), (D,)))
+    cos, sin = op.ropeTables(100, D)
+    pos = torch.arange(37, dtype=torch.int32, device="cuda") + 63  # the last row of the tables among them
+
+    def run(q, k, wq, wk, cos, sin, pos, gq, gk):
+        leaves = [x.detach().requires_grad_() for x in (q, k, wq, wk)]
+        out = fused.qkNormRope(*leaves, cos, sin, pos)
+        return [*out, *torch.autograd.grad(out, leaves, (gq, gk))]
+
+    want = run(q, k, wq, wk, cos, sin, pos, gq, gk)
+    got = run(*(ref.at_the_end(x) for x in (q, k, wq, wk, cos, sin, pos, gq, gk)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -316,6 +316,24 @@ def test_plans_that_follow_one_another(D):
         assert (b[0].float() - back[0].float()).abs().max() <= 2 ** -7 * back[0].float().abs().max()
 
 
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 8, 2), (128, 8, 1), (64, 3, 3)])
+def test_operands_that_end_where_their_memory_does(D, Hq, Hkv):
+    from tinytorch_b200 import op
+
+    lens = (200, 1, 900, 40)
+    q, k, v, g = (make(sum(lens), h, D, torch.bfloat16, h) for h in (Hq, Hkv, Hkv, Hq))
+    want = op.sdpAttentionPackedFwd(q, k, v, offsets(lens), True)
+    qe, ke, ve, ge = (ref.at_the_end(x) for x in (q, k, v, g))
+    cu = ref.at_the_end(offsets(lens))
+    got = op.sdpAttentionPackedFwd(qe, ke, ve, cu, True)
+    oe, le = ref.at_the_end(got[0]), ref.at_the_end(got[1]).contiguous()
+    grads = op.sdpAttentionPackedBwd(ge, qe, ke, ve, oe, le, cu, True)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    back = op.sdpAttentionPackedBwd(g, q, k, v, *want, offsets(lens), True)
+    assert torch.equal(grads[1], back[1]) and torch.equal(grads[2], back[2])
+
+
 def test_offsets_changed_between_the_passes_are_an_error():
     from tinytorch_b200 import function
     q, k, v = (make(64, h, 64, torch.bfloat16, h).requires_grad_() for h in (4, 2, 2))

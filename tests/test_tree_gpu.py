@@ -319,3 +319,21 @@ def test_a_layer_trains_and_serves():
         a, c = out[b, :, path].transpose(0, 1).double(), longer[at + n:at + n + 3].double()
         assert (a - c).abs().max() <= 4 * 2.0 ** -8 * v2[at:at + n + 3].abs().max().item()
         at += n + 3
+
+
+@pytest.mark.parametrize("dt,D", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)])
+def test_operands_that_end_where_their_memory_does(dt, D):
+    from tinytorch_b200 import op
+
+    g = torch.Generator(device="cuda").manual_seed(D)
+    q, kd, vd, kc, vc = (torch.randn(2, h, n, D, generator=g, device="cuda").to(dt) for h, n in ((6, 5), (2, 5), (2, 5), (2, 301), (2, 301)))
+    lens = torch.tensor([301, 77], dtype=torch.int32, device="cuda")
+    mask = (torch.rand(2, 5, 5, generator=g, device="cuda") < 0.6) | torch.eye(5, dtype=torch.bool, device="cuda")
+    path, counts = torch.tensor([[0, 2], [1, 4]], dtype=torch.int32, device="cuda"), torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+    want = op.sdpAttentionTree(q, kd, vd, kc, vc, lens, mask, needLse=True)
+    e = [ref.at_the_end(x) for x in (q, kd, vd, kc, vc, lens, mask, path, counts)]
+    got = op.sdpAttentionTree(*e[:7], needLse=True)
+    new = op.cacheAccept(*e[1:6], *e[7:])
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert new.tolist() == [301, 79] and torch.equal(e[3][1, :, 77:79], kd[1][:, [1, 4]])

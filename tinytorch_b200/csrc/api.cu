@@ -607,9 +607,10 @@ int tt_attn_packed_bwd(const tt_attn_packed_bwd_params* p) {
   a.dqs = packed_strides(p->dq_strides, p->Hq, p->total_q, p->D);
   a.dks = packed_strides(p->dk_strides, p->Hkv, p->total_k, p->D);
   a.dvs = packed_strides(p->dv_strides, p->Hkv, p->total_k, p->D);
-  const void* ptrs[] = {p->q, p->k, p->v, p->o, p->d_o, p->dq, p->dk, p->dv, p->lse};
+  const void* ptrs[] = {p->q, p->k, p->v, p->o, p->d_o, p->dq, p->dk, p->dv};
   for (const void* q : ptrs)
     if (!aligned16(q)) return TT_ATTN_ERR_ALIGN;
+  if (reinterpret_cast<uintptr_t>(p->lse) % 4) return TT_ATTN_ERR_ALIGN;
   const Str3* sts[] = {&a.qs, &a.ks, &a.vs, &a.os, &a.dos, &a.dqs, &a.dks, &a.dvs};
   for (const Str3* s : sts)
     if (!strides_ok(*s, es)) return TT_ATTN_ERR_ALIGN;
