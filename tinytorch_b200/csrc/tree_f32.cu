@@ -3,8 +3,8 @@
 // fp32 has no tensor-core product of its own precision, so products are FMAs from shared memory: a CTA, one of two on an SM, holds a block of
 // R = 8 or 32 rows and walks over tiles of 4096 / D keys (cp.async, a tile or two ahead, on into the next walk).  With 8 rows a tile's arithmetic is
 // less than the time its keys take to arrive, with 32 rows, whose loads from shared memory set the pace, about twice that; more rows are more
-// blocks, which find the keys in L2.  4 sequences of 500 to 1003 rows, 5 drafts, 16 heads, D = 64: 19.5 us, of which the keys' bytes take 4: each CTA's few tiles
-// follow one another (with one CTA to an SM 20.7).
+// blocks, which find the keys in L2.  4 sequences of 500 to 1003 rows, 5 drafts, 16 heads, D = 64: 17.3 us, of which the keys' bytes take 4: each CTA's few tiles
+// follow one another (with one CTA to an SM 1.2 more).
 #include <type_traits>
 
 #include "ptx.cuh"
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_f32_kernel(const TreeArgs a)
 }
 
 // The walk that begins in piece blockIdx.x and goes on, if there is one: its partial results in the order of the pieces.  A thread has
-// four channels of a row; neighbouring threads neighbouring rows.
+// four channels of a row; neighbouring threads neighbouring rows.  (Only rows that a block has get threads: 5 rows of D = 64 by 296 CTAs, not 2368.)
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a) {
   ptx::grid_dep_launch();
@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a) {
   const int4 w = a.pieces[blockIdx.x];
   if (w.x < 2) return;
   const int group = a.Hq / a.Hkv, draft0 = w.w * a.block, drafts = a.T - draft0 < a.block ? a.T - draft0 : a.block;
-  const int at = blockIdx.y * 256 + threadIdx.x, c4 = at / kTreeRows, r = at % kTreeRows;
-  if (r >= drafts * group) return;
+  const int rows = a.block * group, at = blockIdx.y * 256 + threadIdx.x, c4 = at / rows, r = at - c4 * rows;
+  if (c4 >= D / 4 || r >= drafts * group) return;
   // the walk's first piece is the last of its CTA, the others the first of theirs
   const float* part = a.partial + static_cast<size_t>(blockIdx.x) * 2 * tree_partial_floats(D);
   auto piece = [&](int i) { return part + (i == 0 ? 1 : 2 * i) * tree_partial_floats(D); };
@@ -296,7 +296,7 @@ cudaError_t launch_r(const TreeArgs& a, int ctas, cudaStream_t stream) {
 
 template <typename T>
 cudaError_t launch_combine(int D, const TreeArgs& a, int ctas, cudaStream_t stream) {
-  const dim3 grid(ctas, kTreeRows * (D / 4) / 256);
+  const dim3 grid(ctas, (a.block * (a.Hq / a.Hkv) * (D / 4) + 255) / 256);
   return D == 64 ? launch_early(tree_combine_kernel<T, 64>, grid, dim3(256), 0, stream, 1, a)
                  : launch_early(tree_combine_kernel<T, 128>, grid, dim3(256), 0, stream, 1, a);
 }

@@ -16,7 +16,7 @@
 // for the others): a tile's exponentials then are the work of all four warps of a warpgroup, on all four of an SM's
 // special-function units, instead of one warp's.  The copies are added up through shared memory at the end of a segment.
 // Measured, us: 32 sequences of 1000 to 8160 rows, 32 drafts, 32/8 heads, D = 128, bf16: 117 with the combine kernel (the scan alone 5.7 TB/s; one walk a CTA,
-// as it came: 150); one of 2000 rows, 8 drafts: 13.7 (before the copies of few rows: 15.6); 16 of 16 drafts, D = 64: 54 (77).
+// as it came: 150); one of 2000 rows, 8 drafts: 12.4 (before the copies of few rows 2 more); 16 of 16 drafts, D = 64: 52 (77).
 // Every mbarrier wait is bounded.
 #include <cuda.h>
 
