@@ -231,3 +231,29 @@ def test_operands_that_end_where_their_memory_does(dt, D):
     got = run(*(ref.at_the_end(x) for x in (q, k, wq, wk, cos, sin, pos, gq, gk)))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_rows_far_away():
+    """More than 2^31 elements: the last rows are those of a call of their own."""
+    from tinytorch_b200 import fused, op
+
+    T, D = 540_000, 128
+    q, k = torch.zeros(T, 32, D, dtype=torch.bfloat16, device="cuda"), torch.zeros(T, 2, D, dtype=torch.bfloat16, device="cuda")
+    assert q.numel() > 2 ** 31
+    q[-9:], k[-9:] = randn((9, 32, D), torch.bfloat16, 1), randn((9, 2, D), torch.bfloat16, 2)
+    w = randn((D,), torch.bfloat16, 3)
+    cos, sin = op.ropeTables(64, D)
+    pos = positions((T,), 64, 4)
+
+    def run(q, k, pos):
+        leaves = [q.detach().requires_grad_(), k.detach().requires_grad_(), w.clone().requires_grad_(), w.clone().requires_grad_()]
+        out = fused.qkNormRope(*leaves, cos, sin, pos)
+        return [x.detach() for x in out], torch.autograd.grad(out, leaves, (q.detach(), k.detach()))
+
+    out, grads = run(q, k, pos)
+    want, back = run(q[-9:].clone(), k[-9:].clone(), pos[-9:])
+    assert all(torch.equal(x[-9:], y) for x, y in zip(out + list(grads[:2]), want + list(back[:2])))
+    # (the other rows' outputs and their gradients are zeros: so are their shares of the weights' gradients)
+    assert not out[0][:-9].any() and not grads[0][:-9].any()
+    for x, y in zip(grads[2:], back[2:]):
+        assert (x.float() - y.float()).abs().max() <= 2 ** -7 * y.float().abs().max()

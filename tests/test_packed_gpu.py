@@ -334,6 +334,50 @@ def test_operands_that_end_where_their_memory_does(D, Hq, Hkv):
     assert torch.equal(grads[1], back[1]) and torch.equal(grads[2], back[2])
 
 
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 2, 1), (128, 3, 3)])
+def test_thousands_of_sequences(D, Hq, Hkv):
+    """More than the plan keeps in shared memory: each of 0 to 3 rows, and a long one among them."""
+    lens = [(7 * i) % 4 for i in range(2500)]
+    lens[1700] = 400
+    q, k, v, g = (make(sum(lens) + 5, h, D, torch.float16, 3 + h) for h in (Hq, Hkv, Hkv, Hq))
+    from tinytorch_b200 import op
+    o, lse = op.sdpAttentionPackedFwd(q, k, v, offsets(lens), True)
+    grads = op.sdpAttentionPackedBwd(g, q, k, v, o, lse, offsets(lens), True)
+    # the first 40, those around the long one, the last 40, each part a call of its own
+    at = [0] + list(offsets(lens).tolist())[1:]
+    for a, b in ((0, 40), (1690, 1712), (2460, 2500)):
+        rows = slice(at[a], at[b])
+        part = [x[rows] for x in (q, k, v)]
+        po, pl = op.sdpAttentionPackedFwd(*part, offsets(lens[a:b]), True)
+        back = op.sdpAttentionPackedBwd(g[rows], *part, po, pl, offsets(lens[a:b]), True)
+        check((po, pl, *back), *part, lens[a:b], True, g=g[rows])
+        assert torch.equal(o[rows], po) and torch.equal(lse[:, rows], pl)
+        for x, y in zip(grads, back):
+            assert (x[rows].float() - y.float()).abs().max() <= 2 ** -9 * y.float().abs().max()
+    assert not o[at[-1]:].any() and not any(x[at[-1]:].any() for x in grads)
+
+
+def test_rows_far_away():
+    """Elements of q, o and dq beyond 2^31, bytes of the sum for dq beyond 2^32."""
+    from tinytorch_b200 import op
+
+    total, Hq, Hkv, D, n = 540_000, 32, 1, 128, 300
+    q = torch.zeros(total, Hq, D, dtype=torch.bfloat16, device="cuda")
+    k, v = (torch.zeros(total, Hkv, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    assert q.numel() > 2 ** 31
+    for i, x in enumerate((q, k, v)):
+        x[-n:] = make(n, x.shape[1], D, torch.bfloat16, i)
+    cu = torch.tensor([total - n, total - 100, total], dtype=torch.int32, device="cuda")
+    o, lse = op.sdpAttentionPackedFwd(q, k, v, cu, True)
+    part = [x[-n:].clone() for x in (q, k, v)]
+    po, pl = op.sdpAttentionPackedFwd(*part, cu - (total - n), True)
+    assert torch.equal(o[-n:], po) and torch.equal(lse[:, -n:], pl) and not o[:-n].any()
+    grads = op.sdpAttentionPackedBwd(q, q, k, v, o, lse, cu, True)
+    back = op.sdpAttentionPackedBwd(part[0], *part, po, pl, cu - (total - n), True)
+    for x, y in zip(grads, back):
+        assert (x[-n:].float() - y.float()).abs().max() <= 2 ** -6 * y.float().abs().max() and not x[:-n].any()
+
+
 def test_offsets_changed_between_the_passes_are_an_error():
     from tinytorch_b200 import function
     q, k, v = (make(64, h, 64, torch.bfloat16, h).requires_grad_() for h in (4, 2, 2))
