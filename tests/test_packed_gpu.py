@@ -378,6 +378,42 @@ def test_rows_far_away():
         assert (x[-n:].float() - y.float()).abs().max() <= 2 ** -6 * y.float().abs().max() and not x[:-n].any()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("most", [32, 64])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 2), (4, 2), (6, 2), (16, 2), (14, 2), (6, 1), (3, 3)])
+def test_short_sequences(D, Hq, Hkv, most):
+    """Sequences of up to 32 or 64 rows, whose heads share tiles where they share keys, a longer one among them; lengths of the keys of their own."""
+    from tinytorch_b200 import op
+
+    lens, lens_k = ((1, 32, 0, 17, 31, 2, 33, 5, 32, 8, 20, 1), (32, 1, 4, 17, 0, 32, 33, 40, 9, 8, 31, 1))
+    if most == 64:
+        lens, lens_k = (64, 33, 0, 50, 63, 2, 65, 40, 64, 40, 1, 40), (64, 1, 9, 64, 0, 2, 70, 33, 80, 200, 1, 63)
+    for causal, keys in ((True, None), (False, None), ("bottom-right", lens_k), (True, lens_k)):
+        m, tail = sum(keys or lens), 0 if keys else 3
+        q, k, v = (make(n + tail, h, D, torch.bfloat16, 5 + h) for n, h in ((sum(lens), Hq), (m, Hkv), (m, Hkv)))
+        cu_k = None if keys is None else offsets(keys)
+        o, lse = op.sdpAttentionPackedFwd(q, k, v, offsets(lens), causal, cuSeqlensK=cu_k)
+        g = make(sum(lens) + tail, Hq, D, torch.bfloat16, 9)
+        grads = op.sdpAttentionPackedBwd(g, q, k, v, o, lse, offsets(lens), causal, cuSeqlensK=cu_k)
+        check((o, lse, *grads), q, k, v, lens, causal, lens_k=keys, g=g)
+
+
+@pytest.mark.parametrize("poison", [math.inf, math.nan])
+def test_short_sequences_keep_to_themselves(poison):
+    """An infinite value of one sequence, or of one kv head, is in no other's results."""
+    from tinytorch_b200 import op
+
+    lens, Hq, Hkv, D = (20, 9, 32, 16), 8, 2, 64
+    q, k, v = (make(sum(lens), h, D, torch.bfloat16, h) for h in (Hq, Hkv, Hkv))
+    want = op.sdpAttentionPackedFwd(q, k, v, offsets(lens), True)
+    v[22, 1], k[23, 1] = poison, poison
+    got = op.sdpAttentionPackedFwd(q, k, v, offsets(lens), True)
+    keep = torch.ones(sum(lens), Hq, dtype=torch.bool, device="cuda")
+    keep[20:29, 4:] = False
+    assert torch.equal(got[0][keep], want[0][keep]) and torch.equal(got[1].t()[keep], want[1].t()[keep])
+    assert not got[0][22:29, 4:].isfinite().all()
+
+
 def test_offsets_changed_between_the_passes_are_an_error():
     from tinytorch_b200 import function
     q, k, v = (make(64, h, 64, torch.bfloat16, h).requires_grad_() for h in (4, 2, 2))

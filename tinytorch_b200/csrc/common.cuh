@@ -68,9 +68,10 @@ struct PackedSplit {
 };
 struct PackedArgs {
   const PackedEntry* items;
-  const int* n_items;  // [0] items, [1] splits
+  const int* n_items;  // [0] items, [1] splits, [2] narrow items, which follow the others
   const PackedSplit* splits;
   const void* maps;  // CUtensorMap [sequence][kPackedFwdMaps or kPackedBwdMaps]
+  int heads, blocks;  // forward, narrow items (of short sequences): query heads of a block, blocks of a kv head
 };
 enum PackedMap { kMapQ, kMapK, kMapV, kMapO, kPackedFwdMaps, kMapdO = kMapO, kMapdQ, kMapdK, kMapdV, kPackedBwdMaps };
 

@@ -75,6 +75,7 @@ struct Item {
   int n_max;                   // the longer walk; -1: no more items
   int mask;                    // whether the mask has to be looked at
   int q0, lq, seq;             // packed: the sequence, its first row of q and how many
+  int narrow;                  // packed: the blocks are NARROW rows of several heads
 };
 
 struct __align__(16) SmemCtl {
@@ -103,8 +104,8 @@ constexpr int smem_bytes() {
 // GEN: 1: the variant for a causal triangle that is not top-left aligned, 2: that and a mask; the fast variant (0) compiles
 // all of that out.
 // KEYS: `per_head` items (query blocks) per (batch, kv head), `rank` of `cluster` shares of the key tiles; else pairs.
-// PACKED: a head's items are those of all sequences, as the plan has sorted them.
-template <int GEN, bool KEYS, bool PACKED>
+// PACKED: a head's items are those of all sequences, as the plan has sorted them; NARROW: behind them those of sequences of up to so many rows.
+template <int GEN, bool KEYS, bool PACKED, int NARROW>
 __device__ __forceinline__ Item decode_item(const FwdArgs& a, int w, int per_head, int rank = 0, int cluster = 1) {
   Item it;
   // Heads in order, the longest (latest causal) pair of a head first: the CTAs running at any moment share few
@@ -113,6 +114,21 @@ __device__ __forceinline__ Item decode_item(const FwdArgs& a, int w, int per_hea
   // CTAs finish together (in head order the last head's longest pair, an eighth of a CTA's whole share of
   // 128 heads of 4096 rows, would be drawn when most CTAs are nearly done).  Those heads' K/V together fit L2.
   const int n_heads = a.B * a.Hkv, group = a.Hq / a.Hkv;
+  if constexpr (NARROW > 0) {
+    if (w >= per_head * n_heads) {
+      const PackedArgs& p = a.packed;
+      const int y = w - per_head * n_heads, at = y / n_heads;
+      const int4* e = reinterpret_cast<const int4*>(p.items + per_head + at);
+      const int4 rows = __ldcg(e), place = __ldcg(e + 1);
+      it.narrow = 1, it.b = 0, it.hk = y - at * n_heads, it.row0[0] = it.row0[1] = 0, it.j0 = 0, it.n_max = 1, it.mask = 0;
+      it.q0 = rows.x, it.lq = rows.y, it.kv_len = rows.w, it.seq = place.y;
+      it.shift = GEN ? causal_shift(a.causal, it.kv_len, it.lq) : 0;
+      it.h[0] = it.hk * group + place.x * p.heads, it.h[1] = it.h[0] + p.heads;
+      it.nt[0] = 1, it.nt[1] = place.x + 1 < p.blocks;
+      return it;
+    }
+  }
+  it.narrow = 0;
   int tail_heads = (kTailWaves * static_cast<int>(gridDim.x) + per_head - 1) / per_head;
   if (tail_heads > n_heads) tail_heads = n_heads;
   const int w0 = (n_heads - tail_heads) * per_head;
@@ -333,7 +349,7 @@ __device__ __forceinline__ void combine_rows(const FwdArgs& a, const Item& it, i
   }
 }
 
-template <int D, bool BF16, int GEN, bool KEYS, bool PACKED>
+template <int D, bool BF16, int GEN, bool KEYS, bool PACKED, int NARROW>
 __global__ void __launch_bounds__(kThreads, 1)
     fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
@@ -356,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int per_head = KEYS ? n_blocks : (n_blocks + QT - 1) / QT;  // (packed: the producer asks the plan)
   const int rank = KEYS && !PACKED && cluster > 1 ? static_cast<int>(ptx::cluster_rank()) : 0;
   auto item_of = [&](int w) {
-    return KEYS ? decode_item<GEN, true, PACKED>(a, w, per_head, rank, cluster) : decode_item<GEN, false, PACKED>(a, w, per_head);
+    return decode_item<GEN, KEYS, PACKED, NARROW>(a, w, per_head, rank, cluster);
   };
   // packed: the maps of an item's sequence, which the plan has made, instead of those of the whole tensors
   auto map_of = [&](int seq, int which) { return static_cast<const CUtensorMap*>(a.packed.maps) + seq * static_cast<int64_t>(kPackedFwdMaps) + which; };
@@ -419,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t g = 0;             // K/V tiles requested so far (ring position)
         uint32_t qc0 = 0, qc1 = 0;  // items whose Q tile 0 / 1 was requested so far
         if (PACKED) per_head = __ldcg(a.packed.n_items);
-        const int n_items = per_head * a.Hkv * a.B;
+        const int n_items = per_head * a.Hkv * a.B + (NARROW ? __ldcg(a.packed.n_items + 2) * a.Hkv : 0);
         for (uint32_t i = 0;; ++i) {
           // the first item is the CTA's own number; the counter, where one is needed, hands out the rest
           int w;
@@ -442,13 +458,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             mq = map_of(it.seq, kMapQ), mk = map_of(it.seq, kMapK), mv = map_of(it.seq, kMapV);
             ptx::tensormap_acquire(mq), ptx::tensormap_acquire(mk);  // (V's when Q and K are on their way)
           }
+          const uint32_t q_bytes = NARROW && it.narrow ? a.packed.heads * NARROW * D * 2 : TB, kv_bytes = NARROW && it.narrow ? NARROW * D * 2 : TB;
           bool ok = true;
           // a Q tile is loaded only if it has key tiles to walk; tile 0 goes first and, with the first K tile,
           // ahead of tile 1: the issuer starts tile 0 of this item while tile 1 of the previous one still works
           auto load_q = [&](int t, uint32_t& qc) {
             if ((t == 0 ? it.nt[0] : it.nt[1]) == 0) return true;
             if (!ptx::mbar_wait(&ctl->q_empty[t], (qc & 1) ^ 1, abort_flag)) return false;
-            ptx::mbar_arrive_expect_tx(&ctl->q_full[t], TB);
+            ptx::mbar_arrive_expect_tx(&ctl->q_full[t], q_bytes);
 #pragma unroll
             for (int hf = 0; hf < HALVES; ++hf)
               ptx::tma_load_4d(sQ + t * TB + hf * HALF_BYTES, mq, &ctl->q_full[t], hf * 64,
@@ -483,14 +500,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int st = g % NSTAGE;
               const uint32_t ph = (g / NSTAGE) & 1;
               if (!(ok = ptx::mbar_wait(&ctl->k_empty[st], ph ^ 1, abort_flag))) break;
-              ptx::mbar_arrive_expect_tx(&ctl->k_full[st], TB);
+              ptx::mbar_arrive_expect_tx(&ctl->k_full[st], kv_bytes);
 #pragma unroll
               for (int hf = 0; hf < HALVES; ++hf)
                 ptx::tma_load_4d(sK + st * TB + hf * HALF_BYTES, mk, &ctl->k_full[st], hf * 64, (it.j0 + j) * BN, it.hk, it.b);
               if (j == 0 && !(ok = load_q(1, qc1))) break;
               if (PACKED && j == 0) ptx::tensormap_acquire(mv);
               if (!(ok = ptx::mbar_wait(&ctl->v_empty[st], ph ^ 1, abort_flag))) break;
-              ptx::mbar_arrive_expect_tx(&ctl->v_full[st], TB);
+              ptx::mbar_arrive_expect_tx(&ctl->v_full[st], kv_bytes);
 #pragma unroll
               for (int hf = 0; hf < HALVES; ++hf)
                 ptx::tma_load_4d(sV + st * TB + hf * HALF_BYTES, mv, &ctl->v_full[st], hf * 64, (it.j0 + j) * BN, it.hk, it.b);
@@ -541,13 +558,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (leader) ptx::mma_commit(&ctl->s_full[t]);
         };
+        int pv_keys = BN / 16;  // k-steps of a product P V: what lies behind a narrow block's keys is of an earlier tile
         auto issue_pv = [&](int t, uint32_t g, bool first) {
           const uint32_t b0 = vlo + (g % NSTAGE) * (TB >> 4), d = tmem + 256 + t * D, a0 = tmem + t * 128;
 #pragma unroll
           for (int ks = 0; ks < BN / 16; ++ks) {
             // V is N(=D)-contiguous: 16 keys per k-step = 2048 bytes; the two
             // 64-wide column blocks of D=128 are HALF_BYTES apart (LBO).
-            if (leader) ptx::mma_ts2(d, a0 + ks * 8, b0 + ks * (2048 >> 4), kHi, idesc_pv, (!first || ks > 0) ? 1u : 0u);
+            if (leader && (!NARROW || ks < pv_keys)) ptx::mma_ts2(d, a0 + ks * 8, b0 + ks * (2048 >> 4), kHi, idesc_pv, (!first || ks > 0) ? 1u : 0u);
           }
         };
 
@@ -570,6 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int slot = i & 1;
           if (!uwait(&ctl->item_full[slot], (i >> 1) & 1)) break;
           const int nt0 = ctl->item[slot].nt[0], nt1 = ctl->item[slot].nt[1], n_max = ctl->item[slot].n_max;
+          if constexpr (NARROW > 0) pv_keys = ctl->item[slot].narrow ? NARROW / 16 : BN / 16;
           __syncwarp();  // every lane has read the slot before it is handed back
           if (leader) ptx::mbar_arrive(&ctl->item_empty[slot]);
           if (n_max < 0) break;
@@ -703,20 +722,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int b = pub->b, kv_len = pub->kv_len, shift = pub->shift, j0 = pub->j0, n_max = pub->n_max;
       const int n_t = pub->nt[t], tile_row0 = pub->row0[t], head = pub->h[t];
       const int q0 = PACKED ? pub->q0 : 0, lq = PACKED ? pub->lq : a.Lq;
+      const bool narrow = NARROW && pub->narrow;
       const CUtensorMap* mo = &tmO;
       if constexpr (PACKED) mo = map_of(pub->seq, kMapO);
       const bool use_mask = GEN == 2 && pub->mask;
       if (!KEYS) ptx::mbar_arrive(&ctl->item_empty[slot]);  // (KEYS: read again after the walk, and then handed back)
       if (n_max < 0) break;
-      const int row = tile_row0 + r_in;  // query row of this thread
+      constexpr int kRows = NARROW > 0 ? NARROW : BM;
+      const int row = tile_row0 + (narrow ? r_in % kRows : r_in);  // query row of this thread
+      const int head_in = narrow ? r_in / kRows : 0;               // its head is `head` + this
+      const bool has = !narrow || head_in < a.packed.heads;
       T* orow = reinterpret_cast<T*>(a.o) + b * a.os.b + head * a.os.h + static_cast<int64_t>(q0 + row) * a.os.s;
-      float* lse_row = a.lse ? a.lse + (static_cast<int64_t>(b) * a.Hq + head) * a.Lq + q0 + row : nullptr;
+      float* lse_row = a.lse ? a.lse + (static_cast<int64_t>(b) * a.Hq + head + head_in) * a.Lq + q0 + row : nullptr;
       if (PACKED && n_max > 0 && r_in == 0) ptx::tensormap_acquire(mo);
 
       if (KEYS ? cluster == 1 && n_max == 0 : n_t == 0) {
         if (KEYS) ptx::mbar_arrive(&ctl->item_empty[slot]);
         // no participating key (or tile beyond Lq): O = 0, LSE = -inf
-        if (row < lq && (!KEYS || t == 0)) {
+        if (row < lq && (!KEYS || t == 0) && !narrow) {
 #pragma unroll
           for (int e = 0; e < D; e += 8) *reinterpret_cast<uint4*>(orow + e) = make_uint4(0, 0, 0, 0);
           if (lse_row) *lse_row = -INFINITY;
@@ -752,7 +775,44 @@ __global__ void __launch_bounds__(kThreads, 1)
 
       float m_ref = -INFINITY;  // reference max, in scaled log2 units
       float2 l2 = make_float2(0.f, 0.f);
-      for (int j = 0; j < n_t && ok; ++j) {
+      if constexpr (NARROW > 0) {
+        if (narrow) {
+          // One tile, of which only the first NARROW columns are keys.
+          ok = ptx::mbar_wait(&ctl->s_full[t], cnt & 1, abort_flag);
+          ptx::tc_fence_after();
+          if (ok && has) {
+#pragma unroll
+            for (int cc = 0; cc < NARROW / 32; ++cc) ptx::tmem_ld32p(tS + cc * 32, s + cc * 32);
+            ptx::tmem_wait_ld();
+            int lim = kv_len - 1;
+            if (a.causal && row + shift < lim) lim = row + shift;
+            float mx[8];
+#pragma unroll
+            for (int e = 0; e < NARROW; ++e) {
+              const float x = e > lim ? -INFINITY : __uint_as_float(s[e]);
+              s[e] = __float_as_uint(x);
+              mx[e % 8] = e < 8 ? x : fmaxf(mx[e % 8], x);
+            }
+            m_ref = ptx::max3(ptx::max3(mx[0], mx[1], mx[2]), ptx::max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * c;
+            const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+            const float2 nm2 = make_float2(-m_use, -m_use);
+            uint32_t pk[NARROW / 2];
+#pragma unroll
+            for (int e = 0; e < NARROW; e += 2) {
+              const float2 x = ptx::fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, nm2);
+              const float2 p = make_float2(ptx::ex2(x.x), ptx::ex2(x.y));
+              l2 = ptx::add2(l2, p);
+              pk[e / 2] = pack2<BF16>(p.x, p.y);
+            }
+            if constexpr (NARROW == 32) ptx::tmem_st16(tS, pk);
+            else ptx::tmem_st32(tS, pk);
+            ptx::tmem_wait_st();
+          }
+          ptx::tc_fence_before();
+          ptx::mbar_arrive(&ctl->p_full[t]);
+        }
+      }
+      for (int j = 0; j < n_t && ok && !narrow; ++j) {
         ok = ptx::mbar_wait(&ctl->s_full[t], (cnt + j) & 1, abort_flag);
         if (!ok) break;
         ptx::tc_fence_after();
@@ -989,7 +1049,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ptx::bulk_commit();
         }
       }
-      if (ok && row < lq && lse_row) *lse_row = l > 0.f ? (m_ref + log2f(l)) * kLn2 : -INFINITY;
+      if (ok && row < lq && has && lse_row) *lse_row = l > 0.f ? (m_ref + log2f(l)) * kLn2 : -INFINITY;
     }
     if (r_in == 0) ptx::bulk_wait_all();
   }
@@ -1021,13 +1081,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------ host ----
-template <int D, bool BF16, int GEN, bool KEYS, bool PACKED = false>
+template <int D, bool BF16, int GEN, bool KEYS, bool PACKED = false, int NARROW = 0>
 cudaError_t launch_k(const FwdArgs& a, int dtype, int grid, int cluster, cudaStream_t stream) {
   CUtensorMap tq, tk, tv, to;
   if (!make_map(&tq, dtype, a.q, D, a.Lq, a.Hq, a.B, a.qs) || !make_map(&tk, dtype, a.k, D, a.Skv, a.Hkv, a.B, a.ks) ||
       !make_map(&tv, dtype, a.v, D, a.Skv, a.Hkv, a.B, a.vs) || !make_map(&to, dtype, a.o, D, a.Lq, a.Hq, a.B, a.os))
     return cudaErrorInvalidValue;
-  auto kern = fwd_tc_kernel<D, BF16, GEN, KEYS, PACKED>;
+  auto kern = fwd_tc_kernel<D, BF16, GEN, KEYS, PACKED, NARROW>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D, GEN>());
   if (e != cudaSuccess) return e;
   return launch_early(kern, dim3(grid), dim3(kThreads), smem_bytes<D, GEN>(), stream, cluster, tq, tk, tv, to, a, cluster);
@@ -1042,7 +1102,7 @@ int cluster_slots(int device, int cluster) {
   std::atomic<int>& k = known[device][cluster == 2 ? 0 : (cluster == 4 ? 1 : 2)];
   int n = k.load(std::memory_order_relaxed);
   if (n == 0) {
-    auto kern = fwd_tc_kernel<D, BF16, GEN, true, false>;
+    auto kern = fwd_tc_kernel<D, BF16, GEN, true, false, 0>;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
@@ -1152,20 +1212,30 @@ cudaError_t launch_packed(FwdArgs a, const PackedCall& c, int dtype, int device,
   // sequences, whose walks are short: 16.5, 17.5)
   const double est = (a.Lq / BM + 0.5 * c.n) * a.Hq;
   const bool keys = est <= 2.0 * sms && c.total_k >= 256ll * c.n;
+  // Short sequences, where the rows say that many are: a block is 32 rows of up to four heads of a group, or 64 of two, and so many keys (300 of 17 rows,
+  // D = 128: 32/8 heads 168 -> 57 us, 8/1 heads 55 -> 20, 16 heads of their own 141 -> 98).  Heads with keys of their own do not share tiles: an infinite
+  // value of one would reach another as 0 x inf.
+  const int narrow = keys || a.Lq > 64ll * c.n ? 0 : (a.Lq > 32ll * c.n ? 64 : 32);
+  int heads = narrow > 0 ? BM / narrow : 1;
+  while (group % heads != 0) --heads;
+  a.packed.heads = heads, a.packed.blocks = group / heads;
   PackedPlan p{};
+  p.narrow = narrow, p.narrow_items = (a.packed.blocks + QT - 1) / QT;
   p.cu_q = c.cu_q, p.cu_k = c.cu_k, p.n = c.n, p.total_q = a.Lq, p.total_k = c.total_k;
   p.group = group, p.causal = a.causal, p.step_log = keys ? 0 : 1, p.sched = a.sched, p.status = a.status;
   const void* ptr[kPackedFwdMaps] = {a.q, a.k, a.v, a.o};
   const Str3* st[kPackedFwdMaps] = {&a.qs, &a.ks, &a.vs, &a.os};
   for (int m = 0; m < kPackedFwdMaps; ++m) {
     const bool of_k = m == kMapK || m == kMapV;
-    if (!packed_map(&p, dtype, ptr[m], D, of_k ? a.Skv : a.Lq, of_k ? a.Hkv : a.Hq, *st[m], 128, of_k)) return cudaErrorInvalidValue;
+    if (!packed_map(&p, dtype, ptr[m], D, of_k ? a.Skv : a.Lq, of_k ? a.Hkv : a.Hq, *st[m], 128, of_k, narrow > 0 ? (of_k ? 1 : heads) : 0)) return cudaErrorInvalidValue;
   }
   p.zero[0] = PackedPlan::Rows{static_cast<char*>(a.o), a.os.s * 2, a.os.h * 2, a.Hq, D * 2, false};
   p.n_zero = 1, p.lse = a.lse;
   cudaError_t e = launch_packed_plan(p, c.scratch, &a.packed, stream);
   if (e != cudaSuccess) return e;
   const int grid = static_cast<int>(blocks < static_cast<size_t>(sms) ? blocks : sms);
+  if (narrow == 32) return launch_k<D, BF16, GEN, false, true, 32>(a, dtype, grid, 1, stream);
+  if (narrow == 64) return launch_k<D, BF16, GEN, false, true, 64>(a, dtype, grid, 1, stream);
   return keys ? launch_k<D, BF16, GEN, true, true>(a, dtype, grid, 1, stream) : launch_k<D, BF16, GEN, false, true>(a, dtype, grid, 1, stream);
 }
 

@@ -31,6 +31,9 @@ struct PackedPlan {
   int64_t row_bytes[kPackedBwdMaps];
   bool of_k[kPackedBwdMaps];
   int n_maps;
+  // forward: sequences of up to `narrow` rows and keys have items of their own (0: none), so many, and maps whose boxes are so many rows of several heads
+  int narrow, narrow_items;
+  CUtensorMap narrow_base[kPackedFwdMaps], narrow_small[kPackedFwdMaps];
   CUtensorMap* maps;
   // rows behind the last sequence: zeros in these (of 16-byte multiples), and -inf in lse
   struct Rows {
@@ -59,7 +62,8 @@ size_t packed_plan_bytes(int n, int total_q, int total_k, int group, bool bwd);
 int packed_slots(int n, int total_q, int total_k, int Hq, int Hkv);
 
 // Adds the map of an operand [rows][H][D] (fp32: dense [H][rows][D]).
-bool packed_map(PackedPlan* p, int dtype, const void* ptr, int D, int rows, int H, const Str3& st, int box_rows, bool of_k);
+// narrow_heads: also one with boxes of p->narrow rows of so many heads.
+bool packed_map(PackedPlan* p, int dtype, const void* ptr, int D, int rows, int H, const Str3& st, int box_rows, bool of_k, int narrow_heads = 0);
 
 // Fills in items, maps and args from `scratch` and enqueues the planning kernel.
 cudaError_t launch_packed_plan(PackedPlan p, void* scratch, PackedArgs* args, cudaStream_t stream);

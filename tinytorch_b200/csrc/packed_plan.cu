@@ -29,9 +29,12 @@ struct Seq {
 };
 // x / group, exact up to 2^40 / group: a division by a variable takes as long as the rest of an item's plan
 __device__ __forceinline__ int by_group(const PackedPlan& p, int x) { return static_cast<int>(static_cast<uint64_t>(x) * p.per_group >> 40); }
+// A sequence whose heads share tiles.
+__device__ __forceinline__ bool is_narrow(const PackedPlan& p, const Seq& s) { return s.lq > 0 && s.lk > 0 && s.lq <= p.narrow && s.lk <= p.narrow; }
 // Items of a sequence, and the tiles that item i walks over.
 __device__ __forceinline__ int items_of(const PackedPlan& p, const Seq& s) {
   if (p.bwd) return (s.lk + kTile - 1) / kTile;
+  if (is_narrow(p, s)) return p.narrow_items;
   return ((s.lq + kTile - 1) / kTile * p.group + (1 << p.step_log) - 1) >> p.step_log;
 }
 __device__ __forceinline__ int walk_of(const PackedPlan& p, const Seq& s, int i) {  // (query tiles of one head; key tiles of the longer of a pair)
@@ -97,7 +100,10 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
       const Seq q = load_seq(s);
       const int row = p.of_k[m] ? q.k0 : q.q0, rows = p.of_k[m] ? q.lk : q.lq;
       if (rows <= 0) continue;
-      s_map[warp][lane] = reinterpret_cast<const uint32_t*>(rows < p.long_rows[m] ? &p.small[m] : &p.base[m])[lane];
+      const bool small = rows < p.long_rows[m];
+      const CUtensorMap* from = small ? &p.small[m] : &p.base[m];
+      if (is_narrow(p, q)) from = small ? &p.narrow_small[m] : &p.narrow_base[m];
+      s_map[warp][lane] = reinterpret_cast<const uint32_t*>(from)[lane];
       __syncwarp();
       if (lane == 0) {
         const uint32_t at = ptx::smem_u32(s_map[warp]);
@@ -130,10 +136,12 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
   // ------------------------------------------------------------------ the items --
   if (p.sched && tid == 0) *p.sched = 0;
   if (bad) {
-    if (tid == 0) p.n_items[0] = p.n_items[1] = 0;
+    if (tid == 0) p.n_items[0] = p.n_items[1] = p.n_items[2] = 0;
     if (tid == 0 && p.status) atomicOr(p.status, kStatusBadOffsets);
     return;
   }
+  // (narrow items have a level of their own, below the others')
+  auto level_of = [&](const Seq& q, int steps) { return p.narrow == 0 ? steps >> p.shift : (is_narrow(p, q) ? 0 : (steps >> p.shift) + 1); };
   // A thread to a short sequence, up to all of them to a long one.
   const int width = 1 << p.width_log, mine = tid >> p.width_log, teams = kThreads >> p.width_log, id = tid & (width - 1);
   int share = 0x7fffffff;  // no walk is longer
@@ -153,7 +161,7 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
     const int n = items_of(p, q);
     for (int i = id; i < n; i += width) {
       const int steps = p.bwd ? walk_of(p, q, i) * p.group : walk_of(p, q, i), parts = parts_of(steps, share);
-      for (int k = 0; k < parts; ++k) atomicAdd(&s_level[(part_from(steps, k + 1, parts) - part_from(steps, k, parts)) >> p.shift], 1);
+      for (int k = 0; k < parts; ++k) atomicAdd(&s_level[level_of(q, part_from(steps, k + 1, parts) - part_from(steps, k, parts))], 1);
     }
   }
   __syncthreads();
@@ -180,7 +188,7 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
       if (lane >= of) w += o;
     }
     if (lane < kWarps) s_warp_sum[lane] = w;
-    if (lane == 31) *p.n_items = w;
+    if (lane == 31) p.n_items[0] = w - (p.narrow > 0 ? s_level[0] : 0), p.n_items[2] = p.narrow > 0 ? s_level[0] : 0;
   }
   __syncthreads();
   int place = upto - sum + (warp > 0 ? s_warp_sum[warp - 1] : 0);
@@ -203,7 +211,7 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
       }
       for (int k = 0; k < parts; ++k) {
         const int from = part_from(steps, k, parts), own = part_from(steps, k + 1, parts) - from;
-        int4* e = reinterpret_cast<int4*>(p.items + atomicAdd(&s_level[own >> p.shift], 1));
+        int4* e = reinterpret_cast<int4*>(p.items + atomicAdd(&s_level[level_of(q, own)], 1));
         e[0] = make_int4(q.q0, q.lq, q.k0, q.lk);
         e[1] = make_int4(p.bwd ? i : i << p.step_log, s, from, own);
         if (p.bwd) e[2] = make_int4(slot < 0 ? -1 : slot + k, 0, 0, 0);
@@ -230,7 +238,7 @@ bool same_kind(const CUtensorMap& a, const CUtensorMap& b) {
 
 }  // namespace
 
-bool packed_map(PackedPlan* p, int dtype, const void* ptr, int D, int rows, int H, const Str3& st, int box_rows, bool of_k) {
+bool packed_map(PackedPlan* p, int dtype, const void* ptr, int D, int rows, int H, const Str3& st, int box_rows, bool of_k, int narrow_heads) {
   const int m = p->n_maps++;
   const int64_t es = dtype == TT_ATTN_F32 ? 4 : 2;
   auto encode = [&](CUtensorMap* map, int n) {
@@ -238,6 +246,9 @@ bool packed_map(PackedPlan* p, int dtype, const void* ptr, int D, int rows, int 
   };
   p->address[m] = static_cast<const char*>(ptr), p->row_bytes[m] = st.s * es, p->of_k[m] = of_k;
   if (!encode(&p->base[m], rows) || !encode(&p->small[m], 1)) return false;
+  if (narrow_heads > 0 && (!make_map(&p->narrow_base[m], dtype, ptr, D, rows, H, 1, st, p->narrow, 64, narrow_heads) ||
+                           !make_map(&p->narrow_small[m], dtype, ptr, D, 1, H, 1, st, p->narrow, 64, narrow_heads)))
+    return false;
   if (same_kind(p->base[m], p->small[m])) {
     p->long_rows[m] = 1;
     return true;
@@ -300,12 +311,12 @@ cudaError_t launch_packed_plan(PackedPlan p, void* scratch, PackedArgs* args, cu
   // levels 0 ... the longest walk that there can be
   const int64_t longest = p.bwd ? (static_cast<int64_t>(p.total_q) + kTile - 1) / kTile * p.group : (static_cast<int64_t>(p.total_k) + kTile - 1) / kTile;
   p.shift = 0;
-  while ((longest >> p.shift) >= kMine * threads) ++p.shift;
-  p.levels = static_cast<int>(longest >> p.shift) + 1;
+  while ((longest >> p.shift) + 1 >= kMine * threads) ++p.shift;
+  p.levels = static_cast<int>(longest >> p.shift) + 1 + (p.narrow > 0);
   // threads to a sequence: as many as it has items on the average, unless there are more threads than that takes
   p.width_log = 0;
   for (int width = 1; width < threads && (static_cast<size_t>(width) * p.n < items || 2ll * width * p.n <= threads); width *= 2) ++p.width_log;
-  *args = PackedArgs{p.items, p.n_items, p.splits, p.maps};
+  args->items = p.items, args->n_items = p.n_items, args->splits = p.splits, args->maps = p.maps;
   const int64_t maps = static_cast<int64_t>(p.n) * p.n_maps + (p.total_q + p.total_k) / 64;  // a warp each, and one to 64 rows, which may have to be cleared
   const int64_t most = 2 * kSms * (1024 / threads), ctas = (maps + warps - 1) / warps;
   const dim3 grid(1 + static_cast<unsigned>(ctas < 1 ? 1 : (ctas < most ? ctas : most)));
