@@ -412,6 +412,15 @@ def test_short_sequences_keep_to_themselves(poison):
     keep[20:29, 4:] = False
     assert torch.equal(got[0][keep], want[0][keep]) and torch.equal(got[1].t()[keep], want[1].t()[keep])
     assert not got[0][22:29, 4:].isfinite().all()
+    g = make(sum(lens), Hq, D, torch.bfloat16, 4)
+    back = op.sdpAttentionPackedBwd(g, q, k, v, *got, offsets(lens), True)
+    v[22, 1], k[23, 1] = 0, 0
+    clean = op.sdpAttentionPackedFwd(q, k, v, offsets(lens), True)
+    fine = op.sdpAttentionPackedBwd(g, q, k, v, *clean, offsets(lens), True)
+    for i, (x, y) in enumerate(zip(back, fine)):
+        keep = torch.ones(x.shape[:2], dtype=torch.bool, device="cuda")
+        keep[20:29, 4 if i == 0 else 1:] = False
+        assert torch.equal(x[keep], y[keep])
 
 
 def test_offsets_changed_between_the_passes_are_an_error():

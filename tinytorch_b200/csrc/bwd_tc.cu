@@ -62,6 +62,7 @@ struct Item {
   int mask;                      // whether the mask has to be looked at
   int n_q;                       // packed: query tiles of the sequence,
   int q0, lq, k0, lk, seq;       // its first rows of q and k, and how many
+  int heads, cols;               // query heads of a tile (short sequences: several), and its columns of one, less one
 };
 
 struct __align__(8) SmemCtl {
@@ -219,8 +220,9 @@ __device__ __forceinline__ void ds_chunk(const uint32_t (&p)[16], const uint32_t
 // GEN: the general variant (a mask and / or a causal triangle that is not top-left
 // aligned); the fast variant compiles all of that out.  PARTS: a key tile's walk is
 // divided among a.parts work items (see bwd_parts).  PACKED: sequences packed behind one another, whose items and tensor
-// maps packed_plan.cu has made; without a mask; PARTS: some walks are divided (a.parts: slots for shares of dK / dV, per kv head).
-template <bool BF16, bool GEN, bool PARTS, bool PACKED>
+// maps packed_plan.cu has made; without a mask; PARTS: some walks are divided (a.parts: slots for shares of dK / dV, per kv head);
+// NARROW: a query tile of a short sequence is several heads' rows.
+template <bool BF16, bool GEN, bool PARTS, bool PACKED, bool NARROW>
 __global__ void __launch_bounds__(Cfg128::kThreads, 1)
     bwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
@@ -289,6 +291,10 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
       it.q0 = rows.x, it.lq = Lq = rows.y, it.k0 = rows.z, it.lk = kv_len = rows.w;
       nt = place.x, it.seq = place.y;
       it.n_q = n_q_tiles = (Lq + BQ - 1) / BQ;
+      if constexpr (NARROW) {
+        const bool narrow = Lq <= a.packed.narrow;
+        it.heads = narrow ? a.packed.heads : 1, it.cols = narrow ? a.packed.narrow - 1 : BQ - 1;
+      }
       if (PARTS) from = place.z, steps = place.w, it.part = __ldcg(&a.packed.items[nt0].slot);
     }
     it.kv0 = nt * BM;
@@ -302,17 +308,17 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
     // BM == BQ: query tiles before the key tile see none of it (general: first tile with a row i >= kv0 - shift)
     it.qt_begin = a.causal ? (GEN ? (it.kv0 - it.shift > 0 ? (it.kv0 - it.shift) / BQ : 0) : nt) : 0;
     const int per_head = (it.kv0 < kv_len && it.qt_begin < n_q_tiles) ? n_q_tiles - it.qt_begin : 0;
-    it.n_steps = per_head * group, it.h = it.hk * group, it.qt = it.qt_begin;
+    it.n_steps = per_head * (NARROW && it.heads > 1 ? a.packed.blocks : group), it.h = it.hk * group, it.qt = it.qt_begin;
     if (PARTS && per_head > 0) {
       const int n0 = PACKED ? from : part_begin(it.n_steps, it.part, a.parts);
       it.n_steps = PACKED ? steps : part_begin(it.n_steps, it.part + 1, a.parts) - n0;
-      it.h += n0 / per_head, it.qt += n0 % per_head;
+      it.h += n0 / per_head * (NARROW ? it.heads : 1), it.qt += n0 % per_head;
     }
     return it;
   };
   // the next query tile of the walk
   auto advance = [&](int& h, int& qt, const Item& it) {
-    if (++qt == (PACKED ? it.n_q : n_q_all)) qt = it.qt_begin, ++h;
+    if (++qt == (PACKED ? it.n_q : n_q_all)) qt = it.qt_begin, h += NARROW ? it.heads : 1;
   };
 
   if (warp == C::kProdWarp && lane == 0) {
@@ -381,9 +387,12 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
         const int row = j * 32 + lane;
         lv[j] = -INFINITY;  // rows beyond Lq behave like rows without any participating key: P = 0
         dl[j] = 0.f;
-        if (q0 + row < (PACKED ? it.lq : a.Lq)) {
-          lv[j] = a.lse[base + row];
-          dl[j] = a.delta[base + row];
+        // (narrow: row `at` of one of the tile's heads)
+        const int at = NARROW ? row & it.cols : row;
+        const int64_t i = base + at + (NARROW ? static_cast<int64_t>(row - at) / (it.cols + 1) * a.Lq : 0);
+        if (q0 + at < (PACKED ? it.lq : a.Lq)) {
+          lv[j] = a.lse[i];
+          dl[j] = a.delta[i];
         }
       }
       float* nv = svec + (g & 1) * 2 * BQ;
@@ -617,6 +626,7 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
       // a warpgroup leaves as one (its named barriers below count all 128 threads) when any of its waits ran out
       if (ptx::named_barrier_or(3 + wg, BM, !ok)) break;
       if (it.n_steps < 0) break;
+      const int cols = NARROW ? it.cols : 0;
       const int b = it.b, hk = it.hk, kv0 = it.kv0, kv_len = it.kv_len, shift = it.shift, n_steps = it.n_steps;
       int h = it.h, qt = it.qt;  // query head and tile of the step
       const int kv_row = kv0 + r;
@@ -685,7 +695,7 @@ __global__ void __launch_bounds__(Cfg128::kThreads, 1)
           ptx::tmem_wait_ld();
           uint32_t pk[8], dk[8];
           int n_hidden = 0;
-          if (masked) n_hidden = !row_valid ? 16 : (diag ? kv_row - (q0 + col + shift) : 0);
+          if (masked) n_hidden = !row_valid ? 16 : (diag ? kv_row - (q0 + (NARROW ? col & cols : col) + shift) : 0);
           p_chunk<BF16, MASK, T>(a, s, vec + col, c2v, n_hidden, MASK && it.mask, mw[sc], pk);
           ds_chunk<BF16>(s, dp, vec + BQ + col, sc2, dk);
           // Warpgroup w keeps its 16-bit results in columns [32w, 32w+16) of the
@@ -842,7 +852,7 @@ struct Cfg64 {
   static constexpr int kProdWarp = 20, kIssWarp = 21, kThreads = 768;
 };
 
-template <bool BF16, bool GEN, bool PARTS, bool PACKED>
+template <bool BF16, bool GEN, bool PARTS, bool PACKED, bool NARROW>
 __global__ void __launch_bounds__(Cfg64::kThreads, 1)
     bwd_tc64_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
@@ -906,6 +916,10 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
       it.q0 = rows.x, it.lq = Lq = rows.y, it.k0 = rows.z, it.lk = kv_len = rows.w;
       nt = place.x, it.seq = place.y;
       it.n_q = n_q_tiles = (Lq + BQ - 1) / BQ;
+      if constexpr (NARROW) {
+        const bool narrow = Lq <= a.packed.narrow;
+        it.heads = narrow ? a.packed.heads : 1, it.cols = narrow ? a.packed.narrow - 1 : BQ - 1;
+      }
       if (PARTS) from = place.z, steps = place.w, it.part = __ldcg(&a.packed.items[nt0].slot);
     }
     it.kv0 = nt * BM;
@@ -919,17 +933,17 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
     // BM == BQ: query tiles before the key tile see none of it (general: first tile with a row i >= kv0 - shift)
     it.qt_begin = a.causal ? (GEN ? (it.kv0 - it.shift > 0 ? (it.kv0 - it.shift) / BQ : 0) : nt) : 0;
     const int per_head = (it.kv0 < kv_len && it.qt_begin < n_q_tiles) ? n_q_tiles - it.qt_begin : 0;
-    it.n_steps = per_head * group, it.h = it.hk * group, it.qt = it.qt_begin;
+    it.n_steps = per_head * (NARROW && it.heads > 1 ? a.packed.blocks : group), it.h = it.hk * group, it.qt = it.qt_begin;
     if (PARTS && per_head > 0) {
       const int n0 = PACKED ? from : part_begin(it.n_steps, it.part, a.parts);
       it.n_steps = PACKED ? steps : part_begin(it.n_steps, it.part + 1, a.parts) - n0;
-      it.h += n0 / per_head, it.qt += n0 % per_head;
+      it.h += n0 / per_head * (NARROW ? it.heads : 1), it.qt += n0 % per_head;
     }
     return it;
   };
   // the next query tile of the walk
   auto advance = [&](int& h, int& qt, const Item& it) {
-    if (++qt == (PACKED ? it.n_q : n_q_all)) qt = it.qt_begin, ++h;
+    if (++qt == (PACKED ? it.n_q : n_q_all)) qt = it.qt_begin, h += NARROW ? it.heads : 1;
   };
 
   if (warp == C::kProdWarp && lane == 0) {
@@ -1096,9 +1110,12 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
             const int row = j * 32 + lane;
             lv[j] = -INFINITY;  // rows beyond Lq behave like rows without any participating key: P = 0
             dl[j] = 0.f;
-            if (q0 + row < (PACKED ? it.lq : a.Lq)) {
-              lv[j] = a.lse[base + row];
-              dl[j] = a.delta[base + row];
+            // (narrow: row `at` of one of the tile's heads)
+            const int at = NARROW ? row & it.cols : row;
+            const int64_t i = base + at + (NARROW ? static_cast<int64_t>(row - at) / (it.cols + 1) * a.Lq : 0);
+            if (q0 + at < (PACKED ? it.lq : a.Lq)) {
+              lv[j] = a.lse[i];
+              dl[j] = a.delta[i];
             }
           }
           float* nv = svec + (g & 1) * 2 * BQ;
@@ -1295,7 +1312,8 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
             }
           }
         }
-        const int h = it.h, q0 = it.qt * BQ + wj * 32;
+        // (narrow: a warp's rows are of one head)
+        const int q0 = it.qt * BQ + (NARROW ? (wj * 32) & it.cols : wj * 32), h = it.h + (NARROW ? wj * 32 / (it.cols + 1) : 0);
         wwait(&ctl->dq_full[g & 1], (g >> 1) & 1);
         ptx::tc_fence_after();
 #pragma unroll
@@ -1365,7 +1383,7 @@ __global__ void __launch_bounds__(Cfg64::kThreads, 1)
           ptx::tmem_wait_ld();
           uint32_t pk[8];
           int n_hidden = 0;
-          if (masked) n_hidden = kv_row >= it.kv_len ? 16 : (diag ? kv_row - (q0 + col + it.shift) : 0);
+          if (masked) n_hidden = kv_row >= it.kv_len ? 16 : (diag ? kv_row - (q0 + (NARROW ? col & it.cols : col) + it.shift) : 0);
           p_chunk<BF16, MASK, T>(a, p[sc], vec + col, c2v, n_hidden, MASK && it.mask, mw[sc], pk);
           // Warpgroup w keeps its 16-bit results in columns [32w, 32w+16) of the region, i.e. over the first 16
           // columns it loaded itself, never over columns another warpgroup still has to read.
@@ -1506,8 +1524,8 @@ cudaError_t launch_t(const BwdArgs& a, int dtype, int device, cudaStream_t strea
     return cudaErrorInvalidValue;
   cudaError_t e;  // (dq_accum has been cleared by the delta pre-pass)
   void (*kern)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, BwdArgs);
-  if constexpr (D == 64) kern = a.parts > 1 ? bwd_tc64_kernel<BF16, GEN, true, false> : bwd_tc64_kernel<BF16, GEN, false, false>;
-  else kern = a.parts > 1 ? bwd_tc_kernel<BF16, GEN, true, false> : bwd_tc_kernel<BF16, GEN, false, false>;
+  if constexpr (D == 64) kern = a.parts > 1 ? bwd_tc64_kernel<BF16, GEN, true, false, false> : bwd_tc64_kernel<BF16, GEN, false, false, false>;
+  else kern = a.parts > 1 ? bwd_tc_kernel<BF16, GEN, true, false, false> : bwd_tc_kernel<BF16, GEN, false, false, false>;
   constexpr int kSmemBytes = D == 64 ? Cfg64::kSmem : Cfg128::kSmem;
   constexpr int kBlock = D == 64 ? Cfg64::kThreads : Cfg128::kThreads;
   e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
@@ -1571,23 +1589,28 @@ cudaError_t launch_packed(BwdArgs a, const PackedCall& c, int dtype, int device,
   constexpr int kOutRows = D == 64 ? 32 : 128;
   const int sms = sm_count(device);
   PackedPlan p{};
+  PackedMaps maps;
   p.cu_q = c.cu_q, p.cu_k = c.cu_k, p.n = c.n, p.total_q = a.Lq, p.total_k = c.total_k;
   p.group = a.Hq / a.Hkv, p.causal = a.causal, p.bwd = true, p.status = a.status;
   p.kv_heads = a.Hkv, p.slots = c.shares ? packed_slots(c.n, a.Lq, c.total_k, a.Hq, a.Hkv) : 0;
+  // Short sequences, where the rows say that many are: a tile of queries is 32 rows of four heads of a group, or 64 of two (whole tiles alone: what lay in the
+  // others' place would go into sums).  300 of 17 rows, 32/8 heads: D = 128 318 -> 178 us, D = 64 165 -> 105; 64 of 64 rows 117 -> 98, 61 -> 54.
+  const int narrow = a.Lq <= 32ll * c.n && p.group % 4 == 0 ? 32 : (a.Lq <= 64ll * c.n && p.group % 2 == 0 ? 64 : 0), heads = narrow > 0 ? BQ / narrow : 1;
+  a.packed.narrow = p.narrow = narrow, a.packed.heads = heads, a.packed.blocks = p.narrow_items = p.group / heads;
   // (an absent output gets a map that is never used)
   const Str3 accum{0, static_cast<int64_t>(a.Lq) * D, D};
   const void* ptr[kPackedBwdMaps] = {a.q, a.k, a.v, a.d_o, a.dq_accum, a.dk ? a.dk : a.k, a.dv ? a.dv : a.v};
   const Str3* st[kPackedBwdMaps] = {&a.qs, &a.ks, &a.vs, &a.dos, &accum, a.dk ? &a.dks : &a.ks, a.dv ? &a.dvs : &a.vs};
   for (int m = 0; m < kPackedBwdMaps; ++m) {
     const bool of_k = m == kMapK || m == kMapV || m == kMapdK || m == kMapdV;
-    const bool made = m == kMapdQ ? packed_map(&p, TT_ATTN_F32, a.dq_accum, D, a.Lq, a.Hq, accum, D == 64 ? 32 : 128, false)
-                                  : packed_map(&p, dtype, ptr[m], D, of_k ? a.Skv : a.Lq, of_k ? a.Hkv : a.Hq, *st[m],
-                                               m == kMapdK || m == kMapdV ? kOutRows : 128, of_k);
+    const bool made = m == kMapdQ ? packed_map(&p, &maps, TT_ATTN_F32, a.dq_accum, D, a.Lq, a.Hq, accum, D == 64 ? 32 : 128, false, D == 64 ? 0 : heads)
+                                  : packed_map(&p, &maps, dtype, ptr[m], D, of_k ? a.Skv : a.Lq, of_k ? a.Hkv : a.Hq, *st[m],
+                                               m == kMapdK || m == kMapdV ? kOutRows : 128, of_k, of_k ? 0 : heads);
     if (!made) return cudaErrorInvalidValue;
   }
   if (a.dk) p.zero[p.n_zero++] = PackedPlan::Rows{static_cast<char*>(a.dk), a.dks.s * 2, a.dks.h * 2, a.Hkv, D * 2, true};
   if (a.dv) p.zero[p.n_zero++] = PackedPlan::Rows{static_cast<char*>(a.dv), a.dvs.s * 2, a.dvs.h * 2, a.Hkv, D * 2, true};
-  cudaError_t e = launch_packed_plan(p, c.scratch, &a.packed, stream);
+  cudaError_t e = launch_packed_plan(p, maps, c.scratch, &a.packed, stream);
   if (e != cudaSuccess) return e;
   a.parts = p.slots, a.dkv_part = c.shares;
   BwdArgs pre = a;
@@ -1595,9 +1618,13 @@ cudaError_t launch_packed(BwdArgs a, const PackedCall& c, int dtype, int device,
   e = launch_bwd_delta(dtype, D, pre, stream);
   if (e != cudaSuccess) return e;
   void (*kern)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, BwdArgs);
-  if constexpr (D == 64) kern = p.slots > 0 ? bwd_tc64_kernel<BF16, GEN, true, true> : bwd_tc64_kernel<BF16, GEN, false, true>;
-  else kern = p.slots > 0 ? bwd_tc_kernel<BF16, GEN, true, true> : bwd_tc_kernel<BF16, GEN, false, true>;
-  CUtensorMap tdk = p.base[kMapdK], tdv = p.base[kMapdV];  // (whole walks go through their sequence's)
+  auto pick = [&](auto nw) {
+    constexpr bool N = decltype(nw)::value;
+    if constexpr (D == 64) return p.slots > 0 ? bwd_tc64_kernel<BF16, GEN, true, true, N> : bwd_tc64_kernel<BF16, GEN, false, true, N>;
+    else return p.slots > 0 ? bwd_tc_kernel<BF16, GEN, true, true, N> : bwd_tc_kernel<BF16, GEN, false, true, N>;
+  };
+  kern = narrow > 0 ? pick(std::true_type{}) : pick(std::false_type{});
+  CUtensorMap tdk = maps.kind[0][kMapdK], tdv = maps.kind[0][kMapdV];  // (whole walks go through their sequence's)
   if (p.slots > 0 && (!make_map_f32(&tdk, c.shares, D, BM, a.Hkv * p.slots, 1, kOutRows) ||
                       !make_map_f32(&tdv, c.shares + static_cast<int64_t>(a.Hkv) * p.slots * BM * D, D, BM, a.Hkv * p.slots, 1, kOutRows)))
     return cudaErrorInvalidValue;
@@ -1607,7 +1634,7 @@ cudaError_t launch_packed(BwdArgs a, const PackedCall& c, int dtype, int device,
   if (e != cudaSuccess) return e;
   const size_t most = (packed_items(c.n, a.Skv, 1, 1) + p.slots) * a.Hkv;
   e = launch_early(kern, dim3(static_cast<unsigned>(most < static_cast<size_t>(sms) ? most : sms)), dim3(kBlock), kSmemBytes, stream, 1,
-                   p.base[kMapQ], p.base[kMapK], p.base[kMapV], p.base[kMapdO], p.base[kMapdQ], tdk, tdv, a);
+                   maps.kind[0][kMapQ], maps.kind[0][kMapK], maps.kind[0][kMapV], maps.kind[0][kMapdO], maps.kind[0][kMapdQ], tdk, tdv, a);
   if (e == cudaSuccess && p.slots > 0) e = launch_early(packed_sum_kernel<T, D>, dim3(4 * sms), dim3(256), 0, stream, 1, a);
   if (e != cudaSuccess || !a.dq) return e;
   a.parts = 1;  // (to the conversion: there is dQ only)

@@ -71,7 +71,8 @@ struct PackedArgs {
   const int* n_items;  // [0] items, [1] splits, [2] narrow items, which follow the others
   const PackedSplit* splits;
   const void* maps;  // CUtensorMap [sequence][kPackedFwdMaps or kPackedBwdMaps]
-  int heads, blocks;  // forward, narrow items (of short sequences): query heads of a block, blocks of a kv head
+  // short sequences, whose heads share tiles: of up to `narrow` rows (backward; 0: none); query heads of a tile, and tiles of a kv head
+  int narrow, heads, blocks;
 };
 enum PackedMap { kMapQ, kMapK, kMapV, kMapO, kPackedFwdMaps, kMapdO = kMapO, kMapdQ, kMapdK, kMapdV, kPackedBwdMaps };
 

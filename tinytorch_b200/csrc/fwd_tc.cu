@@ -38,7 +38,7 @@
 //                       the next item's first QK.
 // P never leaves TMEM: the second MMA takes its A operand from TMEM.
 // PACKED: sequences behind one another; the items and a set of tensor maps for every sequence come from packed_plan.cu, so that the loops are the same.
-// 12 prompts of 1 to 4096 rows, 32/8 heads, D = 128, bf16: 306 us (1092 TFLOP/s, as unpacked); five of 677 rows: 16 us, most of it latency.
+// 12 prompts of 1 to 4096 rows, 32/8 heads, D = 128, bf16: 305 us (1097 TFLOP/s, as unpacked); five of 677 rows: 15.5 us, most of it latency.
 // Every mbarrier wait is bounded; an expired wait sets the status word and makes
 // the CTA unwind.
 #include <cuda.h>
@@ -1220,6 +1220,7 @@ cudaError_t launch_packed(FwdArgs a, const PackedCall& c, int dtype, int device,
   while (group % heads != 0) --heads;
   a.packed.heads = heads, a.packed.blocks = group / heads;
   PackedPlan p{};
+  PackedMaps maps;
   p.narrow = narrow, p.narrow_items = (a.packed.blocks + QT - 1) / QT;
   p.cu_q = c.cu_q, p.cu_k = c.cu_k, p.n = c.n, p.total_q = a.Lq, p.total_k = c.total_k;
   p.group = group, p.causal = a.causal, p.step_log = keys ? 0 : 1, p.sched = a.sched, p.status = a.status;
@@ -1227,11 +1228,11 @@ cudaError_t launch_packed(FwdArgs a, const PackedCall& c, int dtype, int device,
   const Str3* st[kPackedFwdMaps] = {&a.qs, &a.ks, &a.vs, &a.os};
   for (int m = 0; m < kPackedFwdMaps; ++m) {
     const bool of_k = m == kMapK || m == kMapV;
-    if (!packed_map(&p, dtype, ptr[m], D, of_k ? a.Skv : a.Lq, of_k ? a.Hkv : a.Hq, *st[m], 128, of_k, narrow > 0 ? (of_k ? 1 : heads) : 0)) return cudaErrorInvalidValue;
+    if (!packed_map(&p, &maps, dtype, ptr[m], D, of_k ? a.Skv : a.Lq, of_k ? a.Hkv : a.Hq, *st[m], 128, of_k, narrow > 0 ? (of_k ? 1 : heads) : 0)) return cudaErrorInvalidValue;
   }
   p.zero[0] = PackedPlan::Rows{static_cast<char*>(a.o), a.os.s * 2, a.os.h * 2, a.Hq, D * 2, false};
   p.n_zero = 1, p.lse = a.lse;
-  cudaError_t e = launch_packed_plan(p, c.scratch, &a.packed, stream);
+  cudaError_t e = launch_packed_plan(p, maps, c.scratch, &a.packed, stream);
   if (e != cudaSuccess) return e;
   const int grid = static_cast<int>(blocks < static_cast<size_t>(sms) ? blocks : sms);
   if (narrow == 32) return launch_k<D, BF16, GEN, false, true, 32>(a, dtype, grid, 1, stream);

@@ -23,17 +23,16 @@ struct PackedPlan {
   int* n_items;         // [0] items, [1] divided key tiles
   int* sched;           // set to zero, or null
   int32_t* status;
-  // tensor maps (see packed_map): those of the whole tensors, those of one row, and from how many rows on a sequence takes the former;
-  // which of them go along with k; rows are dimension 1
-  CUtensorMap base[kPackedBwdMaps], small[kPackedBwdMaps];
+  // tensor maps (see PackedMaps): from how many rows on a sequence takes those of the whole tensors; which go along with k; rows are dimension 1
   int long_rows[kPackedBwdMaps];
   const char* address[kPackedBwdMaps];
   int64_t row_bytes[kPackedBwdMaps];
   bool of_k[kPackedBwdMaps];
   int n_maps;
-  // forward: sequences of up to `narrow` rows and keys have items of their own (0: none), so many, and maps whose boxes are so many rows of several heads
+  // Sequences of up to `narrow` rows (forward: and keys; 0: none) have maps of their own, where there are such, whose boxes are so many rows of several
+  // heads; forward: items of their own, so many; backward: so many steps for a query tile of all heads of a group
   int narrow, narrow_items;
-  CUtensorMap narrow_base[kPackedFwdMaps], narrow_small[kPackedFwdMaps];
+  bool has_narrow[kPackedBwdMaps];
   CUtensorMap* maps;
   // rows behind the last sequence: zeros in these (of 16-byte multiples), and -inf in lse
   struct Rows {
@@ -44,6 +43,11 @@ struct PackedPlan {
   } zero[3];
   int n_zero;
   float* lse;  // [heads of zero[0]][total_q]
+};
+
+// What sequences' maps are made of: the maps of the whole tensors and of one row, and those two with narrow boxes.
+struct PackedMaps {
+  CUtensorMap kind[4][kPackedBwdMaps];
 };
 
 // A call over packed sequences.
@@ -63,10 +67,10 @@ int packed_slots(int n, int total_q, int total_k, int Hq, int Hkv);
 
 // Adds the map of an operand [rows][H][D] (fp32: dense [H][rows][D]).
 // narrow_heads: also one with boxes of p->narrow rows of so many heads.
-bool packed_map(PackedPlan* p, int dtype, const void* ptr, int D, int rows, int H, const Str3& st, int box_rows, bool of_k, int narrow_heads = 0);
+bool packed_map(PackedPlan* p, PackedMaps* maps, int dtype, const void* ptr, int D, int rows, int H, const Str3& st, int box_rows, bool of_k, int narrow_heads = 0);
 
 // Fills in items, maps and args from `scratch` and enqueues the planning kernel.
-cudaError_t launch_packed_plan(PackedPlan p, void* scratch, PackedArgs* args, cudaStream_t stream);
+cudaError_t launch_packed_plan(PackedPlan p, const PackedMaps& maps, void* scratch, PackedArgs* args, cudaStream_t stream);
 
 // The forward and the backward; a's B is 1, its Lq and Skv are the rows of all sequences.
 cudaError_t launch_fwd_packed(int dtype, int D, const FwdArgs& a, const PackedCall& c, int device, cudaStream_t stream);

@@ -13,6 +13,8 @@
 // knows that from the rows and heads) walks that are longer than an SM's share of all steps are divided, into items of half a share
 // at most, each of which leaves dK and dV in a slot of the workspace.  Steps, D = 128, 2.9 us: 8192 rows, 8/1 heads 1397 -> 475 us;
 // 4096, 8/2 heads 365 -> 156; divided without need, 2 x 1000 rows of 16 heads take 72 us instead of 50.
+#include <type_traits>
+
 #include "packed.cuh"
 
 #include "ptx.cuh"
@@ -30,16 +32,21 @@ struct Seq {
 // x / group, exact up to 2^40 / group: a division by a variable takes as long as the rest of an item's plan
 __device__ __forceinline__ int by_group(const PackedPlan& p, int x) { return static_cast<int>(static_cast<uint64_t>(x) * p.per_group >> 40); }
 // A sequence whose heads share tiles.
-__device__ __forceinline__ bool is_narrow(const PackedPlan& p, const Seq& s) { return s.lq > 0 && s.lk > 0 && s.lq <= p.narrow && s.lk <= p.narrow; }
+template <bool BWD, bool NARROW>
+__device__ __forceinline__ bool is_narrow(const PackedPlan& p, const Seq& s) {
+  return NARROW && s.lq > 0 && s.lk > 0 && s.lq <= p.narrow && (BWD || s.lk <= p.narrow);
+}
 // Items of a sequence, and the tiles that item i walks over.
+template <bool BWD, bool NARROW>
 __device__ __forceinline__ int items_of(const PackedPlan& p, const Seq& s) {
-  if (p.bwd) return (s.lk + kTile - 1) / kTile;
-  if (is_narrow(p, s)) return p.narrow_items;
+  if (BWD) return (s.lk + kTile - 1) / kTile;
+  if (is_narrow<BWD, NARROW>(p, s)) return p.narrow_items;
   return ((s.lq + kTile - 1) / kTile * p.group + (1 << p.step_log) - 1) >> p.step_log;
 }
+template <bool BWD>
 __device__ __forceinline__ int walk_of(const PackedPlan& p, const Seq& s, int i) {  // (query tiles of one head; key tiles of the longer of a pair)
   const int shift = causal_shift(p.causal, s.lk, s.lq);
-  if (p.bwd) {
+  if (BWD) {
     const int nq = (s.lq + kTile - 1) / kTile, first = i * kTile - shift;
     const int from = p.causal && first > 0 ? first / kTile : 0;
     return from < nq ? nq - from : 0;
@@ -53,6 +60,12 @@ __device__ __forceinline__ int walk_of(const PackedPlan& p, const Seq& s, int i)
   return (end + kTile - 1) / kTile;
 }
 
+// ... and the steps that those are: backward, for every head of the group, or several heads at a time
+template <bool BWD, bool NARROW>
+__device__ __forceinline__ int steps_of(const PackedPlan& p, const Seq& s, int i) {
+  return walk_of<BWD>(p, s, i) * (BWD ? (is_narrow<BWD, NARROW>(p, s) ? p.narrow_items : p.group) : 1);
+}
+
 // Items that a key tile's n steps are divided into, and where one of them begins.  `share`: an SM's of all steps.
 __device__ __forceinline__ int parts_of(int n, int share) {
   const int most = max(share / 2 + share % 2, kLeastSteps);
@@ -60,8 +73,17 @@ __device__ __forceinline__ int parts_of(int n, int share) {
 }
 __device__ __forceinline__ int part_from(int n, int p, int parts) { return parts == 1 ? n * p : static_cast<int>(static_cast<int64_t>(n) * p / parts); }
 
-template <int kThreads>
-__global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_constant__ PackedPlan p) {
+// The plan is a short call's first few microseconds (677 rows of 5 sequences, 32/8 heads: 2 of 15.5), most of them instructions that no cache has yet: no
+// divisions, a kernel of its own for each direction, for calls with short sequences and for few items (one kernel for all: 1.2 us more).
+constexpr int maps_of(bool bwd, bool narrow) { return (bwd ? kPackedBwdMaps : kPackedFwdMaps) * (narrow ? 4 : 2); }
+template <int N>
+struct MapSet {
+  CUtensorMap map[N];  // [kind][map]
+};
+
+template <int kThreads, bool BWD, bool NARROW>
+__global__ void __launch_bounds__(kThreads)
+    packed_plan_kernel(const __grid_constant__ PackedPlan p, const __grid_constant__ MapSet<maps_of(BWD, NARROW)> maps) {
   constexpr int kWarps = kThreads / 32, kLevels = kMine * kThreads;
   __shared__ int s_level[kLevels];  // items of a level; then where its next one goes
   __shared__ int s_warp_sum[kWarps];
@@ -96,14 +118,13 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
   if (blockIdx.x > 0) {
     const unsigned first = (blockIdx.x - 1) * kWarps + warp, step = (gridDim.x - 1) * kWarps;
     for (unsigned i = first; i < static_cast<unsigned>(p.n) * p.n_maps && !bad; i += step) {
-      const int s = p.bwd ? i / kPackedBwdMaps : i / kPackedFwdMaps, m = i - s * p.n_maps;
+      constexpr int kMaps = BWD ? kPackedBwdMaps : kPackedFwdMaps;
+      const int s = i / kMaps, m = i - s * kMaps;
       const Seq q = load_seq(s);
       const int row = p.of_k[m] ? q.k0 : q.q0, rows = p.of_k[m] ? q.lk : q.lq;
       if (rows <= 0) continue;
-      const bool small = rows < p.long_rows[m];
-      const CUtensorMap* from = small ? &p.small[m] : &p.base[m];
-      if (is_narrow(p, q)) from = small ? &p.narrow_small[m] : &p.narrow_base[m];
-      s_map[warp][lane] = reinterpret_cast<const uint32_t*>(from)[lane];
+      const int kind = (rows < p.long_rows[m] ? 1 : 0) + (p.has_narrow[m] && is_narrow<BWD, NARROW>(p, q) ? 2 : 0);
+      s_map[warp][lane] = reinterpret_cast<const uint32_t*>(&maps.map[kind * kMaps + m])[lane];
       __syncwarp();
       if (lane == 0) {
         const uint32_t at = ptx::smem_u32(s_map[warp]);
@@ -141,16 +162,16 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
     return;
   }
   // (narrow items have a level of their own, below the others')
-  auto level_of = [&](const Seq& q, int steps) { return p.narrow == 0 ? steps >> p.shift : (is_narrow(p, q) ? 0 : (steps >> p.shift) + 1); };
+  auto level_of = [&](const Seq& q, int steps) { return !NARROW || BWD ? steps >> p.shift : (is_narrow<BWD, NARROW>(p, q) ? 0 : (steps >> p.shift) + 1); };
   // A thread to a short sequence, up to all of them to a long one.
   const int width = 1 << p.width_log, mine = tid >> p.width_log, teams = kThreads >> p.width_log, id = tid & (width - 1);
   int share = 0x7fffffff;  // no walk is longer
-  if (p.slots > 0) {
+  if (BWD && p.slots > 0) {
     unsigned long long steps = 0;
     for (int s = mine; s < p.n; s += teams) {
       const Seq q = load_seq(s);
-      const int n = items_of(p, q);
-      for (int i = id; i < n; i += width) steps += static_cast<unsigned>(walk_of(p, q, i) * p.group);
+      const int n = items_of<BWD, NARROW>(p, q);
+      for (int i = id; i < n; i += width) steps += static_cast<unsigned>(steps_of<BWD, NARROW>(p, q, i));
     }
     atomicAdd(&s_steps, steps);
     __syncthreads();
@@ -158,9 +179,9 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
   }
   for (int s = mine; s < p.n; s += teams) {
     const Seq q = load_seq(s);
-    const int n = items_of(p, q);
+    const int n = items_of<BWD, NARROW>(p, q);
     for (int i = id; i < n; i += width) {
-      const int steps = p.bwd ? walk_of(p, q, i) * p.group : walk_of(p, q, i), parts = parts_of(steps, share);
+      const int steps = steps_of<BWD, NARROW>(p, q, i), parts = BWD ? parts_of(steps, share) : 1;
       for (int k = 0; k < parts; ++k) atomicAdd(&s_level[level_of(q, part_from(steps, k + 1, parts) - part_from(steps, k, parts))], 1);
     }
   }
@@ -188,7 +209,7 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
       if (lane >= of) w += o;
     }
     if (lane < kWarps) s_warp_sum[lane] = w;
-    if (lane == 31) p.n_items[0] = w - (p.narrow > 0 ? s_level[0] : 0), p.n_items[2] = p.narrow > 0 ? s_level[0] : 0;
+    if (lane == 31) p.n_items[0] = w - (NARROW && !BWD ? s_level[0] : 0), p.n_items[2] = NARROW ? s_level[0] : 0;
   }
   __syncthreads();
   int place = upto - sum + (warp > 0 ? s_warp_sum[warp - 1] : 0);
@@ -201,9 +222,9 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
   __syncthreads();
   for (int s = mine; s < p.n; s += teams) {
     const Seq q = load_seq(s);
-    const int n = items_of(p, q);
+    const int n = items_of<BWD, NARROW>(p, q);
     for (int i = id; i < n; i += width) {
-      const int steps = p.bwd ? walk_of(p, q, i) * p.group : walk_of(p, q, i), parts = parts_of(steps, share);
+      const int steps = steps_of<BWD, NARROW>(p, q, i), parts = BWD ? parts_of(steps, share) : 1;
       int slot = -1;
       if (parts > 1) {
         slot = atomicAdd(&s_slots, parts);
@@ -213,8 +234,8 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const __grid_cons
         const int from = part_from(steps, k, parts), own = part_from(steps, k + 1, parts) - from;
         int4* e = reinterpret_cast<int4*>(p.items + atomicAdd(&s_level[level_of(q, own)], 1));
         e[0] = make_int4(q.q0, q.lq, q.k0, q.lk);
-        e[1] = make_int4(p.bwd ? i : i << p.step_log, s, from, own);
-        if (p.bwd) e[2] = make_int4(slot < 0 ? -1 : slot + k, 0, 0, 0);
+        e[1] = make_int4(BWD ? i : i << p.step_log, s, from, own);
+        if (BWD) e[2] = make_int4(slot < 0 ? -1 : slot + k, 0, 0, 0);
       }
     }
   }
@@ -238,18 +259,24 @@ bool same_kind(const CUtensorMap& a, const CUtensorMap& b) {
 
 }  // namespace
 
-bool packed_map(PackedPlan* p, int dtype, const void* ptr, int D, int rows, int H, const Str3& st, int box_rows, bool of_k, int narrow_heads) {
+bool packed_map(PackedPlan* p, PackedMaps* maps, int dtype, const void* ptr, int D, int rows, int H, const Str3& st, int box_rows, bool of_k, int narrow_heads) {
   const int m = p->n_maps++;
   const int64_t es = dtype == TT_ATTN_F32 ? 4 : 2;
+  const int whole_rows = box_rows;
+  int box_heads = 1;
   auto encode = [&](CUtensorMap* map, int n) {
-    return dtype == TT_ATTN_F32 ? make_map_f32(map, static_cast<const float*>(ptr), D, rows, H, 1, box_rows, n) : make_map(map, dtype, ptr, D, n, H, 1, st, box_rows);
+    return dtype == TT_ATTN_F32 ? make_map_f32(map, static_cast<const float*>(ptr), D, rows, H, 1, box_rows, n, box_heads)
+                                : make_map(map, dtype, ptr, D, n, H, 1, st, box_rows, 64, box_heads);
   };
   p->address[m] = static_cast<const char*>(ptr), p->row_bytes[m] = st.s * es, p->of_k[m] = of_k;
-  if (!encode(&p->base[m], rows) || !encode(&p->small[m], 1)) return false;
-  if (narrow_heads > 0 && (!make_map(&p->narrow_base[m], dtype, ptr, D, rows, H, 1, st, p->narrow, 64, narrow_heads) ||
-                           !make_map(&p->narrow_small[m], dtype, ptr, D, 1, H, 1, st, p->narrow, 64, narrow_heads)))
-    return false;
-  if (same_kind(p->base[m], p->small[m])) {
+  if (!encode(&maps->kind[0][m], rows) || !encode(&maps->kind[1][m], 1)) return false;
+  p->has_narrow[m] = p->narrow > 0 && narrow_heads > 0;
+  if (p->has_narrow[m]) {
+    box_rows = p->narrow, box_heads = narrow_heads;
+    if (!encode(&maps->kind[2][m], rows) || !encode(&maps->kind[3][m], 1)) return false;
+    box_rows = whole_rows, box_heads = 1;
+  }
+  if (same_kind(maps->kind[0][m], maps->kind[1][m])) {
     p->long_rows[m] = 1;
     return true;
   }
@@ -257,13 +284,13 @@ bool packed_map(PackedPlan* p, int dtype, const void* ptr, int D, int rows, int 
   const int64_t first = static_cast<int64_t>(H - 1) * st.h * es + D * es, more = (int64_t(128) << 10) - first;
   int64_t n = 1 + (more > 0 ? (more + st.s * es - 1) / (st.s * es) : 0);
   CUtensorMap at, below;
-  if (n < 2 || n > rows || !encode(&at, static_cast<int>(n)) || !encode(&below, static_cast<int>(n - 1)) || !same_kind(at, p->base[m]) ||
-      same_kind(below, p->base[m])) {
+  if (n < 2 || n > rows || !encode(&at, static_cast<int>(n)) || !encode(&below, static_cast<int>(n - 1)) || !same_kind(at, maps->kind[0][m]) ||
+      same_kind(below, maps->kind[0][m])) {
     int64_t lo = 1, hi = rows;
     while (hi - lo > 1) {
       const int64_t mid = (lo + hi) / 2;
       if (!encode(&at, static_cast<int>(mid))) return false;
-      (same_kind(at, p->base[m]) ? hi : lo) = mid;
+      (same_kind(at, maps->kind[0][m]) ? hi : lo) = mid;
     }
     n = hi;
   }
@@ -297,15 +324,14 @@ int packed_slots(int n, int total_q, int total_k, int Hq, int Hkv) {
   return few < most ? static_cast<int>(few) + 1 : most;
 }
 
-cudaError_t launch_packed_plan(PackedPlan p, void* scratch, PackedArgs* args, cudaStream_t stream) {
+cudaError_t launch_packed_plan(PackedPlan p, const PackedMaps& maps, void* scratch, PackedArgs* args, cudaStream_t stream) {
   char* at = static_cast<char*>(scratch);
   p.n_items = reinterpret_cast<int*>(at);
   p.items = reinterpret_cast<PackedEntry*>(at + 256);
   p.splits = reinterpret_cast<PackedSplit*>(at + 256 + items_bytes(p.n, p.total_q, p.total_k, p.group, p.bwd));
   p.maps = reinterpret_cast<CUtensorMap*>(reinterpret_cast<char*>(p.splits) + splits_bytes(p.bwd));
   p.per_group = ((uint64_t(1) << 40) + p.group - 1) / p.group;
-  // A large CTA sorts many items quickly, but each of its barriers takes longer: 677 rows of 5 sequences, 32/8 heads, 26 items: the plan
-  // 2.6 us with 256 threads.
+  // A large CTA sorts many items quickly, but each of its barriers takes longer.
   const size_t items = p.bwd ? packed_items(p.n, p.total_k, 1, 1) : packed_items(p.n, p.total_q, p.group, 1 << p.step_log);
   const int threads = items <= 512 && p.n <= 256 ? 256 : 1024, warps = threads / 32;
   // levels 0 ... the longest walk that there can be
@@ -317,10 +343,20 @@ cudaError_t launch_packed_plan(PackedPlan p, void* scratch, PackedArgs* args, cu
   p.width_log = 0;
   for (int width = 1; width < threads && (static_cast<size_t>(width) * p.n < items || 2ll * width * p.n <= threads); width *= 2) ++p.width_log;
   args->items = p.items, args->n_items = p.n_items, args->splits = p.splits, args->maps = p.maps;
-  const int64_t maps = static_cast<int64_t>(p.n) * p.n_maps + (p.total_q + p.total_k) / 64;  // a warp each, and one to 64 rows, which may have to be cleared
-  const int64_t most = 2 * kSms * (1024 / threads), ctas = (maps + warps - 1) / warps;
+  const int64_t tasks = static_cast<int64_t>(p.n) * p.n_maps + (p.total_q + p.total_k) / 64;  // a warp each, and one to 64 rows, which may have to be cleared
+  const int64_t most = 2 * kSms * (1024 / threads), ctas = (tasks + warps - 1) / warps;
   const dim3 grid(1 + static_cast<unsigned>(ctas < 1 ? 1 : (ctas < most ? ctas : most)));
-  return threads == 256 ? launch_early(packed_plan_kernel<256>, grid, dim3(256), 0, stream, 1, p) : launch_early(packed_plan_kernel<1024>, grid, dim3(1024), 0, stream, 1, p);
+  auto go = [&](auto bwd, auto narrow) {
+    constexpr bool BWD = decltype(bwd)::value, NARROW = decltype(narrow)::value;
+    MapSet<maps_of(BWD, NARROW)> set;
+    for (int i = 0; i < maps_of(BWD, NARROW); ++i) set.map[i] = maps.kind[i / p.n_maps][i % p.n_maps];
+    return threads == 256 ? launch_early(packed_plan_kernel<256, BWD, NARROW>, grid, dim3(256), 0, stream, 1, p, set)
+                          : launch_early(packed_plan_kernel<1024, BWD, NARROW>, grid, dim3(1024), 0, stream, 1, p, set);
+  };
+  using Yes = std::true_type;
+  using No = std::false_type;
+  if (p.bwd) return p.narrow > 0 ? go(Yes{}, Yes{}) : go(Yes{}, No{});
+  return p.narrow > 0 ? go(No{}, Yes{}) : go(No{}, No{});
 }
 
 }  // namespace ttattn

@@ -52,15 +52,15 @@ inline bool make_map_2d(CUtensorMap* m, int dtype, const void* ptr, int cols, in
   return make_map(m, dtype, ptr, cols, rows, 1, 1, Str3{ld * rows, ld * rows, ld}, box_rows, box_cols);
 }
 
-// Dense fp32 [B, H, S, D] buffer, or its first `rows` of S, box = 32 floats (128 bytes) x `box_rows` rows, for TMA reductions.
-inline bool make_map_f32(CUtensorMap* m, const float* ptr, int D, int S, int H, int B, int box_rows = 128, int rows = -1) {
+// Dense fp32 [B, H, S, D] buffer, or its first `rows` of S, box = 32 floats (128 bytes) x `box_rows` rows x `box_heads`, for TMA reductions.
+inline bool make_map_f32(CUtensorMap* m, const float* ptr, int D, int S, int H, int B, int box_rows = 128, int rows = -1, int box_heads = 1) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows < 0 ? S : rows), static_cast<cuuint64_t>(H),
                         static_cast<cuuint64_t>(B)};
   cuuint64_t strides[3] = {static_cast<cuuint64_t>(D) * 4, static_cast<cuuint64_t>(S) * D * 4,
                            static_cast<cuuint64_t>(H) * S * D * 4};
-  cuuint32_t box[4] = {32, static_cast<cuuint32_t>(box_rows), 1, 1};
+  cuuint32_t box[4] = {32, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(box_heads), 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, const_cast<float*>(ptr), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
