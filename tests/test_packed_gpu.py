@@ -423,6 +423,23 @@ def test_short_sequences_keep_to_themselves(poison):
         assert torch.equal(x[keep], y[keep])
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 2), (6, 2), (14, 2), (3, 3)])
+@pytest.mark.parametrize("causal", ["bottom-right", True, False])
+def test_few_new_rows_behind_many(D, Hq, Hkv, causal):
+    """Short queries over long keys: heads share tiles of queries that walk over many tiles of keys."""
+    from tinytorch_b200 import op
+
+    for lens, keys in (((20, 1, 32, 0, 9, 40, 3), (700, 129, 300, 50, 0, 500, 128)), ((60, 64, 1, 40, 33, 90, 5), (1000, 64, 257, 1, 384, 90, 70))):
+        q = make(sum(lens), Hq, D, torch.float16, 1)
+        k, v = (make(sum(keys), Hkv, D, torch.float16, i) for i in (2, 3))
+        cu, cu_k = offsets(lens), offsets(keys)
+        o, lse = op.sdpAttentionPackedFwd(q, k, v, cu, causal, cuSeqlensK=cu_k)
+        g = make(sum(lens), Hq, D, torch.float16, 4)
+        grads = op.sdpAttentionPackedBwd(g, q, k, v, o, lse, cu, causal, cuSeqlensK=cu_k)
+        check((o, lse, *grads), q, k, v, lens, causal, lens_k=keys, g=g)
+
+
 def test_offsets_changed_between_the_passes_are_an_error():
     from tinytorch_b200 import function
     q, k, v = (make(64, h, 64, torch.bfloat16, h).requires_grad_() for h in (4, 2, 2))

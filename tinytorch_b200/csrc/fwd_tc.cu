@@ -75,7 +75,7 @@ struct Item {
   int n_max;                   // the longer walk; -1: no more items
   int mask;                    // whether the mask has to be looked at
   int q0, lq, seq;             // packed: the sequence, its first row of q and how many
-  int narrow;                  // packed: the blocks are NARROW rows of several heads
+  int narrow;                  // packed: the blocks are NARROW rows of several heads (1: and the keys a tile of so many)
 };
 
 struct __align__(16) SmemCtl {
@@ -148,6 +148,7 @@ __device__ __forceinline__ Item decode_item(const FwdArgs& a, int w, int per_hea
     const int4* e = reinterpret_cast<const int4*>(a.packed.items + (per_head - 1 - mp));
     const int4 rows = __ldcg(e), place = __ldcg(e + 1);  // (the plan runs while this kernel is coming up)
     it.q0 = rows.x, it.lq = Lq = rows.y, kv_len = rows.w, first = place.x, it.seq = place.y;
+    if (NARROW > 0 && Lq <= NARROW && kv_len > 0) it.narrow = 2;
   } else if (a.kv_lens) {
     int l = a.kv_lens[it.b];
     kv_len = l < 0 ? 0 : (l < a.Skv ? l : a.Skv);
@@ -158,11 +159,12 @@ __device__ __forceinline__ Item decode_item(const FwdArgs& a, int w, int per_hea
   const int x = first, qt0 = x / group, qt1 = KEYS ? qt0 : (x + 1) / group;
   it.h[0] = it.hk * group + x - qt0 * group, it.h[1] = KEYS ? it.h[0] : it.hk * group + x + 1 - qt1 * group;
   it.row0[0] = qt0 * BM, it.row0[1] = qt1 * BM;
+  if (NARROW > 0 && it.narrow) it.h[0] = it.hk * group + first * a.packed.heads, it.h[1] = it.h[0] + a.packed.heads, it.row0[0] = 0, it.row0[1] = first + 1 < a.packed.blocks ? 0 : Lq;
   // key tiles that a block sees (0 for one wholly beyond Lq)
   auto tiles = [&](int row0) {
     int e = kv_len;
     if (a.causal) {
-      int c = row0 + BM + it.shift;
+      int c = row0 + (NARROW > 0 && it.narrow ? NARROW : BM) + it.shift;
       if (GEN) c = c > 0 ? c : 0;
       if (c < e) e = c;
     }
@@ -458,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mq = map_of(it.seq, kMapQ), mk = map_of(it.seq, kMapK), mv = map_of(it.seq, kMapV);
             ptx::tensormap_acquire(mq), ptx::tensormap_acquire(mk);  // (V's when Q and K are on their way)
           }
-          const uint32_t q_bytes = NARROW && it.narrow ? a.packed.heads * NARROW * D * 2 : TB, kv_bytes = NARROW && it.narrow ? NARROW * D * 2 : TB;
+          const uint32_t q_bytes = NARROW && it.narrow ? a.packed.heads * NARROW * D * 2 : TB, kv_bytes = NARROW && it.narrow == 1 ? NARROW * D * 2 : TB;
           bool ok = true;
           // a Q tile is loaded only if it has key tiles to walk; tile 0 goes first and, with the first K tile,
           // ahead of tile 1: the issuer starts tile 0 of this item while tile 1 of the previous one still works
@@ -588,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int slot = i & 1;
           if (!uwait(&ctl->item_full[slot], (i >> 1) & 1)) break;
           const int nt0 = ctl->item[slot].nt[0], nt1 = ctl->item[slot].nt[1], n_max = ctl->item[slot].n_max;
-          if constexpr (NARROW > 0) pv_keys = ctl->item[slot].narrow ? NARROW / 16 : BN / 16;
+          if constexpr (NARROW > 0) pv_keys = ctl->item[slot].narrow == 1 ? NARROW / 16 : BN / 16;
           __syncwarp();  // every lane has read the slot before it is handed back
           if (leader) ptx::mbar_arrive(&ctl->item_empty[slot]);
           if (n_max < 0) break;
@@ -722,7 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int b = pub->b, kv_len = pub->kv_len, shift = pub->shift, j0 = pub->j0, n_max = pub->n_max;
       const int n_t = pub->nt[t], tile_row0 = pub->row0[t], head = pub->h[t];
       const int q0 = PACKED ? pub->q0 : 0, lq = PACKED ? pub->lq : a.Lq;
-      const bool narrow = NARROW && pub->narrow;
+      const bool narrow = NARROW && pub->narrow, single = NARROW && pub->narrow == 1;
       const CUtensorMap* mo = &tmO;
       if constexpr (PACKED) mo = map_of(pub->seq, kMapO);
       const bool use_mask = GEN == 2 && pub->mask;
@@ -776,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m_ref = -INFINITY;  // reference max, in scaled log2 units
       float2 l2 = make_float2(0.f, 0.f);
       if constexpr (NARROW > 0) {
-        if (narrow) {
+        if (single) {
           // One tile, of which only the first NARROW columns are keys.
           ok = ptx::mbar_wait(&ctl->s_full[t], cnt & 1, abort_flag);
           ptx::tc_fence_after();
@@ -812,10 +814,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           ptx::mbar_arrive(&ctl->p_full[t]);
         }
       }
-      for (int j = 0; j < n_t && ok && !narrow; ++j) {
+      for (int j = 0; j < n_t && ok && !single; ++j) {
         ok = ptx::mbar_wait(&ctl->s_full[t], (cnt + j) & 1, abort_flag);
         if (!ok) break;
         ptx::tc_fence_after();
+        if (NARROW > 0 && !has) {  // (rows of no head)
+          ptx::tc_fence_before();
+          ptx::mbar_arrive(&ctl->p_full[t]);
+          continue;
+        }
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) ptx::tmem_ld32p(tS + cc * 32, s + cc * 32);
         ptx::tmem_wait_ld();
@@ -1212,8 +1219,9 @@ cudaError_t launch_packed(FwdArgs a, const PackedCall& c, int dtype, int device,
   // sequences, whose walks are short: 16.5, 17.5)
   const double est = (a.Lq / BM + 0.5 * c.n) * a.Hq;
   const bool keys = est <= 2.0 * sms && c.total_k >= 256ll * c.n;
-  // Short sequences, where the rows say that many are: a block is 32 rows of up to four heads of a group, or 64 of two, and so many keys (300 of 17 rows,
-  // D = 128: 32/8 heads 168 -> 57 us, 8/1 heads 55 -> 20, 16 heads of their own 141 -> 98).  Heads with keys of their own do not share tiles: an infinite
+  // Short sequences, where the rows say that many are: a block is 32 rows of up to four heads of a group, or 64 of two, and its keys, if they are as few, one
+  // narrow tile (300 of 17 rows, D = 128: 32/8 heads 168 -> 53 us, 8/1 heads 55 -> 18, 16 heads of their own 141 -> 94; 16 of 20 rows over 4000 keys,
+  // 32/8 heads: 121 -> 62).  Heads with keys of their own do not share tiles: an infinite
   // value of one would reach another as 0 x inf.
   const int narrow = keys || a.Lq > 64ll * c.n ? 0 : (a.Lq > 32ll * c.n ? 64 : 32);
   int heads = narrow > 0 ? BM / narrow : 1;

@@ -34,7 +34,12 @@ __device__ __forceinline__ int by_group(const PackedPlan& p, int x) { return sta
 // A sequence whose heads share tiles.
 template <bool BWD, bool NARROW>
 __device__ __forceinline__ bool is_narrow(const PackedPlan& p, const Seq& s) {
-  return NARROW && s.lq > 0 && s.lk > 0 && s.lq <= p.narrow && (BWD || s.lk <= p.narrow);
+  return NARROW && s.lq > 0 && s.lk > 0 && s.lq <= p.narrow;
+}
+// ... and whose keys are one narrow tile (forward).
+template <bool BWD, bool NARROW>
+__device__ __forceinline__ bool is_single(const PackedPlan& p, const Seq& s) {
+  return !BWD && is_narrow<BWD, NARROW>(p, s) && s.lk <= p.narrow;
 }
 // Items of a sequence, and the tiles that item i walks over.
 template <bool BWD, bool NARROW>
@@ -123,7 +128,7 @@ __global__ void __launch_bounds__(kThreads)
       const Seq q = load_seq(s);
       const int row = p.of_k[m] ? q.k0 : q.q0, rows = p.of_k[m] ? q.lk : q.lq;
       if (rows <= 0) continue;
-      const int kind = (rows < p.long_rows[m] ? 1 : 0) + (p.has_narrow[m] && is_narrow<BWD, NARROW>(p, q) ? 2 : 0);
+      const int kind = (rows < p.long_rows[m] ? 1 : 0) + (p.has_narrow[m] && (p.of_k[m] ? is_single<BWD, NARROW>(p, q) : is_narrow<BWD, NARROW>(p, q)) ? 2 : 0);
       s_map[warp][lane] = reinterpret_cast<const uint32_t*>(&maps.map[kind * kMaps + m])[lane];
       __syncwarp();
       if (lane == 0) {
@@ -161,8 +166,8 @@ __global__ void __launch_bounds__(kThreads)
     if (tid == 0 && p.status) atomicOr(p.status, kStatusBadOffsets);
     return;
   }
-  // (narrow items have a level of their own, below the others')
-  auto level_of = [&](const Seq& q, int steps) { return !NARROW || BWD ? steps >> p.shift : (is_narrow<BWD, NARROW>(p, q) ? 0 : (steps >> p.shift) + 1); };
+  // (items of one narrow tile have a level of their own, below the others')
+  auto level_of = [&](const Seq& q, int steps) { return !NARROW || BWD ? steps >> p.shift : (is_single<BWD, NARROW>(p, q) ? 0 : (steps >> p.shift) + 1); };
   // A thread to a short sequence, up to all of them to a long one.
   const int width = 1 << p.width_log, mine = tid >> p.width_log, teams = kThreads >> p.width_log, id = tid & (width - 1);
   int share = 0x7fffffff;  // no walk is longer
