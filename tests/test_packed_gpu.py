@@ -440,6 +440,30 @@ def test_few_new_rows_behind_many(D, Hq, Hkv, causal):
         check((o, lse, *grads), q, k, v, lens, causal, lens_k=keys, g=g)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_short_sequences_of_other_layouts(D):
+    """Parts of a projection's output, heads outside rows, gradients of any strides, no keys at all."""
+    from tinytorch_b200 import op
+
+    lens, Hq, Hkv = (20, 0, 31, 5, 32, 1), 8, 2
+    n = sum(lens)
+    qkv = make(n, Hq + 2 * Hkv, D, torch.bfloat16, 1)
+    q, k, v = qkv[:, :Hq], qkv[:, Hq:Hq + Hkv], qkv[:, Hq + Hkv:]
+    g = make(n, Hq, D, torch.bfloat16, 2)
+    want = op.sdpAttentionPackedFwd(q.contiguous(), k.contiguous(), v.contiguous(), offsets(lens), True)
+    back = op.sdpAttentionPackedBwd(g, q.contiguous(), k.contiguous(), v.contiguous(), *want, offsets(lens), True)
+    swap = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v, g)]
+    for a, b, c, d in ((q, k, v, g), swap):
+        o, lse = op.sdpAttentionPackedFwd(a, b, c, offsets(lens), True)
+        assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+        got = op.sdpAttentionPackedBwd(d, a, b, c, o, lse, offsets(lens), True)
+        assert torch.equal(got[1], back[1]) and torch.equal(got[2], back[2])
+        assert (got[0].float() - back[0].float()).abs().max() <= 2 ** -7 * back[0].float().abs().max()
+    none = torch.zeros(0, Hkv, D, dtype=torch.bfloat16, device="cuda")
+    o, lse = op.sdpAttentionPackedFwd(q, none, none, offsets(lens), True, cuSeqlensK=torch.zeros(7, dtype=torch.int32, device="cuda"))
+    assert not o.any() and bool((lse == -math.inf).all())
+
+
 def test_offsets_changed_between_the_passes_are_an_error():
     from tinytorch_b200 import function
     q, k, v = (make(64, h, 64, torch.bfloat16, h).requires_grad_() for h in (4, 2, 2))
