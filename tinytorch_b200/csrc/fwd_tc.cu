@@ -1089,10 +1089,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------ host ----
 template <int D, bool BF16, int GEN, bool KEYS, bool PACKED = false, int NARROW = 0>
-cudaError_t launch_k(const FwdArgs& a, int dtype, int grid, int cluster, cudaStream_t stream) {
+cudaError_t launch_k(const FwdArgs& a, int dtype, int grid, int cluster, cudaStream_t stream, const CUtensorMap* made = nullptr) {
   CUtensorMap tq, tk, tv, to;
-  if (!make_map(&tq, dtype, a.q, D, a.Lq, a.Hq, a.B, a.qs) || !make_map(&tk, dtype, a.k, D, a.Skv, a.Hkv, a.B, a.ks) ||
-      !make_map(&tv, dtype, a.v, D, a.Skv, a.Hkv, a.B, a.vs) || !make_map(&to, dtype, a.o, D, a.Lq, a.Hq, a.B, a.os))
+  if (PACKED)
+    tq = made[kMapQ], tk = made[kMapK], tv = made[kMapV], to = made[kMapO];
+  else if (!make_map(&tq, dtype, a.q, D, a.Lq, a.Hq, a.B, a.qs) || !make_map(&tk, dtype, a.k, D, a.Skv, a.Hkv, a.B, a.ks) ||
+           !make_map(&tv, dtype, a.v, D, a.Skv, a.Hkv, a.B, a.vs) || !make_map(&to, dtype, a.o, D, a.Lq, a.Hq, a.B, a.os))
     return cudaErrorInvalidValue;
   auto kern = fwd_tc_kernel<D, BF16, GEN, KEYS, PACKED, NARROW>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D, GEN>());
@@ -1243,9 +1245,10 @@ cudaError_t launch_packed(FwdArgs a, const PackedCall& c, int dtype, int device,
   cudaError_t e = launch_packed_plan(p, maps, c.scratch, &a.packed, stream);
   if (e != cudaSuccess) return e;
   const int grid = static_cast<int>(blocks < static_cast<size_t>(sms) ? blocks : sms);
-  if (narrow == 32) return launch_k<D, BF16, GEN, false, true, 32>(a, dtype, grid, 1, stream);
-  if (narrow == 64) return launch_k<D, BF16, GEN, false, true, 64>(a, dtype, grid, 1, stream);
-  return keys ? launch_k<D, BF16, GEN, true, true>(a, dtype, grid, 1, stream) : launch_k<D, BF16, GEN, false, true>(a, dtype, grid, 1, stream);
+  const CUtensorMap* made = maps.kind[0];
+  if (narrow == 32) return launch_k<D, BF16, GEN, false, true, 32>(a, dtype, grid, 1, stream, made);
+  if (narrow == 64) return launch_k<D, BF16, GEN, false, true, 64>(a, dtype, grid, 1, stream, made);
+  return keys ? launch_k<D, BF16, GEN, true, true>(a, dtype, grid, 1, stream, made) : launch_k<D, BF16, GEN, false, true>(a, dtype, grid, 1, stream, made);
 }
 
 }  // namespace

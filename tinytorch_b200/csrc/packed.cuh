@@ -48,6 +48,10 @@ struct PackedPlan {
 // What sequences' maps are made of: the maps of the whole tensors and of one row, and those two with narrow boxes.
 struct PackedMaps {
   CUtensorMap kind[4][kPackedBwdMaps];
+  struct Layout {  // of those whose long_rows the driver has been asked for
+    int rows, heads;
+    int64_t row_stride, head_stride;
+  } layout[kPackedBwdMaps] = {};
 };
 
 // A call over packed sequences.

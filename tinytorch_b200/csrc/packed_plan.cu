@@ -285,6 +285,12 @@ bool packed_map(PackedPlan* p, PackedMaps* maps, int dtype, const void* ptr, int
     p->long_rows[m] = 1;
     return true;
   }
+  for (int i = 0; i < m; ++i)  // (a tensor of the same layout has been looked at: V as K, O as Q)
+    if (dtype != TT_ATTN_F32 && maps->layout[i].rows == rows && maps->layout[i].heads == H && maps->layout[i].row_stride == st.s && maps->layout[i].head_stride == st.h) {
+      p->long_rows[m] = p->long_rows[i];
+      return true;
+    }
+  if (dtype != TT_ATTN_F32) maps->layout[m] = PackedMaps::Layout{rows, H, st.s, st.h};
   // The fewest rows that count as long: those that reach over 128 KB; should a driver see it otherwise, they are searched for.
   const int64_t first = static_cast<int64_t>(H - 1) * st.h * es + D * es, more = (int64_t(128) << 10) - first;
   int64_t n = 1 + (more > 0 ? (more + st.s * es - 1) / (st.s * es) : 0);
