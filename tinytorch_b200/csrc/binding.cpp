@@ -123,10 +123,17 @@ const Tensor& tensor_of(PyObject* o, const char* name) {
 }
 Tensor optional_of(PyObject* o, const char* name) { return o == Py_None ? Tensor() : tensor_of(o, name); }
 
+// Rows that share memory: all strides of a tensor that is expanded in every dimension but the last are 0, which the C ABI takes for
+// a dense tensor, whose memory there is not.
+void check_rows(const Tensor& t, const char* name, int64_t dim) {
+  if (t.size(dim) > 1 && t.stride(dim) == 0) raise(PyExc_ValueError, "%s: rows must have their own memory (an expanded tensor needs contiguous())", name);
+}
+
 void check_attn_tensor(const Tensor& t, const char* name) {
   if (!t.is_cuda()) raise(PyExc_ValueError, "%s must be a CUDA tensor (this op has no CPU path)", name);
   if (t.dim() != 4) raise(PyExc_ValueError, "%s must be [B, H, S, D]", name);
   if (t.stride(3) != 1) raise(PyExc_ValueError, "%s: innermost dimension must be contiguous", name);
+  check_rows(t, name, 2);
   if (dtype_of(t.scalar_type()) < 0) raise(PyExc_ValueError, "%s: dtype %s not supported", name, c10::toString(t.scalar_type()));
 }
 
@@ -138,6 +145,7 @@ void check_operand(const Tensor& t, const char* name, const Tensor& q, int64_t B
   if (t.size(0) < B || t.size(1) < H || t.size(2) < S || t.size(3) < q.size(3))
     raise(PyExc_ValueError, "%s is smaller than [%lld, %lld, %lld, %lld], which q and the keys ask for", name, (long long)B,
           (long long)H, (long long)S, (long long)q.size(3));
+  check_rows(t, name, 2);
 }
 // `grads`: gradients of the same shapes are to be written, every element of them
 void check_kv(const Tensor& q, const Tensor& k, const Tensor& v, bool grads) {
@@ -147,7 +155,21 @@ void check_kv(const Tensor& q, const Tensor& k, const Tensor& v, bool grads) {
     raise(PyExc_ValueError, "gradients need k and v of one shape, with the batch and head dimension of q");
 }
 
-tt_attn_strides strides_of(const Tensor& t) { return {t.stride(0), t.stride(1), t.stride(2)}; }
+// Strides for a kernel that reads 16 bytes at a time; of a dimension of one element any (torch leaves anything there).
+int64_t stride_or(const Tensor& t, int64_t dim, int64_t any) { return t.size(dim) > 1 ? t.stride(dim) : any; }
+tt_attn_strides strides_of(const Tensor& t) {  // [B, H, S, D]
+  const int64_t D = t.size(3);
+  return {stride_or(t, 0, D), stride_or(t, 1, D), stride_or(t, 2, D)};
+}
+bool vector_aligned(const Tensor& t) {
+  const int64_t es = t.element_size();
+  if (t.stride(-1) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d)
+    if (t.size(d) > 1 && (t.stride(d) <= 0 || t.stride(d) * es % 16)) return false;
+  return true;
+}
+// A gradient may be a part of a larger one, or one value expanded: any strides and offset.  It is copied where a kernel cannot read it.
+Tensor readable(const Tensor& t) { return t.numel() == 0 || vector_aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
 Tensor empty(at::IntArrayRef sizes, at::ScalarType dt, const at::Device& dev) {
   return Tensor(at::detail::empty_cuda(sizes, dt, dev, c10::nullopt));
@@ -288,6 +310,7 @@ BwdResult attn_bwd(const Tensor& dO, const Tensor& q, const Tensor& k, const Ten
 }
 
 void check_bwd(const Tensor& dO, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse) {
+  check_rows(q, "q", 2);
   check_kv(q, k, v, true);
   check_operand(dO, "dO", q, q.size(0), q.size(1), q.size(2));
   check_operand(o, "o", q, q.size(0), q.size(1), q.size(2));
@@ -317,7 +340,7 @@ struct AttentionBackward : public torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     at::NoGradGuard no_grad;
     const Tensor qt = q.unpack(), kt = k.unpack(), vt = v.unpack(), ot = o.unpack(shared_from_this()), lt = lse.unpack();
-    if (dO.stride(3) != 1) dO = dO.contiguous();
+    dO = readable(dO);
     check_bwd(dO, qt, kt, vt, ot, lt);
     const bool needs[3] = {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2)};
     BwdResult r = attn_bwd(dO, qt, kt, vt, ot, lt, mode, scale, kv_lens, needs, mask);
@@ -470,22 +493,10 @@ Tensor linear_autograd(const Tensor& x, const Tensor& w, const Tensor& bias) {
 }
 
 // ------------------------------------------------------------------------------------------- packed sequences --
-// Strides of an operand of three or four dimensions for a kernel that reads 16 bytes at a time: those of the rows and heads, of a
-// dimension of one element any (torch leaves anything there).
-int64_t stride_or(const Tensor& t, int64_t dim, int64_t any) { return t.size(dim) > 1 ? t.stride(dim) : any; }
 tt_attn_strides packed_strides_of(const Tensor& t) {  // [rows, heads, D]
   const int64_t D = t.size(2);
   return {0, stride_or(t, 1, D), stride_or(t, 0, t.size(1) * D)};
 }
-bool vector_aligned(const Tensor& t) {
-  const int64_t es = t.element_size();
-  if (t.stride(-1) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
-  for (int64_t d = 0; d + 1 < t.dim(); ++d)
-    if (t.size(d) > 1 && (t.stride(d) <= 0 || t.stride(d) * es % 16)) return false;
-  return true;
-}
-// A gradient may be a part of a larger one, or one value expanded: any strides and offset.  It is copied where a kernel cannot read it.
-Tensor readable(const Tensor& t) { return t.numel() == 0 || vector_aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
 void check_packed_tensor(const Tensor& t, const char* name, const Tensor& q) {
   if (!t.is_cuda()) raise(PyExc_ValueError, "%s must be a CUDA tensor (this op has no CPU path)", name);
@@ -495,6 +506,7 @@ void check_packed_tensor(const Tensor& t, const char* name, const Tensor& q) {
   if (t.scalar_type() != q.scalar_type() || t.device() != q.device()) raise(PyExc_ValueError, "%s must have the dtype and device of q", name);
   if (t.size(2) != q.size(2)) raise(PyExc_ValueError, "%s must have the head dimension of q", name);
   if (t.numel() > 0 && t.stride(2) != 1) raise(PyExc_ValueError, "%s: innermost dimension must be contiguous", name);
+  check_rows(t, name, 0);
 }
 void check_offsets(const Tensor& cu, const char* name, const Tensor& q) {
   if (cu.dim() != 1 || cu.size(0) < 2) raise(PyExc_ValueError, "%s must be [sequences + 1], with one sequence or more", name);
@@ -617,8 +629,7 @@ Dims dims_of(const Tensor& t) {
 }
 tt_attn_strides head_strides_of(const Tensor& t) {
   if (t.dim() == 3) return {t.size(0) * t.size(1) * t.size(2), stride_or(t, 1, t.size(2)), stride_or(t, 0, t.size(1) * t.size(2))};
-  const int64_t D = t.size(3);
-  return {stride_or(t, 0, D), stride_or(t, 1, D), stride_or(t, 2, D)};
+  return strides_of(t);
 }
 // Dense, heads inside rows or rows inside heads as in `t`: attention and the next projection read it as they would have read `t`.
 Tensor empty_ordered(const Tensor& t) {
@@ -691,8 +702,10 @@ struct Pair {
 };
 Pair norm_rope_fwd(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Rope& r, const Tensor& status) {
   Pair out{empty_ordered(q), empty_ordered(k)};
+  at::NoGradGuard no_grad;
+  const Tensor x = readable(q), y = readable(k);
   tt_qk_norm_rope_params p{};
-  set_norm_rope(&p, q, k, qw, kw, r);
+  set_norm_rope(&p, x, y, qw, kw, r);
   p.q_out = out.q.data_ptr(), p.k_out = out.k.data_ptr();
   p.q_out_strides = head_strides_of(out.q), p.k_out_strides = head_strides_of(out.k);
   p.status = ints_ptr(status);
@@ -710,10 +723,10 @@ NormRopeGrads norm_rope_bwd(const Tensor& gq, const Tensor& gk, const Tensor& q,
   if (needs[1]) out.g[1] = empty_ordered(k);
   for (int i = 2; i < 4; ++i)
     if (needs[i]) out.g[i] = empty({q.size(-1)}, q.scalar_type(), q.device());
-  const Tensor a = readable(gq), b = readable(gk);
+  const Tensor a = readable(gq), b = readable(gk), x = readable(q), y = readable(k);
   tt_qk_norm_rope_bwd_params p{};
   p.struct_size = sizeof(p);
-  set_norm_rope(&p.fwd, q, k, qw, kw, r);
+  set_norm_rope(&p.fwd, x, y, qw, kw, r);
   if (needs[0]) p.fwd.q_out = out.g[0].data_ptr(), p.fwd.q_out_strides = head_strides_of(out.g[0]);
   if (needs[1]) p.fwd.k_out = out.g[1].data_ptr(), p.fwd.k_out_strides = head_strides_of(out.g[1]);
   p.dq_out = a.data_ptr(), p.dk_out = b.data_ptr();

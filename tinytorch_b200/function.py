@@ -43,7 +43,7 @@ class FuncSDPAttention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         query, key, value, o, lse = ctx.saved_tensors
-        if grad.stride(3) != 1:
+        if grad.stride(3) != 1 or grad.size(2) > 1 and grad.stride(2) == 0:  # (one value, or one row, expanded)
             grad = grad.contiguous()
         dq, dk, dv = op.sdpAttentionBwd(grad, query, key, value, o, lse, ctx.isCausal, ctx.scale, ctx.kvLens,
                                         needs=ctx.needs_input_grad[:3], attnMask=ctx.attnMask)

@@ -55,8 +55,8 @@ def qkNormRope(q, k, qWeight=None, kWeight=None, cos=None, sin=None, positions=N
                status=None):
     """The RMS norm of every head of q and k, times a weight [D], and the rotation to the rows' positions -> (q', k').
 
-    q [B, Hq, S, D] and k [B, Hkv, S, D], or packed rows [T, Hq, D] and [T, Hkv, D], with any strides (parts of the projection's
-    output, say); the results are dense in the same order.  Without a weight an operand is not normalised.  cos, sin: fp32
+    q [B, Hq, S, D] and k [B, Hkv, S, D], or packed rows [T, Hq, D] and [T, Hkv, D], channels contiguous, with any other strides
+    (parts of the projection's output, say; an operand whose rows do not start on 16 bytes, or share memory, is copied first); the results are dense in the same order.  Without a weight an operand is not normalised.  cos, sin: fp32
     tables [positions, D/2] as op.ropeTables makes them, or None for no rotation; positions: int32 [S] or [B, S] ([T]
     for packed rows).  Pairs are the channels (i, i + D/2), or (2i, 2i + 1) if interleaved.  Positions of several axes (time, height,
     width): positions [axes, ...] and sections, how many of the D/2 pairs belong to each axis, in order.  A position outside the
