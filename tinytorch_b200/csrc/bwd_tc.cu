@@ -176,25 +176,17 @@ __device__ __forceinline__ void p_chunk(const BwdArgs& a, uint32_t (&s)[16], con
     for (int i = 0; i < 16; ++i)
       if (i < n_hidden) s[i] = 0xff800000u;  // -inf
   }
+  // (one exponential in eight on the FMA pipe: the compute warps saturate the MUFU units in this phase)
+  const float2 on_fma = ptx::ex2_fma2<true>(make_float2(__uint_as_float(s[7]), __uint_as_float(s[15])));
 #pragma unroll
   for (int i = 0; i < 16; i += 4) {
-    // (one exponential in eight on the FMA pipe: the compute warps saturate the MUFU units in this phase)
     const float p0 = ptx::ex2(__uint_as_float(s[i])), p1 = ptx::ex2(__uint_as_float(s[i + 1]));
     const float p2 = ptx::ex2(__uint_as_float(s[i + 2]));
-    const float p3 = (i & 4) ? ptx::ex2_fma(__uint_as_float(s[i + 3])) : ptx::ex2(__uint_as_float(s[i + 3]));
+    const float p3 = i == 4 ? on_fma.x : (i == 12 ? on_fma.y : ptx::ex2(__uint_as_float(s[i + 3])));
     s[i] = __float_as_uint(p0), s[i + 1] = __float_as_uint(p1);
     s[i + 2] = __float_as_uint(p2), s[i + 3] = __float_as_uint(p3);
     pk[(i >> 1) + 0] = pack2<BF16>(p0, p1);
     pk[(i >> 1) + 1] = pack2<BF16>(p2, p3);
-  }
-  // (the FMA-pipe exponential of -inf is a denormal, not 0: a hidden pair must leave nothing behind)
-  if (n_hidden > 7) {
-    s[7] = 0u;
-    pk[3] = pack2<BF16>(__uint_as_float(s[6]), 0.f);
-    if (n_hidden > 15) {
-      s[15] = 0u;
-      pk[7] = pack2<BF16>(__uint_as_float(s[14]), 0.f);
-    }
   }
 }
 

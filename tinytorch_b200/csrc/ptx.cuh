@@ -517,6 +517,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// ... NaN if one of them is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 // One lane of a converged warp.  A loop that issues tcgen05.mma is run by the whole warp with only the
 // instruction itself under this predicate: addresses and descriptors then stay warp-uniform (uniform registers and
@@ -569,18 +575,27 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// 2^x on the FMA and integer pipes (no MUFU): x = n + f with n = round(x), f in [-0.5, 0.5]; a cubic for 2^f
-// (maximum relative error 7.5e-5, below half a unit in the last place of fp16 and bf16) and n added to the exponent
-// field.  Arguments below -126 (-inf included) give a value below 2^-125; NaN gives that too.  For kernels whose
+// 2^x of a pair on the FMA and integer pipes (no MUFU): x = n + f with n = round(x), f in [-0.5, 0.5]; a cubic for 2^f
+// (maximum relative error 7.5e-5, below half a unit in the last place of fp16 and bf16) times 2^n, whose bits are n + 127
+// in the exponent field.  0 below -126.5 (-inf included).  ANY: as ex2 at the other end, too, infinite above 127.5 and NaN for NaN;
+// without it whoever calls looks for arguments above 127 and NaN, which give anything.  For kernels whose
 // exponentials are bound by the four MUFU units of an SM sub-partition: a share of them goes here.
-__device__ __forceinline__ float ex2_fma(float x) {
-  x = fmaxf(x, -126.f);
-  const float magic = 12582912.f;  // 1.5 * 2^23: the sum holds round(x) in its low mantissa bits
-  const float xr = x + magic;
-  const float f = x - (xr - magic);
-  const float p = fmaf(fmaf(fmaf(0.055171750485897064f, f, 0.24261131882667542f), f, 0.6932609677314758f), f,
-                       0.9999280571937561f);
-  return __int_as_float(__float_as_int(p) + (__float_as_int(xr) << 23));
+template <bool ANY>
+__device__ __forceinline__ float2 ex2_fma2(float2 x) {
+  if constexpr (ANY) {
+    asm("max.NaN.f32 %0, %0, %2;\n\tmax.NaN.f32 %1, %1, %2;" : "+f"(x.x), "+f"(x.y) : "f"(-127.f));
+    asm("min.NaN.f32 %0, %0, %2;\n\tmin.NaN.f32 %1, %1, %2;" : "+f"(x.x), "+f"(x.y) : "f"(128.f));
+  } else {
+    x.x = fmaxf(x.x, -127.f), x.y = fmaxf(x.y, -127.f);
+  }
+  auto both = [](float c) { return make_float2(c, c); };
+  constexpr float magic = 12582912.f;  // 1.5 * 2^23: the sum holds round(x) in its low mantissa bits
+  const float2 xr = add2(x, both(magic));
+  const float2 f = fma2(add2(xr, both(-magic)), both(-1.f), x);
+  const float2 p = fma2(fma2(fma2(both(0.055171750485897064f), f, both(0.24261131882667542f)), f, both(0.6932609677314758f)), f,
+                        both(0.9999280571937561f));
+  auto power = [](float r) { return __uint_as_float((__float_as_uint(r) << 23) + 0x3f800000u); };
+  return mul2(p, make_float2(power(xr.x), power(xr.y)));
 }
 
 }  // namespace ptx
