@@ -24,6 +24,11 @@ constexpr int kStatusCacheFull = 4;      // no free row in the cache of some seq
 constexpr int kStatusRopeRange = 8;      // position beyond the rotary tables
 constexpr int kStatusBadOffsets = 16;    // packed sequences: offsets that fall or leave the rows; cacheAccept: a draft that does not exist
 
+// Of a row's maximum m (to the base 2) and sum l of exponentials.  A row without a key has the sum 0, exactly, and gives O = 0 and LSE = -inf; the sum of a
+// row with a score that is NaN or +inf is NaN, and so are O and LSE (m may be -inf: maxima pass over NaN).
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
+__device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2; }
+
 // two values, rounded to the 16-bit type, in one register
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {

@@ -336,17 +336,17 @@ __device__ __forceinline__ void combine_rows(const FwdArgs& a, const Item& it, i
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int r = 0; r < CS; ++r) {
-        if (ml[u][r].x == -INFINITY) continue;  // (a CTA without key tiles for the row left no O)
+        if (ml[u][r].y == 0.f) continue;  // (a CTA without keys for the row)
         const float w = ptx::ex2(ml[u][r].x - m);
         l = fmaf(ml[u][r].y, w, l);
         v.x = fmaf(x[u][r].x, w, v.x), v.y = fmaf(x[u][r].y, w, v.y), v.z = fmaf(x[u][r].z, w, v.z), v.w = fmaf(x[u][r].w, w, v.w);
       }
       if (row >= a.Lq) continue;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = inverse_sum(l);
       *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.o) + it.b * a.os.b + head * a.os.h + static_cast<int64_t>(row) * a.os.s +
                                 c4 * 4) = make_uint2(pack2<BF16>(v.x * inv, v.y * inv), pack2<BF16>(v.z * inv, v.w * inv));
       if (a.lse && c4 == 0)
-        a.lse[(static_cast<int64_t>(it.b) * a.Hq + head) * a.Lq + row] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        a.lse[(static_cast<int64_t>(it.b) * a.Hq + head) * a.Lq + row] = row_lse(m, l);
     }
   }
 }
@@ -974,7 +974,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (r_in == 0) ptx::bulk_wait_read();  // previous store out of this block has been read
             ptx::named_barrier(1 + t, BM);
           }
-          const float inv = cluster > 1 ? 1.f : (l > 0.f ? 1.f / l : 0.f);
+          const float inv = cluster > 1 ? 1.f : inverse_sum(l);
           const float ua = wa * inv, ub = wb * inv;
           const uint32_t ta = tmem + 256 + lane_addr + c0;
 #pragma unroll 1
@@ -985,7 +985,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
               const float x = nt0 > 0 ? __uint_as_float(s[e]) * ua : 0.f;
-              s[e] = __float_as_uint(nt1 > 0 ? fmaf(__uint_as_float(s[32 + e]), ub, x) : x);
+              const float y = nt1 > 0 ? fmaf(__uint_as_float(s[32 + e]), ub, x) : x;
+              s[e] = GEN && l == 0.f ? 0u : __float_as_uint(y);  // (no key: 0, whatever the values are)
             }
             if (cluster == 1) {
 #pragma unroll
@@ -1021,7 +1022,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ptx::bulk_commit();
           }
         }
-        if (t == 0 && row < lq && lse_row) *lse_row = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        if (t == 0 && row < lq && lse_row) *lse_row = row_lse(m, l);
         continue;
       }
 
@@ -1034,10 +1035,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int cc = 0; cc < D / 32; ++cc) ptx::tmem_ld32p(tO + cc * 32, s + cc * 32);
       ptx::tmem_wait_ld();
-      // (a row without a key: D = 64's exponentials on the FMA pipe have left denormals in its sum and in O)
-      const float l = GEN && m_ref == -INFINITY ? 0.f : l2.x + l2.y;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      if (GEN && !(l > 0.f)) {
+      const float l = l2.x + l2.y, inv = inverse_sum(l);
+      if (GEN && l == 0.f) {  // (no key: 0, whatever the values are)
 #pragma unroll
         for (int e = 0; e < D; ++e) s[e] = 0;
       }
@@ -1066,7 +1065,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ptx::bulk_commit();
         }
       }
-      if (ok && row < lq && has && lse_row) *lse_row = l > 0.f ? (m_ref + log2f(l)) * kLn2 : -INFINITY;
+      if (ok && row < lq && has && lse_row) *lse_row = row_lse(m_ref, l);
     }
     if (r_in == 0) ptx::bulk_wait_all();
   }
