@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_f32_kernel(const TreeArgs a)
         if (s.piece >= 0) {
           *reinterpret_cast<float4*>(part + c4 * (kTreeRows * 4) + r * 4) = acc[i];
         } else {
-          const float l = sL[r], inv = l > 0.f ? 1.f / l : 0.f;
+          const float inv = inverse_sum(sL[r]);
           *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.o) + s.b * a.os.b + (s.hk * group + r % group) * a.os.h +
                                      static_cast<int64_t>(draft0 + r / group) * a.os.s + c4 * 4) =
               make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
@@ -214,9 +214,9 @@ __global__ void __launch_bounds__(kThreads, 2) tree_f32_kernel(const TreeArgs a)
     if (tid < rows) {
       const float l = sL[tid], m = sM[tid];
       if (s.piece >= 0)
-        *reinterpret_cast<float2*>(part + kTreeRows * D + tid * 2) = make_float2(l > 0.f ? m : -INFINITY, l);
+        *reinterpret_cast<float2*>(part + kTreeRows * D + tid * 2) = make_float2(l == 0.f ? -INFINITY : m, l);
       else if (a.lse)
-        a.lse[(static_cast<int64_t>(s.b) * a.Hq + s.hk * group + tid % group) * a.T + draft0 + tid / group] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        a.lse[(static_cast<int64_t>(s.b) * a.Hq + s.hk * group + tid % group) * a.T + draft0 + tid / group] = row_lse(m, l);
     }
   }
   ptx::cp_async_wait();
@@ -258,13 +258,13 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a) {
     l *= alpha, o.x *= alpha, o.y *= alpha, o.z *= alpha, o.w *= alpha, m = top;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      if (ml[i].x == -INFINITY) continue;  // (no piece, or one that has seen no key)
+      if (ml[i].y == 0.f) continue;  // (no piece, or one that has seen no key)
       const float f = ptx::ex2(ml[i].x - m);
       l = fmaf(ml[i].y, f, l);
       o.x = fmaf(x[i].x, f, o.x), o.y = fmaf(x[i].y, f, o.y), o.z = fmaf(x[i].z, f, o.z), o.w = fmaf(x[i].w, f, o.w);
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = inverse_sum(l);
   const int head = w.z * group + r % group, draft = draft0 + r / group;
   T* dst = reinterpret_cast<T*>(a.o) + w.y * a.os.b + head * a.os.h + static_cast<int64_t>(draft) * a.os.s + c4 * 4;
   if constexpr (std::is_same_v<T, float>) {
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeArgs a) {
     constexpr bool BF = std::is_same_v<T, __nv_bfloat16>;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<BF>(o.x * inv, o.y * inv), pack2<BF>(o.z * inv, o.w * inv));
   }
-  if (a.lse && c4 == 0) a.lse[(static_cast<int64_t>(w.y) * a.Hq + head) * a.T + draft] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+  if (a.lse && c4 == 0) a.lse[(static_cast<int64_t>(w.y) * a.Hq + head) * a.T + draft] = row_lse(m, l);
 }
 
 constexpr size_t round256(size_t n) { return (n + 255) & ~size_t(255); }

@@ -388,7 +388,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::tc_fence_before();
       if (ptx::named_barrier_or(3, kSoft, !ok)) break;
       if (puts && mine) {
-        // over the copies and halves of the row; one that has seen no key for it holds zeros, or nothing at all, and takes no part
+        // over the copies and halves of the row; one that has seen no key for it holds zeros, or nothing at all, and takes no part (weight 0; a NaN sum
+        // counts whatever its weight is)
         float m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * R; ++i) m = fmaxf(m, s_stat[i * kLanes + row].x);
@@ -398,19 +399,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float2 x = s_stat[i * kLanes + row];
           l = fmaf(x.y, weight(x.x), l);
         }
-        const float inv = g.piece >= 0 ? 1.f : (l > 0.f ? 1.f / l : 0.f);
+        const float inv = g.piece >= 0 ? 1.f : inverse_sum(l);
         const float ua = weight(s_stat[r].x) * inv, ub = weight(s_stat[BM + r].x) * inv;
 #pragma unroll
         for (int e = 0; e < 64; ++e) {
-          float x = ua > 0.f ? __uint_as_float(s[e]) * ua : 0.f;
-          if (two && ub > 0.f) x = fmaf(__uint_as_float(s[64 + e]), ub, x);
+          float x = ua != 0.f ? __uint_as_float(s[e]) * ua : 0.f;
+          if (two && ub != 0.f) x = fmaf(__uint_as_float(s[64 + e]), ub, x);
           s[e] = __float_as_uint(x);
         }
         if (t == 0 && copy == 0) {
           if (g.piece >= 0)
-            *reinterpret_cast<float2*>(part_of(g) + kTreeRows * D + row * 2) = make_float2(l > 0.f ? m : -INFINITY, l);
+            *reinterpret_cast<float2*>(part_of(g) + kTreeRows * D + row * 2) = make_float2(l == 0.f ? -INFINITY : m, l);
           else if (a.lse)
-            a.lse[(static_cast<int64_t>(g.b) * a.Hq + head) * a.T + draft] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+            a.lse[(static_cast<int64_t>(g.b) * a.Hq + head) * a.T + draft] = row_lse(m, l);
         }
       }
       if constexpr (R > 1) {
