@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(kThreads, G == 1 ? 3 : 1) decode_kernel(const 
   const int end = min(len, begin + a.chunk);
   if (begin >= end && split > 0) return;  // (the combine kernel reads the splits that have rows, and the first)
   const float c = a.scale * kLog2e;
+  const int stop = c == c ? end : begin;  // (with a scale that is not a number no key takes part)
 
   for (int g0 = 0; g0 < group; g0 += G) {
     const int h0 = hk * group + g0;
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, G == 1 ? 3 : 1) decode_kernel(const 
     }
 
     // warp w takes rows begin + (it*kWarps + w)*UNR*KPW + u*KPW + sub
-    for (int base = begin + warp * UNR * KPW; base < end; base += kWarps * UNR * KPW) {
+    for (int base = begin + warp * UNR * KPW; base < stop; base += kWarps * UNR * KPW) {
       uint4 kw[UNR], vw[UNR];
       bool valid[UNR];
 #pragma unroll
@@ -228,7 +229,11 @@ __global__ void __launch_bounds__(kThreads, G == 1 ? 3 : 1) decode_kernel(const 
         float mx = m[g];
 #pragma unroll
         for (int u = 0; u < UNR; ++u) mx = fmaxf(mx, s[g][u]);
-        if (mx == -INFINITY) continue;  // nothing valid for this lane group yet
+        if (mx == -INFINITY) {  // nothing valid for this lane group yet (maxima pass over NaN, which stays)
+#pragma unroll
+          for (int u = 0; u < UNR; ++u) s[g][u] = s[g][u] == -INFINITY ? 0.f : s[g][u];
+          continue;
+        }
         const float alpha = exp2f(m[g] - mx);
         m[g] = mx;
         l[g] *= alpha;
@@ -243,10 +248,9 @@ __global__ void __launch_bounds__(kThreads, G == 1 ? 3 : 1) decode_kernel(const 
         Vec16<T>::unpack(vw[u], vf);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const float p = (m[g] == -INFINITY) ? 0.f : s[g][u];
-          l[g] += p;
+          l[g] += s[g][u];
 #pragma unroll
-          for (int i = 0; i < N; ++i) acc[g][i] = fmaf(p, vf[i], acc[g][i]);
+          for (int i = 0; i < N; ++i) acc[g][i] = fmaf(s[g][u], vf[i], acc[g][i]);
         }
       }
     }
@@ -295,9 +299,9 @@ __global__ void __launch_bounds__(kThreads, G == 1 ? 3 : 1) decode_kernel(const 
       }
       const int h = h0 + g;
       if (a.nsplit == 1) {
-        const float inv = lt > 0.f ? 1.f / lt : 0.f;
+        const float inv = inverse_sum(lt);
         reinterpret_cast<T*>(a.o)[b * a.os.b + h * a.os.h + d] = from_f32<T>(at * inv);
-        if (a.lse && d == 0) a.lse[static_cast<int64_t>(b) * a.Hq + h] = lt > 0.f ? (mn + log2f(lt)) * kLn2 : -INFINITY;
+        if (a.lse && d == 0) a.lse[static_cast<int64_t>(b) * a.Hq + h] = row_lse(mn, lt);
       } else {
         float* pp = a.partial + ((static_cast<int64_t>(b) * a.Hq + h) * a.nsplit + split) * (D + 2);
         pp[d] = at;
@@ -360,7 +364,7 @@ __global__ void __launch_bounds__(256) decode_combine_kernel(const DecodeArgs a)
     }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, o);
-    if (tid == 0) s_inv = lt > 0.f ? 1.f / lt : 0.f, s_lse = lt > 0.f ? (mn + log2f(lt)) * kLn2 : -INFINITY;
+    if (tid == 0) s_inv = inverse_sum(lt), s_lse = row_lse(mn, lt);
   }
   __syncthreads();
   float at = 0.f;

@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, OCC)
             const float la = ctl->xsum[0][0][h] + ctl->xsum[0][1][h] + ctl->xsum[0][2][h] + ctl->xsum[0][3][h];
             const float ma = done > 0 ? m[h] : -INFINITY, mbv = mbr[h], lbv = lbr[h];
             const float mn = fmaxf(ma, mbv);
-            // a side without tiles (or without valid keys) has maximum -inf and takes no part
+            // a side without tiles (or without valid keys) has maximum -inf and takes no part (a sum that is NaN counts whatever its weight is)
             const float wa = ma == -INFINITY ? 0.f : ptx::ex2(ma - mn), wb = mbv == -INFINITY ? 0.f : ptx::ex2(mbv - mn);
             const float lt = la * wa + lbv * wb;
             float oh = (wa > 0.f ? __uint_as_float(oa[h]) * wa : 0.f) + (wb > 0.f ? __uint_as_float(ob[h]) * wb : 0.f);
@@ -537,14 +537,14 @@ __global__ void __launch_bounds__(kThreads, OCC)
             if (r < D && h < group && ok) {  // D = 64: lanes 64-127 hold copies; heads beyond the group are padding
               // (nothing is stored after an expired wait: the status word reports it)
               if (a.nsplit == 1) {
-                const float inv = lt > 0.f ? 1.f / lt : 0.f;
+                const float inv = inverse_sum(lt);
                 reinterpret_cast<T*>(a.o)[it.b * a.os.b + hq * a.os.h + r] = from_f32<T>(oh * inv);
                 if (a.lse && r == 0)
-                  a.lse[static_cast<int64_t>(it.b) * a.Hq + hq] = lt > 0.f ? (mn + log2f(lt)) * kLn2 : -INFINITY;
+                  a.lse[static_cast<int64_t>(it.b) * a.Hq + hq] = row_lse(mn, lt);
               } else {
                 float* pp = a.partial + ((static_cast<int64_t>(it.b) * a.Hq + hq) * a.nsplit + it.split) * (D + 2);
                 pp[r] = oh;
-                if (r == 0) pp[D] = lt > 0.f ? mn : -INFINITY, pp[D + 1] = lt;
+                if (r == 0) pp[D] = lt == 0.f ? -INFINITY : mn, pp[D + 1] = lt;
               }
             }
           }
