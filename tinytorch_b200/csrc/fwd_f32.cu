@@ -193,12 +193,12 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_f32_kernel(const FwdArgs a, i
 #pragma unroll
         for (int p = 0; p < kMost; ++p)
           if (p < cluster) ls += l[p] * exp2f(m[p] - ref);
-        const float inv = ls > 0.f ? 1.f / ls : 0.f;
+        const float inv = inverse_sum(ls);
 #pragma unroll
         for (int p = 0; p < kMost; ++p)
           if (p < cluster) weight[tid * kMost + p] = exp2f(m[p] - ref) * inv;
         if (lse && query_of(r) < a.Lq)
-          lse[static_cast<int64_t>(head_of(r)) * a.Lq + query_of(r)] = ls > 0.f ? (mx + log2f(ls)) * kLn2 : -INFINITY;
+          lse[static_cast<int64_t>(head_of(r)) * a.Lq + query_of(r)] = row_lse(mx, ls);
       }
       ptx::named_barrier(2, 256);
 #pragma unroll 1
@@ -350,9 +350,9 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_f32_kernel(const FwdArgs a, i
       if (l_row != l_row) ctl->bad = 1;  // (what is hidden may be anything)
       if (last_pass(careful)) break;
     }
-    stat[tid] = m_row, stat[BM + tid] = SPLIT ? l_row : (l_row > 0.f ? 1.f / l_row : 0.f);
+    stat[tid] = m_row, stat[BM + tid] = SPLIT ? l_row : inverse_sum(l_row);
     if (!SPLIT && lse && query_of(tid) < a.Lq)
-      lse[static_cast<int64_t>(head_of(tid)) * a.Lq + query_of(tid)] = l_row > 0.f ? (m_row + log2f(l_row)) * kLn2 : -INFINITY;
+      lse[static_cast<int64_t>(head_of(tid)) * a.Lq + query_of(tid)] = row_lse(m_row, l_row);
     write_out();
   } else if (warp < 8) {
     // ------------------------------------------------------------------------------------------------------ O --
