@@ -53,9 +53,7 @@ def run(shape, D, dtype, how, poisoned, at, value, where):
     if poisoned == "v":  # (who does not see it may meet it in a tile, as 0 times what it holds)
         met = ~o[b, :group].isfinite()
         assert bool((met if where == "all" else met[..., 5:6])[:, sees[:, at]].all())
-        assert not lse[b].isnan().any()
-        if dtype != torch.float32:
-            assert not o[b, :, ~sees.any(1)].any()
+        assert not o[b, :, ~sees.any(1)].any() and not lse[b].isnan().any()
         return
     assert want[0].isnan().any() or value == -math.inf or not sees[:, at].any()
     nf.agree(o[b], lse[b], want[0], want[1], want[2], vv, dtype)

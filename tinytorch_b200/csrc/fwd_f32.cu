@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_f32_kernel(const FwdArgs a, i
         const float inv = inverse_sum(ls);
 #pragma unroll
         for (int p = 0; p < kMost; ++p)
-          if (p < cluster) weight[tid * kMost + p] = exp2f(m[p] - ref) * inv;
+          if (p < cluster) weight[tid * kMost + p] = ls == 0.f ? -1.f : exp2f(m[p] - ref) * inv;  // (-1: no key, 0 whatever the values are)
         if (lse && query_of(r) < a.Lq)
           lse[static_cast<int64_t>(head_of(r)) * a.Lq + query_of(r)] = row_lse(mx, ls);
       }
@@ -211,6 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_f32_kernel(const FwdArgs a, i
         for (int p = 0; p < kMost; ++p)
           if (p < cluster) {
             const float w = weight[r * kMost + p];
+            if (w == -1.f) continue;
             sum.x = fmaf(x[p].x, w, sum.x), sum.y = fmaf(x[p].y, w, sum.y), sum.z = fmaf(x[p].z, w, sum.z), sum.w = fmaf(x[p].w, w, sum.w);
           }
         store(first + r, d, sum);
@@ -222,7 +223,8 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_f32_kernel(const FwdArgs a, i
       for (int r = tid / (D / 4); r < BM; r += kStep) {
         const float4 x = *reinterpret_cast<const float4*>(out_s + r * LY::kLdO + d);
         const float inv = stat[BM + r];
-        store(r, d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+        // (no key: 0, whatever the values are)
+        store(r, d, inv == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
       }
     }
     if (tid == 0 && *abort_flag && a.status) atomicOr(a.status, kStatusWaitExpired);
