@@ -563,7 +563,7 @@ void check_packed_bwd(const Tensor& dO, const Tensor& q, const Tensor& o, const 
     raise(PyExc_ValueError, "lse must be a contiguous float32 tensor [Hq, rows] on the device of q");
 }
 BwdResult packed_bwd(const Tensor& dO, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse, const Packed& s,
-                     const bool (&needs)[3]) {
+                     const bool (&needs)[3], const Tensor& status) {
   BwdResult r;
   const Tensor* like[3] = {&q, &k, &v};
   const bool nothing = q.numel() == 0 || k.numel() == 0;
@@ -574,7 +574,7 @@ BwdResult packed_bwd(const Tensor& dO, const Tensor& q, const Tensor& k, const T
   }
   if (nothing) return r;
   tt_attn_packed_bwd_params p{};
-  set_packed(&p, q, k, v, s, Tensor());
+  set_packed(&p, q, k, v, s, status);
   p.o = o.data_ptr(), p.d_o = dO.data_ptr(), p.lse = static_cast<const float*>(lse.data_ptr());
   p.o_strides = packed_strides_of(o), p.do_strides = packed_strides_of(dO);
   void** out[3] = {&p.dq, &p.dk, &p.dv};
@@ -585,15 +585,18 @@ BwdResult packed_bwd(const Tensor& dO, const Tensor& q, const Tensor& k, const T
   return r;
 }
 
-// As AttentionBackward.  The offsets are saved like the operands: changing them in place between the two passes is an error.
+// As AttentionBackward.  The offsets are saved like the operands: changing them in place between the two passes is an error.  The status word is the
+// caller's memory, in which both passes set bits.
 struct PackedBackward : public torch::autograd::Node {
   SavedVariable q, k, v, o, lse, cu_q, cu_k;
+  Tensor status;
   int mode;
   float scale;
   std::string name() const override { return "FuncSDPAttentionPackedBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
     q.reset_data(), k.reset_data(), v.reset_data(), o.reset_data(), lse.reset_data(), cu_q.reset_data(), cu_k.reset_data();
+    status.reset();
   }
   variable_list apply(variable_list&& grads) override {
     variable_list out(3);
@@ -606,7 +609,7 @@ struct PackedBackward : public torch::autograd::Node {
     check_packed(qt, kt, vt, s);
     check_packed_bwd(dO, qt, ot, lt);
     const bool needs[3] = {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2)};
-    BwdResult r = packed_bwd(dO, qt, kt, vt, ot, lt, s, needs);
+    BwdResult r = packed_bwd(dO, qt, kt, vt, ot, lt, s, needs, status);
     for (int i = 0; i < 3; ++i) out[i] = std::move(r.g[i]);
     return out;
   }
@@ -1093,26 +1096,28 @@ PyObject* py_linear_raw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// sdp_attention_packed(q, k, v, cuSeqlens, cuSeqlensK, mode, scale) -> O; NotImplemented as sdp_attention
+// sdp_attention_packed(q, k, v, cuSeqlens, cuSeqlensK, mode, scale, status) -> O; NotImplemented as sdp_attention
 PyObject* py_sdp_attention_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  expect(n, 7);
+  expect(n, 8);
   const Tensor &q = tensor_of(a[0], "q"), &k = tensor_of(a[1], "k"), &v = tensor_of(a[2], "v");
   if (needs_python_function({&q, &k, &v})) Py_RETURN_NOTIMPLEMENTED;
   const bool grad = wants_grad(q, k, v);
   if (q.dim() != 3) raise(PyExc_ValueError, "q must be [rows, H, D]");
   const Packed s{tensor_of(a[3], "cuSeqlens"), optional_of(a[4], "cuSeqlensK"), int_arg(a[5]), scale_or_default(scale_arg(a[6]), q.size(2))};
+  const Tensor status = optional_of(a[7], "status");
   check_packed(q, k, v, s);
+  check_ints(status, "status", 1, q);
   FwdResult r;
   {
     NoGil nogil;
-    r = packed_fwd(q, k, v, s, grad, Tensor());
+    r = packed_fwd(q, k, v, s, grad, status);
     if (grad) {
       auto node = std::shared_ptr<PackedBackward>(new PackedBackward(), torch::autograd::deleteNode);
       node->set_next_edges(torch::autograd::collect_next_edges(q, k, v));
       node->q = SavedVariable(q, false), node->k = SavedVariable(k, false), node->v = SavedVariable(v, false);
       node->lse = SavedVariable(r.lse, false), node->cu_q = SavedVariable(s.cu_q, false), node->cu_k = SavedVariable(s.cu_k, false);
-      node->mode = s.mode, node->scale = s.scale;
+      node->status = same_memory(status), node->mode = s.mode, node->scale = s.scale;
       torch::autograd::set_history(r.o, node);
       node->o = SavedVariable(r.o, true);
     }
@@ -1141,14 +1146,16 @@ PyObject* py_packed_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// packed_bwd(dO, q, k, v, o, lse, cuSeqlens, cuSeqlensK, mode, scale, need_dq, need_dk, need_dv) -> (dQ, dK, dV), None where not needed
+// packed_bwd(dO, q, k, v, o, lse, cuSeqlens, cuSeqlensK, mode, scale, need_dq, need_dk, need_dv, status) -> (dQ, dK, dV), None where not needed
 PyObject* py_packed_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  expect(n, 13);
+  expect(n, 14);
   const Tensor &q = tensor_of(a[1], "q"), &k = tensor_of(a[2], "k"), &v = tensor_of(a[3], "v"), &o = tensor_of(a[4], "o"), &lse = tensor_of(a[5], "lse");
   if (q.dim() != 3) raise(PyExc_ValueError, "q must be [rows, H, D]");
   const Packed s{tensor_of(a[6], "cuSeqlens"), optional_of(a[7], "cuSeqlensK"), int_arg(a[8]), scale_or_default(scale_arg(a[9]), q.size(2))};
+  const Tensor status = optional_of(a[13], "status");
   check_packed(q, k, v, s);
+  check_ints(status, "status", 1, q);
   Tensor dO = tensor_of(a[0], "dO");
   if (dO.dim() == 3 && dO.is_cuda()) dO = readable(dO);
   check_packed_bwd(dO, q, o, lse);
@@ -1157,7 +1164,7 @@ PyObject* py_packed_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   {
     NoGil nogil;
     at::NoGradGuard no_grad;
-    r = packed_bwd(dO, q, k, v, o, lse, s, needs);
+    r = packed_bwd(dO, q, k, v, o, lse, s, needs, status);
   }
   return tuple_of({&r.g[0], &r.g[1], &r.g[2]});
   END_HANDLE_TH_ERRORS

@@ -54,35 +54,38 @@ class FuncSDPAttentionPacked(torch.autograd.Function):
     """As FuncSDPAttention, for packed sequences (the native node is PackedBackward)."""
 
     @staticmethod
-    def forward(ctx, query, key, value, cuSeqlens, cuSeqlensK, isCausal, scale):
+    def forward(ctx, query, key, value, cuSeqlens, cuSeqlensK, isCausal, scale, status=None):
         needs_grad = any(ctx.needs_input_grad[:3])
-        o, lse = op.sdpAttentionPackedFwd(query, key, value, cuSeqlens, isCausal, scale, cuSeqlensK, needLse=needs_grad)
+        o, lse = op.sdpAttentionPackedFwd(query, key, value, cuSeqlens, isCausal, scale, cuSeqlensK, needLse=needs_grad, status=status)
         if needs_grad:
             ctx.save_for_backward(query, key, value, o, lse, cuSeqlens, cuSeqlensK)
-            ctx.isCausal, ctx.scale = isCausal, scale
+            ctx.isCausal, ctx.scale, ctx.status = isCausal, scale, status
         return o
 
     @staticmethod
     def backward(ctx, grad):
         query, key, value, o, lse, cuSeqlens, cuSeqlensK = ctx.saved_tensors
         dq, dk, dv = op.sdpAttentionPackedBwd(grad, query, key, value, o, lse, cuSeqlens, ctx.isCausal, ctx.scale, cuSeqlensK,
-                                              needs=ctx.needs_input_grad[:3])
-        return dq, dk, dv, None, None, None, None
+                                              needs=ctx.needs_input_grad[:3], status=ctx.status)
+        return dq, dk, dv, None, None, None, None, None
 
 
-def sdpAttentionPacked(query, key, value, cuSeqlens, isCausal=False, scale=None, cuSeqlensK=None):
+def sdpAttentionPacked(query, key, value, cuSeqlens, isCausal=False, scale=None, cuSeqlensK=None, status=None):
     """Attention over sequences packed behind one another without padding, differentiable: query [rows, Hq, D], key and
     value [rows, Hkv, D], float16 / bfloat16; sequence n is the rows cuSeqlens[n] to cuSeqlens[n + 1] (int32 [N + 1] on the device).
 
     With cuSeqlensK keys have lengths of their own, and isCausal="bottom-right" aligns each sequence's queries to the end of its
     keys.  Sequences may be empty; rows of no sequence (behind the last, say) give O = 0 and zero gradients.  The reference has padded
-    batches only; each sequence here is what sdpAttention makes of it alone."""
+    batches only; each sequence here is what sdpAttention makes of it alone.
+
+    Offsets that fall, are negative or lie beyond the rows give zeros and zero gradients, and set bit 16 of status (int32 [1]), if there
+    is one, in both passes; its bit 1 stands for a device-side wait that expired."""
     if not isinstance(isCausal, str):
         isCausal = bool(isCausal)
-    o = _capi.native().sdp_attention_packed(query, key, value, cuSeqlens, cuSeqlensK, op._causal_mode(isCausal), scale)
+    o = _capi.native().sdp_attention_packed(query, key, value, cuSeqlens, cuSeqlensK, op._causal_mode(isCausal), scale, status)
     if o is NotImplemented:
         scale = op.default_scale(query.shape[-1]) if scale is None else float(scale)
-        o = FuncSDPAttentionPacked.apply(query, key, value, cuSeqlens, cuSeqlensK, isCausal, scale)
+        o = FuncSDPAttentionPacked.apply(query, key, value, cuSeqlens, cuSeqlensK, isCausal, scale, status)
     return o
 
 

@@ -57,10 +57,10 @@ def sdpAttentionPackedFwd(q, k, v, cuSeqlens, isCausal=False, scale=None, cuSeql
     return _capi.native().packed_fwd(q, k, v, cuSeqlens, cuSeqlensK, _causal_mode(isCausal), scale, needLse, status)
 
 
-def sdpAttentionPackedBwd(dO, q, k, v, o, lse, cuSeqlens, isCausal=False, scale=None, cuSeqlensK=None, needs=(True, True, True)):
-    """Gradients (dQ, dK, dV); entries of `needs` that are False come back as None."""
+def sdpAttentionPackedBwd(dO, q, k, v, o, lse, cuSeqlens, isCausal=False, scale=None, cuSeqlensK=None, needs=(True, True, True), status=None):
+    """Gradients (dQ, dK, dV); entries of `needs` that are False come back as None; status as in the forward."""
     return _capi.native().packed_bwd(dO, q, k, v, o, lse, cuSeqlens, cuSeqlensK, _causal_mode(isCausal), scale, needs[0], needs[1],
-                                     needs[2])
+                                     needs[2], status)
 
 
 def sdpAttentionDecode(q, kCache, vCache, kvLens=None, scale=None, needLse=False, workspace=None):
