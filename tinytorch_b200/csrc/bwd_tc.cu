@@ -1595,10 +1595,10 @@ cudaError_t launch_packed(BwdArgs a, const PackedCall& c, int dtype, int device,
   const Str3* st[kPackedBwdMaps] = {&a.qs, &a.ks, &a.vs, &a.dos, &accum, a.dk ? &a.dks : &a.ks, a.dv ? &a.dvs : &a.vs};
   for (int m = 0; m < kPackedBwdMaps; ++m) {
     const bool of_k = m == kMapK || m == kMapV || m == kMapdK || m == kMapdV;
-    const bool made = m == kMapdQ ? packed_map(&p, &maps, TT_ATTN_F32, a.dq_accum, D, a.Lq, a.Hq, accum, D == 64 ? 32 : 128, false, D == 64 ? 0 : heads)
+    cudaError_t e = m == kMapdQ ? packed_map(&p, &maps, TT_ATTN_F32, a.dq_accum, D, a.Lq, a.Hq, accum, D == 64 ? 32 : 128, false, D == 64 ? 0 : heads)
                                   : packed_map(&p, &maps, dtype, ptr[m], D, of_k ? a.Skv : a.Lq, of_k ? a.Hkv : a.Hq, *st[m],
                                                m == kMapdK || m == kMapdV ? kOutRows : 128, of_k, of_k ? 0 : heads);
-    if (!made) return cudaErrorInvalidValue;
+    if (e != cudaSuccess) return e;
   }
   if (a.dk) p.zero[p.n_zero++] = PackedPlan::Rows{static_cast<char*>(a.dk), a.dks.s * 2, a.dks.h * 2, a.Hkv, D * 2, true};
   if (a.dv) p.zero[p.n_zero++] = PackedPlan::Rows{static_cast<char*>(a.dv), a.dvs.s * 2, a.dvs.h * 2, a.Hkv, D * 2, true};

@@ -1247,7 +1247,8 @@ cudaError_t launch_packed(FwdArgs a, const PackedCall& c, int dtype, int device,
   const Str3* st[kPackedFwdMaps] = {&a.qs, &a.ks, &a.vs, &a.os};
   for (int m = 0; m < kPackedFwdMaps; ++m) {
     const bool of_k = m == kMapK || m == kMapV;
-    if (!packed_map(&p, &maps, dtype, ptr[m], D, of_k ? a.Skv : a.Lq, of_k ? a.Hkv : a.Hq, *st[m], 128, of_k, narrow > 0 ? (of_k ? 1 : heads) : 0)) return cudaErrorInvalidValue;
+    cudaError_t e = packed_map(&p, &maps, dtype, ptr[m], D, of_k ? a.Skv : a.Lq, of_k ? a.Hkv : a.Hq, *st[m], 128, of_k, narrow > 0 ? (of_k ? 1 : heads) : 0);
+    if (e != cudaSuccess) return e;
   }
   p.zero[0] = PackedPlan::Rows{static_cast<char*>(a.o), a.os.s * 2, a.os.h * 2, a.Hq, D * 2, false};
   p.n_zero = 1, p.lse = a.lse;

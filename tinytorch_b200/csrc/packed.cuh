@@ -71,7 +71,7 @@ int packed_slots(int n, int total_q, int total_k, int Hq, int Hkv);
 
 // Adds the map of an operand [rows][H][D] (fp32: dense [H][rows][D]).
 // narrow_heads: also one with boxes of p->narrow rows of so many heads.
-bool packed_map(PackedPlan* p, PackedMaps* maps, int dtype, const void* ptr, int D, int rows, int H, const Str3& st, int box_rows, bool of_k, int narrow_heads = 0);
+cudaError_t packed_map(PackedPlan* p, PackedMaps* maps, int dtype, const void* ptr, int D, int rows, int H, const Str3& st, int box_rows, bool of_k, int narrow_heads = 0);
 
 // Fills in items, maps and args from `scratch` and enqueues the planning kernel.
 cudaError_t launch_packed_plan(PackedPlan p, const PackedMaps& maps, void* scratch, PackedArgs* args, cudaStream_t stream);

@@ -15,6 +15,7 @@
 // 4096, 8/2 heads 365 -> 156; divided without need, 2 x 1000 rows of 16 heads take 72 us instead of 50.
 #include <type_traits>
 
+#include "map_kind.h"
 #include "packed.cuh"
 
 #include "ptx.cuh"
@@ -253,18 +254,7 @@ constexpr size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
 }  // namespace
 
-namespace {
-
-// Whether two maps of the same memory differ in nothing but the number of rows (which lies in one of their words).
-bool same_kind(const CUtensorMap& a, const CUtensorMap& b) {
-  int differ = 0;
-  for (size_t i = 0; i < sizeof(a.opaque) / sizeof(a.opaque[0]); ++i) differ += a.opaque[i] != b.opaque[i];
-  return differ <= 1;
-}
-
-}  // namespace
-
-bool packed_map(PackedPlan* p, PackedMaps* maps, int dtype, const void* ptr, int D, int rows, int H, const Str3& st, int box_rows, bool of_k, int narrow_heads) {
+cudaError_t packed_map(PackedPlan* p, PackedMaps* maps, int dtype, const void* ptr, int D, int rows, int H, const Str3& st, int box_rows, bool of_k, int narrow_heads) {
   const int m = p->n_maps++;
   const int64_t es = dtype == TT_ATTN_F32 ? 4 : 2;
   const int whole_rows = box_rows;
@@ -274,39 +264,24 @@ bool packed_map(PackedPlan* p, PackedMaps* maps, int dtype, const void* ptr, int
                                 : make_map(map, dtype, ptr, D, n, H, 1, st, box_rows, 64, box_heads);
   };
   p->address[m] = static_cast<const char*>(ptr), p->row_bytes[m] = st.s * es, p->of_k[m] = of_k;
-  if (!encode(&maps->kind[0][m], rows) || !encode(&maps->kind[1][m], 1)) return false;
+  if (!encode(&maps->kind[0][m], rows) || !encode(&maps->kind[1][m], 1)) return cudaErrorInvalidValue;
   p->has_narrow[m] = p->narrow > 0 && narrow_heads > 0;
   if (p->has_narrow[m]) {
     box_rows = p->narrow, box_heads = narrow_heads;
-    if (!encode(&maps->kind[2][m], rows) || !encode(&maps->kind[3][m], 1)) return false;
+    if (!encode(&maps->kind[2][m], rows) || !encode(&maps->kind[3][m], 1)) return cudaErrorInvalidValue;
     box_rows = whole_rows, box_heads = 1;
-  }
-  if (same_kind(maps->kind[0][m], maps->kind[1][m])) {
-    p->long_rows[m] = 1;
-    return true;
   }
   for (int i = 0; i < m; ++i)  // (a tensor of the same layout has been looked at: V as K, O as Q)
     if (dtype != TT_ATTN_F32 && maps->layout[i].rows == rows && maps->layout[i].heads == H && maps->layout[i].row_stride == st.s && maps->layout[i].head_stride == st.h) {
       p->long_rows[m] = p->long_rows[i];
-      return true;
+      return cudaSuccess;
     }
   if (dtype != TT_ATTN_F32) maps->layout[m] = PackedMaps::Layout{rows, H, st.s, st.h};
-  // The fewest rows that count as long: those that reach over 128 KB; should a driver see it otherwise, they are searched for.
+  // The fewest rows that count as long: those that reach over 128 KB, as a rule.
   const int64_t first = static_cast<int64_t>(H - 1) * st.h * es + D * es, more = (int64_t(128) << 10) - first;
-  int64_t n = 1 + (more > 0 ? (more + st.s * es - 1) / (st.s * es) : 0);
-  CUtensorMap at, below;
-  if (n < 2 || n > rows || !encode(&at, static_cast<int>(n)) || !encode(&below, static_cast<int>(n - 1)) || !same_kind(at, maps->kind[0][m]) ||
-      same_kind(below, maps->kind[0][m])) {
-    int64_t lo = 1, hi = rows;
-    while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) / 2;
-      if (!encode(&at, static_cast<int>(mid))) return false;
-      (same_kind(at, maps->kind[0][m]) ? hi : lo) = mid;
-    }
-    n = hi;
-  }
-  p->long_rows[m] = static_cast<int>(n);
-  return true;
+  const int64_t n = 1 + (more > 0 ? (more + st.s * es - 1) / (st.s * es) : 0);
+  const MapKinds found = long_rows<CUtensorMap>(encode, rows, n, maps->kind[0][m], maps->kind[1][m], &p->long_rows[m]);
+  return found == MapKinds::kFound ? cudaSuccess : (found == MapKinds::kNotEncoded ? cudaErrorInvalidValue : cudaErrorNotSupported);
 }
 
 // Every sequence has at most one item more than its rows fill.
