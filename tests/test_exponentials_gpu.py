@@ -57,3 +57,23 @@ def test_hidden_pairs_give_nothing_to_gradients(dtype, D):
     assert not dk[:, :, hidden].any() and not dv[:, :, hidden].any()
     scaled = torch.autograd.grad(function.sdpAttention(q, k, v, attnMask=mask), v, torch.full((B, H, L, D), big, dtype=dtype, device="cuda"))[0]
     assert not scaled[:, :, hidden].any()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("causal", [False, True])
+def test_hidden_values_give_nothing(D, shape, causal):
+    """The largest values of bf16 behind hidden keys of every column, of a mask or beyond the triangle, leave not a bit."""
+    from tinytorch_b200 import op
+    B, H, L, S = shape
+    q, k, v = (randn((B, H, n, D), torch.bfloat16, i) for i, n in enumerate((L, S, S)))
+    if causal:
+        kw, rows, hidden = dict(isCausal=True), slice(0, 30), torch.arange(S, device="cuda") >= 30
+    else:
+        hidden = torch.arange(S, device="cuda") % 3 == 1
+        mask = (~hidden).expand(L, S).clone()
+        mask[0, 2] = False  # (not one that comes down to a length)
+        kw, rows = dict(attnMask=mask), slice(0, L)
+    want = op.sdpAttentionFwd(q, k, v.masked_fill(hidden[:, None], 0.0), **kw)
+    got = op.sdpAttentionFwd(q, k, v.masked_fill(hidden[:, None], 3e38), **kw)
+    assert torch.equal(got[0][:, :, rows], want[0][:, :, rows]) and torch.equal(got[1], want[1])

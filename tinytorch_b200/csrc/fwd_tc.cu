@@ -907,7 +907,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float m_use = (GEN && m_ref == -INFINITY) ? 0.f : m_ref;
           const float2 nm2 = make_float2(-m_use, -m_use);
           float2 lt = make_float2(0.f, 0.f);
-          float fma_max = -INFINITY;  // of the exponents on the FMA pipe
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
             uint32_t pk[32];
@@ -915,9 +914,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e0 = 0; e0 < 64; e0 += 32) {
               const float2 x0 = exponents(hf * 64 + e0), x16 = exponents(hf * 64 + e0 + 16);
-              // (D = 64, where the exponentials and not the MMAs set the pace: one in sixteen on the FMA pipe)
+              // (D = 64, where the exponentials and not the MMAs set the pace: one in sixteen on the FMA pipe; huge or NaN, they are so in the sum, too)
               float2 on_fma = make_float2(0.f, 0.f);
-              if (D == 64) on_fma = ptx::ex2_fma2<false>(make_float2(x0.y, x16.y)), fma_max = ptx::max3_nan(fma_max, x0.y, x16.y);
+              if (D == 64) on_fma = ptx::ex2_fma2<false>(make_float2(x0.y, x16.y));
 #pragma unroll
               for (int e2 = e0; e2 < e0 + 32; e2 += 2) {
                 const float2 x = e2 == e0 ? x0 : (e2 == e0 + 16 ? x16 : exponents(hf * 64 + e2));
@@ -928,9 +927,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             ptx::tmem_st32(tS + hf * 32, pk);
           }
-          // (one of those far above the reference, or NaN: as the other exponentials then are.  This check, not a clamp of each:
-          // 4 x 16 heads x 2048, causal, 59.1 us without either, 60.1, 61.1)
-          if (D == 64 && !(fma_max <= 127.f)) lt.x = __uint_as_float(0x7fffffffu);
           const float tile_sum = lt.x + lt.y;
           // redo with a fresh maximum if any row of the warp needs it (tcgen05.ld /
           // .st are warp-collective, so the warp decides together)
@@ -1035,7 +1031,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int cc = 0; cc < D / 32; ++cc) ptx::tmem_ld32p(tO + cc * 32, s + cc * 32);
       ptx::tmem_wait_ld();
-      const float l = l2.x + l2.y, inv = inverse_sum(l);
+      // (of a row without a key the exponentials on the FMA pipe, D = 64, have left denormals in the sum)
+      const float sum = l2.x + l2.y, l = GEN && m_ref == -INFINITY && sum == sum ? 0.f : sum, inv = inverse_sum(l);
       if (GEN && l == 0.f) {  // (no key: 0, whatever the values are)
 #pragma unroll
         for (int e = 0; e < D; ++e) s[e] = 0;

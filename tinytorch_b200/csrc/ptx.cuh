@@ -517,12 +517,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// ... NaN if one of them is
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
 
 // One lane of a converged warp.  A loop that issues tcgen05.mma is run by the whole warp with only the
 // instruction itself under this predicate: addresses and descriptors then stay warp-uniform (uniform registers and
@@ -576,17 +570,19 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // 2^x of a pair on the FMA and integer pipes (no MUFU): x = n + f with n = round(x), f in [-0.5, 0.5]; a cubic for 2^f
-// (maximum relative error 7.5e-5, below half a unit in the last place of fp16 and bf16) times 2^n, whose bits are n + 127
-// in the exponent field.  0 below -126.5 (-inf included).  ANY: as ex2 at the other end, too, infinite above 127.5 and NaN for NaN;
-// without it whoever calls looks for arguments above 127 and NaN, which give anything.  For kernels whose
-// exponentials are bound by the four MUFU units of an SM sub-partition: a share of them goes here.
-template <bool ANY>
+// (maximum relative error 7.5e-5, below half a unit in the last place of fp16 and bf16) and n added to the exponent field.  For kernels
+// whose exponentials are bound by the four MUFU units of an SM sub-partition: a share of them goes here.
+// ENDS: 0 below -126.5 (-inf included), infinite above 127.5, NaN for NaN, as ex2: 2^n is a factor then.
+// Without: NaN for NaN and above 128.5 (the exponent field of 129 and any mantissa), and below -127 the least that can be had: where the cubic has
+// just passed 1, n = -127 leaves its last bits, 18 x 2^-149, which is 0 in 16 bits (but not in a sum).
+template <bool ENDS>
 __device__ __forceinline__ float2 ex2_fma2(float2 x) {
-  if constexpr (ANY) {
+  if constexpr (ENDS) {
     asm("max.NaN.f32 %0, %0, %2;\n\tmax.NaN.f32 %1, %1, %2;" : "+f"(x.x), "+f"(x.y) : "f"(-127.f));
     asm("min.NaN.f32 %0, %0, %2;\n\tmin.NaN.f32 %1, %1, %2;" : "+f"(x.x), "+f"(x.y) : "f"(128.f));
   } else {
-    x.x = fmaxf(x.x, -127.f), x.y = fmaxf(x.y, -127.f);
+    constexpr float least = -126.99989318847656f;
+    x.x = fmaxf(fminf(x.x, 129.f), least), x.y = fmaxf(fminf(x.y, 129.f), least);
   }
   auto both = [](float c) { return make_float2(c, c); };
   constexpr float magic = 12582912.f;  // 1.5 * 2^23: the sum holds round(x) in its low mantissa bits
@@ -594,8 +590,9 @@ __device__ __forceinline__ float2 ex2_fma2(float2 x) {
   const float2 f = fma2(add2(xr, both(-magic)), both(-1.f), x);
   const float2 p = fma2(fma2(fma2(both(0.055171750485897064f), f, both(0.24261131882667542f)), f, both(0.6932609677314758f)), f,
                         both(0.9999280571937561f));
-  auto power = [](float r) { return __uint_as_float((__float_as_uint(r) << 23) + 0x3f800000u); };
-  return mul2(p, make_float2(power(xr.x), power(xr.y)));
+  auto shifted = [](float r) { return __float_as_uint(r) << 23; };
+  if constexpr (ENDS) return mul2(p, make_float2(__uint_as_float(shifted(xr.x) + 0x3f800000u), __uint_as_float(shifted(xr.y) + 0x3f800000u)));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + shifted(xr.x)), __uint_as_float(__float_as_uint(p.y) + shifted(xr.y)));
 }
 
 }  // namespace ptx
