@@ -37,7 +37,8 @@
  *    rows at or beyond the length are never used in the result, but must hold
  *    finite values in the prefill path (they may be multiplied by an exact 0).
  *  - A query row with no participating key yields O = 0 and LSE = -inf (the
- *    reference yields NaN there, src/Operation/OpNNLayerCpu.h:28-54).
+ *    reference yields NaN there, src/Operation/OpNNLayerCpu.h:28-54).  A row with
+ *    a score that is NaN or +inf yields NaN in both, as in the reference.
  *  - Grouped-query attention: Hq must be a multiple of Hkv; query head h reads
  *    kv head h / (Hq/Hkv), which equals op::repeatInterleave(kv, group, 1)
  *    (src/Operation/OpTransformCpu.h:399-442) without materialising the copy.

@@ -38,7 +38,8 @@
 //                       the next item's first QK.
 // P never leaves TMEM: the second MMA takes its A operand from TMEM.
 // PACKED: sequences behind one another; the items and a set of tensor maps for every sequence come from packed_plan.cu, so that the loops are the same.
-// 12 prompts of 1 to 4096 rows, 32/8 heads, D = 128, bf16: 305 us (1097 TFLOP/s, as unpacked); five of 677 rows: 15.5 us, most of it latency.
+// 12 prompts of 1 to 4096 rows, 32/8 heads, D = 128, bf16: 363 us pass after pass (920 TFLOP/s; 305 in a burst too short for the power limit, as unpacked);
+// five of 677 rows: 15.6 us, most of it latency.
 // Every mbarrier wait is bounded; an expired wait sets the status word and makes
 // the CTA unwind.
 #include <cuda.h>

@@ -9,8 +9,9 @@
 // with one rounding to the tensor type of each value stored.
 //
 // Bound by memory: x in and y out (backward: x and dy in, dx out), and next to that by instructions (262 and 362 a chunk of 2 KB in and out, 3 KB
-// backward).  8200 tokens of 32/8 heads, D = 128, bf16: forward 29 us (5.8 TB/s), backward 52 us (4.9 TB/s); 4000 tokens of 40/8, D = 64, fp32: 15
-// (6.4) and 32 us (4.6).  A row of D channels belongs to D / 16
+// backward), which set the pace at D = 64 in 16 bits and in the fp32 backward.  In a loop, whose inputs are partly in L2: 8200 tokens of 32/8 heads, D = 128, bf16: forward 29 us (5.8
+// TB/s; 172 MB that are not there 31.7, 5.4), backward 52 us (4.9 TB/s); 8192 of 16/16, D = 64, fp16: 13 (5.2) and 25 us (4.0); 4000 of 40/8, D = 64, fp32: 14
+// (6.9) and 32 us (4.6).  A row of D channels belongs to D / 16
 // neighbouring lanes, each with 8 channels of the first half and the same 8 of the second, so that a pair (i, i + D/2) or
 // (2i, 2i + 1) never leaves a thread, every access is a 16-byte vector of a 64- or 128-byte run, and the means take two or
 // three shuffles; the arithmetic is in packed pairs.  A warp takes 512 / D heads of one token at a time (a chunk), and an equal,
@@ -541,10 +542,11 @@ cudaError_t launch(int dtype, int D, const NormRopeArgs& a, int device, cudaStre
 
 }  // namespace
 
-// CTAs of the backward for q and k, by their heads: as many as are resident at once, or fewer for little work.
+// CTAs of the backward for q and k, by their heads: as many as are resident at once, or fewer for little work.  (A token's chunk costs a warp the same
+// whether its heads fill it or not: one kv head at D = 64, where a chunk is eight, gets an eighth of q's CTAs and as many chunks: 56 us for 8192 tokens of 8/1 heads.)
 void norm_rope_bwd_ctas(int B, int S, const int (&heads)[2], int (&ctas)[2]) {
   const int64_t rows = static_cast<int64_t>(B) * S * (heads[0] + heads[1]);
-  int64_t all = (rows + 4 * kWarps - 1) / (4 * kWarps);  // (no fewer than four rows to a warp: a chunk)
+  int64_t all = (rows + 4 * kWarps - 1) / (4 * kWarps);  // (no fewer than four rows to a warp: a chunk at D = 128, half of one at D = 64)
   if (all > kBwdCtas * kSms) all = kBwdCtas * kSms;
   if (all < 2) all = 2;
   ctas[1] = static_cast<int>(all * heads[1] / (heads[0] + heads[1]));
